@@ -31,6 +31,7 @@
 #define LUX_GPU_QUANT_BACKEND_H
 
 #include "lux_gpu_backend_abi.h"
+#include "lux_gpu_serving_backend.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -163,7 +164,11 @@ typedef struct lux_gpu_quant_vtbl {
     /* frees the buffers linear_load allocated and zeroes *layer */
     void (*linear_free)(LuxBackendContext* ctx, lux_quant_linear* layer);
 
-    void* _reserved[4];
+    /* the operators of a decoding step (lux_gpu_serving_backend.h); NULL in
+     * plugins that predate them */
+    const lux_gpu_serving_vtbl* serving;
+
+    void* _reserved[3];
 } lux_gpu_quant_vtbl;
 
 /* layout pins: LP64 */

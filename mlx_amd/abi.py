@@ -158,6 +158,68 @@ LINEAR_LOAD = C.CFUNCTYPE(Err, Ctx, C.c_char_p, C.c_char_p, _I, _I, C.POINTER(Li
 LINEAR_FREE = C.CFUNCTYPE(None, Ctx, C.POINTER(Linear))
 
 
+# the decoding step's operators (include/lux_gpu_serving_backend.h)
+SERVING_EXT_VERSION = 1
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3
+
+
+class _Args(C.Structure):
+    """An argument record; keyword arguments fill its fields, the rest is 0 / NULL."""
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(type(self))
+
+
+def _fields(ints, floats, longs, bufs, pad=()):
+    return ([("struct_size", C.c_uint32)] + [(n, C.c_int32) for n in ints] + [(n, C.c_float) for n in floats]
+            + [(n, C.c_int32) for n in pad] + [(n, C.c_int64) for n in longs] + [(n, Buf) for n in bufs])
+
+
+class PagedPlanArgs(_Args):
+    """lux_paged_plan_args."""
+    _fields_ = _fields(["requests", "max_tokens", "max_pages", "page_size", "num_pages", "free_count"], [], [],
+                       ["seq_lens", "new_lens", "free_pages", "free_head", "block_table", "slots", "positions",
+                        "token_request", "token_starts", "kv_lens", "counts"], pad=["_pad"])
+
+
+class PagedAppendArgs(_Args):
+    """lux_paged_append_args."""
+    _fields_ = _fields(["tokens", "kv_heads", "head_dim", "page_size", "num_pages", "in_dtype", "cache_dtype"], [],
+                       ["k_offset", "k_row_stride", "v_offset", "v_row_stride"], ["k", "v", "slots", "k_cache", "v_cache"])
+
+
+class PagedAttentionArgs(_Args):
+    """lux_paged_attention_args."""
+    _fields_ = _fields(["requests", "heads", "kv_heads", "head_dim", "page_size", "num_pages", "max_pages", "window",
+                        "dtype"], ["scale", "softcap"], ["q_offset", "q_row_stride", "out_offset", "out_row_stride"],
+                       ["q", "k_cache", "v_cache", "block_table", "kv_lens", "out", "lse"])
+
+
+class BlockNormArgs(_Args):
+    """lux_block_norm_args."""
+    _fields_ = _fields(["rows", "dim", "post_norm", "pre_norm", "gate_mode", "x_dtype", "residual_dtype", "weight_dtype"],
+                       ["residual_scale", "eps"],
+                       ["x_row_stride", "residual_row_stride", "gate_row_stride", "residual_out_row_stride",
+                        "out_row_stride"],
+                       ["x", "residual", "post_weight", "post_bias", "gate", "pre_weight", "pre_bias", "residual_out",
+                        "out"], pad=["_pad"])
+
+
+class ServingVtbl(C.Structure):
+    _fields_ = [
+        ("ext_version", C.c_uint32),
+        ("struct_size", C.c_uint32),
+        ("op_paged_plan", C.CFUNCTYPE(Err, Ctx, C.POINTER(PagedPlanArgs))),
+        ("op_paged_append", C.CFUNCTYPE(Err, Ctx, C.POINTER(PagedAppendArgs))),
+        ("op_paged_attention", C.CFUNCTYPE(Err, Ctx, C.POINTER(PagedAttentionArgs))),
+        ("op_block_norm", C.CFUNCTYPE(Err, Ctx, C.POINTER(BlockNormArgs))),
+        ("buffer_wrap", C.CFUNCTYPE(Buf, Ctx, C.c_void_p, C.c_size_t)),
+        ("_reserved", C.c_void_p * 5),
+    ]
+
+
 class QuantVtbl(C.Structure):
     _fields_ = [
         ("ext_version", C.c_uint32),
@@ -172,7 +234,8 @@ class QuantVtbl(C.Structure):
         ("linear_describe", LINEAR_DESCRIBE),
         ("linear_load", LINEAR_LOAD),
         ("linear_free", LINEAR_FREE),
-        ("_reserved", C.c_void_p * 4),
+        ("serving", C.POINTER(ServingVtbl)),
+        ("_reserved", C.c_void_p * 3),
     ]
 
 
@@ -190,6 +253,8 @@ def check_layout() -> None:
     assert C.sizeof(DeviceInfo) == 48 and DeviceInfo.is_unified_memory.offset == 41
     assert C.sizeof(QuantVtbl) == 8 + 14 * 8 and QuantVtbl.op_quantized_matmul_fused.offset == 8 + 6 * 8
     assert QuantVtbl.linear_free.offset == 80 and C.sizeof(LinearInfo) == 96
+    assert QuantVtbl.serving.offset == 88 and C.sizeof(ServingVtbl) == 88
+    assert [C.sizeof(t) for t in (PagedPlanArgs, PagedAppendArgs, PagedAttentionArgs, BlockNormArgs)] == [120, 104, 136, 160]
 
 
 check_layout()

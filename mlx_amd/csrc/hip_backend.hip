@@ -22,58 +22,14 @@
 
 #include "../../include/lux_gpu_backend_abi.h"
 #include "../../include/lux_gpu_quant_backend.h"
+#include "hip_context.h"
 #include "kernels.h"
 #include "qdispatch.h"
 #include "qweights.h"
 
+using namespace lxh;
+
 namespace {
-
-struct HipContext {
-    int device = 0;
-    hipStream_t stream = nullptr;
-    char name[256] = {0};
-    int compute_units = 0;
-    int max_wg = 0;
-    // kernel workspace (partial sums, tile counters and flags of the kernels
-    // that split K: split-K small-M GEMM, group-wise GEMM, the large GEMMs' K
-    // parts and split last round), allocated and zeroed once here so that no
-    // launch allocates; used only by work on `stream`, which orders its users
-    void* ws = nullptr;
-    size_t ws_bytes = 0;
-    // launches on ws so far: each GEMM launch gets the next number as its
-    // epoch (the split tiles meet by it; never 0)
-    uint32_t epoch = 0;
-};
-
-
-struct HipBuffer {
-    void* ptr = nullptr;
-    size_t size = 0;
-};
-
-HipContext* C(LuxBackendContext* c) { return reinterpret_cast<HipContext*>(c); }
-HipBuffer* B(LuxBackendBuffer* b) { return reinterpret_cast<HipBuffer*>(b); }
-
-LuxBackendError map_err(hipError_t e) {
-    switch (e) {
-    case hipSuccess: return LUX_BACKEND_OK;
-    case hipErrorOutOfMemory: return LUX_BACKEND_ERROR_OUT_OF_MEMORY;
-    case hipErrorInvalidValue: return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
-    case hipErrorNoDevice:
-    case hipErrorInvalidDevice: return LUX_BACKEND_ERROR_DEVICE_LOST;
-    default: return LUX_BACKEND_ERROR_INTERNAL;
-    }
-}
-
-LuxBackendError map_status(lxq::LuxStatus s) {
-    switch (s) {
-    case lxq::LuxStatus::Ok: return LUX_BACKEND_OK;
-    case lxq::LuxStatus::Invalid: return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
-    case lxq::LuxStatus::OutOfMemory: return LUX_BACKEND_ERROR_OUT_OF_MEMORY;
-    case lxq::LuxStatus::NotSupported: return LUX_BACKEND_ERROR_NOT_SUPPORTED;
-    default: return LUX_BACKEND_ERROR_INTERNAL;
-    }
-}
 
 bool is_gfx950(int dev) { return lux_hip_is_gfx950(dev); }
 
@@ -219,7 +175,7 @@ void hip_buffer_free(LuxBackendContext* c, LuxBackendBuffer* buf) {
         // queued kernels may still read the buffer
         hipStreamSynchronize(ctx->stream);
     }
-    if (b->ptr) hipFree(b->ptr);
+    if (b->ptr && b->owned) hipFree(b->ptr);
     delete b;
 }
 
@@ -257,10 +213,6 @@ void* hip_buffer_get_host_ptr(LuxBackendContext*, LuxBackendBuffer*) {
 // quantized matmul extension
 // ---------------------------------------------------------------------------
 
-size_t dtype_size(int dt) { return dt == LUX_DTYPE_FLOAT32 ? 4 : 2; }
-bool dtype_ok(int dt) {
-    return dt == LUX_DTYPE_FLOAT32 || dt == LUX_DTYPE_FLOAT16 || dt == LUX_DTYPE_BFLOAT16;
-}
 bool bits_ok(int b) { return b == 2 || b == 3 || b == 4 || b == 5 || b == 6 || b == 8; }
 
 // shared shape/format validation: OK, INVALID_ARGUMENT or NOT_SUPPORTED
@@ -272,8 +224,6 @@ LuxBackendError check_format(int K, int N, int group_size, int bits) {
     if (K % group_size) return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     return LUX_BACKEND_OK;
 }
-
-bool fits(HipBuffer* b, size_t need) { return b && (need == 0 || (b->ptr && b->size >= need)); }
 
 // M up to this value goes to the GEMV: LUX_HIP_GEMV_MAX_M when set, else 8,
 // or 16 where the GEMV family's MFMA kernels take the shape (16-bit x, 4- or
@@ -627,6 +577,7 @@ lux_gpu_quant_vtbl make_qvtbl() {
     q.linear_describe = hip_linear_describe;
     q.linear_load = hip_linear_load;
     q.linear_free = hip_linear_free;
+    q.serving = lux_hip_serving_table();
     return q;
 }
 

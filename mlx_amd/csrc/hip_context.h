@@ -1,0 +1,69 @@
+// hip_context.h -- the plugin's context and buffer records and the checks that
+// its entry points share (hip_backend.hip, serving_ops.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "../../include/lux_gpu_backend_abi.h"
+#include "../../include/lux_gpu_serving_backend.h"
+#include "kernels.h"
+
+namespace lxh {
+
+struct HipContext {
+    int device = 0;
+    hipStream_t stream = nullptr;
+    char name[256] = {0};
+    int compute_units = 0;
+    int max_wg = 0;
+    // kernel workspace (partial sums, tile counters and flags of the kernels
+    // that split K: split-K small-M GEMM, group-wise GEMM, the large GEMMs' K
+    // parts and split last round), allocated and zeroed once here so that no
+    // launch allocates; used only by work on `stream`, which orders its users
+    void* ws = nullptr;
+    size_t ws_bytes = 0;
+    // launches on ws so far: each GEMM launch gets the next number as its
+    // epoch (the split tiles meet by it; never 0)
+    uint32_t epoch = 0;
+};
+
+struct HipBuffer {
+    void* ptr = nullptr;
+    size_t size = 0;
+    bool owned = true;  // false: a view of memory that the caller frees
+};
+
+inline HipContext* C(LuxBackendContext* c) { return reinterpret_cast<HipContext*>(c); }
+inline HipBuffer* B(LuxBackendBuffer* b) { return reinterpret_cast<HipBuffer*>(b); }
+
+inline LuxBackendError map_err(hipError_t e) {
+    switch (e) {
+    case hipSuccess: return LUX_BACKEND_OK;
+    case hipErrorOutOfMemory: return LUX_BACKEND_ERROR_OUT_OF_MEMORY;
+    case hipErrorInvalidValue: return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
+    case hipErrorNoDevice:
+    case hipErrorInvalidDevice: return LUX_BACKEND_ERROR_DEVICE_LOST;
+    default: return LUX_BACKEND_ERROR_INTERNAL;
+    }
+}
+
+inline LuxBackendError map_status(lxq::LuxStatus s) {
+    switch (s) {
+    case lxq::LuxStatus::Ok: return LUX_BACKEND_OK;
+    case lxq::LuxStatus::Invalid: return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
+    case lxq::LuxStatus::OutOfMemory: return LUX_BACKEND_ERROR_OUT_OF_MEMORY;
+    case lxq::LuxStatus::NotSupported: return LUX_BACKEND_ERROR_NOT_SUPPORTED;
+    default: return LUX_BACKEND_ERROR_INTERNAL;
+    }
+}
+
+inline size_t dtype_size(int dt) { return dt == LUX_DTYPE_FLOAT32 ? 4 : 2; }
+inline bool dtype_ok(int dt) {
+    return dt == LUX_DTYPE_FLOAT32 || dt == LUX_DTYPE_FLOAT16 || dt == LUX_DTYPE_BFLOAT16;
+}
+
+inline bool fits(HipBuffer* b, size_t need) { return b && (need == 0 || (b->ptr && b->size >= need)); }
+
+}  // namespace lxh
+
+// the table of include/lux_gpu_serving_backend.h
+const lux_gpu_serving_vtbl* lux_hip_serving_table();

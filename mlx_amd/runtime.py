@@ -81,6 +81,8 @@ class Context:
         self.handle = self.vt.create_context(device_index)
         if not self.handle:
             raise RuntimeError(f"create_context({device_index}) failed")
+        serving = getattr(self.q, "serving", None)
+        self.s = serving.contents if serving else None
 
     def close(self) -> None:
         if self.handle:
@@ -106,6 +108,15 @@ class Context:
         if not h:
             raise LuxError(abi.ERR_OUT_OF_MEMORY, f"buffer_alloc_with_data({a.nbytes})")
         return Buffer(self, h, a.nbytes)
+
+    def wrap(self, address: int, nbytes: int) -> Buffer:
+        """A buffer over device memory that the caller owns and keeps; free()
+        leaves the memory alone.  Ordering other streams' work on it is the
+        caller's."""
+        h = self._serving().buffer_wrap(self.handle, address, nbytes)
+        if not h:
+            raise LuxError(abi.ERR_INVALID_ARGUMENT, f"buffer_wrap({address:#x}, {nbytes})")
+        return Buffer(self, h, nbytes)
 
     def sync(self) -> None:
         _check(self.vt.sync(self.handle), "sync")
@@ -176,6 +187,31 @@ class Context:
         sb = x_dtype if sb_dtype is None else sb_dtype
         r = f(M, K, N, group_size, bits, x_dtype, sb, sb if out_dtype is None else out_dtype, kernel)
         return None if r is None else r.decode()
+
+    # --- a decoding step over a paged cache (asynchronous on the context stream) ---
+    # Each takes its argument record (abi.Paged*Args, abi.BlockNormArgs), whose
+    # buffer fields are Buffer.handle values; a program may keep a record and
+    # pass it at every step.
+    def _serving(self) -> abi.ServingVtbl:
+        if self.s is None:
+            raise LuxError(abi.ERR_NOT_SUPPORTED, "serving operators")
+        return self.s
+
+    def paged_plan(self, args: abi.PagedPlanArgs) -> None:
+        """Pages and slots of a step's new tokens, from the requests' lengths."""
+        _check(self._serving().op_paged_plan(self.handle, args), "op_paged_plan")
+
+    def paged_append(self, args: abi.PagedAppendArgs) -> None:
+        """A step's keys and values into their slots of the paged cache."""
+        _check(self._serving().op_paged_append(self.handle, args), "op_paged_append")
+
+    def paged_attention(self, args: abi.PagedAttentionArgs) -> None:
+        """Attention of one token per request over its cached tokens."""
+        _check(self._serving().op_paged_attention(self.handle, args), "op_paged_attention")
+
+    def block_norm(self, args: abi.BlockNormArgs) -> None:
+        """h = residual_scale * residual + gate * post_norm(x); out = pre_norm(h)."""
+        _check(self._serving().op_block_norm(self.handle, args), "op_block_norm")
 
     # base f32 tensor ops (vtable slots, as the reference core calls them)
     def binary_f32(self, op: str, a: Buffer, b: Buffer, out: Buffer, n: int) -> None:
