@@ -67,6 +67,13 @@ LuxBackendContext* hip_create_context(int device_index) {
         (void)hipGetLastError();
         ctx->ws = nullptr;
     }
+    if (hipMalloc(&ctx->counts, kCountWords * 4) != hipSuccess) {
+        (void)hipGetLastError();
+        ctx->counts = nullptr;
+    } else if (hipMemset(ctx->counts, 0, kCountWords * 4) != hipSuccess) {
+        hipFree(ctx->counts);
+        ctx->counts = nullptr;
+    }
     return reinterpret_cast<LuxBackendContext*>(ctx);
 }
 
@@ -79,6 +86,7 @@ void hip_destroy_context(LuxBackendContext* c) {
         hipStreamDestroy(ctx->stream);
     }
     if (ctx->ws) hipFree(ctx->ws);
+    if (ctx->counts) hipFree(ctx->counts);
     delete ctx;
 }
 

@@ -18,8 +18,8 @@
 // turn; at its end they meet in LDS.  Where pairs of request and head are too
 // few or too uneven for the card, the tokens of all pairs are laid end to end
 // in units of NW tiles and cut into P equal ranges, one per block: a pair that
-// a cut goes through leaves partial (m, l, O) in the workspace, which a second
-// launch joins.  Bound by HBM.
+// a cut goes through leaves partial (m, l, O) in the workspace, which the last of
+// its blocks to arrive joins.  Bound by HBM.
 #pragma once
 #include "qcommon.h"
 #include "serving.h"
@@ -29,40 +29,34 @@ namespace attn {
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4h __attribute__((ext_vector_type(4), aligned(2)));  // rows of q start anywhere
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+constexpr int kDevice = 16;  // cache policy of the partial results: device scope (sc1)
 constexpr float kLowest = -3.0e38f;  // the maximum of no score
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 
 struct Params {
     AttnArgs a;
-    int HQ;            // heads of keys times query tiles of a group
-    int QT, rows;      // query tiles of a group; rows of a tile kept in partial results
-    int P;             // ranges; 0: one block per pair
-    float* part_o;     // [2 P, rows, D]
-    float* part_ml;    // [2 P, rows, 2]
-    int64_t* meta;     // [P, 4]
-};
-
-// what a boundary between two ranges needs to know to join the pair it cuts
-struct Cut {
-    int r, hq;  // r < 0: nothing to join here
-    int u0, n;  // units of the pair before the cut, and in all
-    int64_t units;
-    int64_t pad;
+    int HQ;           // heads of keys times query tiles of a group
+    int QT, rows;     // query tiles of a group; rows of a tile kept in partial results
+    int P;            // ranges
+    float* part_o;    // [2 P, rows, D]
+    float* part_ml;   // [2 P, rows, 2]
+    uint32_t part_o_bytes, part_ml_bytes;
 };
 
 // of `units` units, range w of P starts at first(w): the first units % P
 // ranges are one unit longer
 struct Ranges {
-    int64_t base, rem;
-    __device__ Ranges(int64_t units, int P) : base(units / P), rem(units - units / P * P) {}
-    __device__ int64_t first(int w) const { return w * base + (w < rem ? w : rem); }
-    __device__ int of(int64_t u) const {
-        const int64_t long_ones = rem * (base + 1);
-        return (int)(u < long_ones ? u / (base + 1) : rem + (u - long_ones) / base);
+    int base, rem;
+    __device__ Ranges(int units, int P) : base((int)((uint32_t)units / (uint32_t)P)), rem(units - base * P) {}
+    __device__ int first(int w) const { return w * base + (w < rem ? w : rem); }
+    __device__ int of(int u) const {
+        const int long_ones = rem * (base + 1);
+        return u < long_ones ? (int)((uint32_t)u / (uint32_t)(base + 1)) : rem + (int)((uint32_t)(u - long_ones) / (uint32_t)base);
     }
 };
 
@@ -99,10 +93,14 @@ __device__ __forceinline__ f4 mfma_qk(const u4& k, const u4& q, f4 c) {
     }
 }
 
-// max / sum over the four lanes that hold one query's tokens
+// max / sum over the four lanes that hold one query's tokens: both halves of a
+// row or wave swap are the pair's values, in either order
 __device__ __forceinline__ float group_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    uint32_t x = __float_as_uint(v);
+    auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = __float_as_uint(fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1])));
+    p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
 }
 __device__ __forceinline__ float group_sum(float v) {
     v += __shfl_xor(v, 16);
@@ -123,7 +121,12 @@ struct Attn {
     static constexpr int LS = DP + 4;                        // LDS row of a query, in floats
     typedef uint32_t uv __attribute__((ext_vector_type(VW)));
 
-    static constexpr size_t lds_bytes(int rows) { return (size_t)NW * (rows * LS + 32) * 4; }
+    static constexpr int NT = 64 * NW;
+    // the waves' results, or what finish() keeps per thread; a word
+    static constexpr size_t lds_floats(int rows) {
+        return (size_t)NW * (rows * LS + 32) > 6 * NT ? (size_t)NW * (rows * LS + 32) : 6 * NT;
+    }
+    static constexpr size_t lds_bytes(int rows) { return lds_floats(rows) * 4 + 16; }
 
     u4 q[NC], k[SUB][NC];
     uv v[4 * SUB][NV];
@@ -343,17 +346,97 @@ struct Attn {
                 acc += *reinterpret_cast<const f4*>(lds + (y * p.rows + i) * LS + d) * f;
             }
             if (slot >= 0) {
-                const int64_t at = (int64_t)slot * p.rows + i;
-                *reinterpret_cast<f4*>(p.part_o + at * a.D + d) = acc;
-                if (d == 0) {
-                    p.part_ml[at * 2] = top;
-                    p.part_ml[at * 2 + 1] = sum;
-                }
+                // device scope: the block that joins them may be on another die
+                const uint32_t at = (uint32_t)(slot * p.rows + i);
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, acc), o_rsrc(p), (at * a.D + d) * 4, 0, kDevice);
+                if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(top), __float_as_uint(sum)}, ml_rsrc(p), at * 8, 0, kDevice);
             } else {
                 store_row(a, r, h * a.G + qt * 16 + i, d, acc, top, sum);
             }
         }
         __syncthreads();
+    }
+
+    __device__ __forceinline__ static __amdgpu_buffer_rsrc_t o_rsrc(const Params& p) {
+        return __builtin_amdgcn_make_buffer_rsrc(p.part_o, 0, (int)p.part_o_bytes, 0x00020000);
+    }
+    __device__ __forceinline__ static __amdgpu_buffer_rsrc_t ml_rsrc(const Params& p) {
+        return __builtin_amdgcn_make_buffer_rsrc(p.part_ml, 0, (int)p.part_ml_bytes, 0x00020000);
+    }
+
+    // a pair's items: four channels of a row each
+    __device__ __forceinline__ static int items_of(const AttnArgs& a, int qt) {
+        return (a.G - qt * 16 < 16 ? a.G - qt * 16 : 16) * (a.D / 4);
+    }
+
+    // Joins the `parts` partial results of items [x0, last) of one pair: slot0,
+    // then every second slot from next on.  Where the items are fewer than the
+    // threads, several share the parts of one item and meet in LDS.
+    __device__ __forceinline__ static void finish(const Params& p, int r, int h, int qt, int x0, int last, int slot0, int next, int parts,
+                                                  float* lds) {
+        const AttnArgs& a = p.a;
+        const int per = a.D / 4, items = last - x0;
+        const int turns = items < NT ? NT / items : 1;
+        const int turn = turns > 1 ? (int)threadIdx.x / items : 0;
+        const __amdgpu_buffer_rsrc_t ro = o_rsrc(p), rm = ml_rsrc(p);
+        for (; x0 < last; x0 += NT) {
+            const int x = x0 + (int)threadIdx.x - turn * items;
+            const bool on = x < last && turn < turns;
+            const int i = x / per, d = (x - i * per) * 4;
+            float top = kLowest, sum = 0.f;
+            f4 acc = {0.f, 0.f, 0.f, 0.f};
+            constexpr int kBatch = 8;  // parts whose loads are in flight together
+            for (int s0 = turn; s0 < parts && on; s0 += kBatch * turns) {
+                u2 ml[kBatch];
+                u4 o[kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; k++) {
+                    const int s = s0 + k * turns;
+                    const uint32_t at = (uint32_t)((s == 0 ? slot0 : next + 2 * (s - 1)) * p.rows + i);
+                    // parts past the last: offsets past the end, which read zeros
+                    ml[k] = __builtin_amdgcn_raw_buffer_load_b64(rm, s < parts ? at * 8 : 0x80000000u, 0, kDevice);
+                    o[k] = __builtin_amdgcn_raw_buffer_load_b128(ro, s < parts ? (at * a.D + d) * 4 : 0x80000000u, 0, kDevice);
+                }
+                float most = top;
+#pragma unroll
+                for (int k = 0; k < kBatch; k++) {
+                    if (s0 + k * turns >= parts) ml[k][0] = __float_as_uint(kLowest);
+                    most = fmaxf(most, __uint_as_float(ml[k][0]));
+                }
+                const float f0 = __builtin_amdgcn_exp2f(top - most);
+                top = most;
+                sum *= f0;
+                acc *= f0;
+#pragma unroll
+                for (int k = 0; k < kBatch; k++) {
+                    const float f = __builtin_amdgcn_exp2f(__uint_as_float(ml[k][0]) - top);
+                    sum = fmaf(__uint_as_float(ml[k][1]), f, sum);
+                    acc += __builtin_bit_cast(f4, o[k]) * f;
+                }
+            }
+            if (turns > 1) {
+                f4* all = reinterpret_cast<f4*>(lds);  // [NT] sums, then [NT][2]
+                float* mls = lds + 4 * NT;
+                if (on) {
+                    all[threadIdx.x] = acc;
+                    mls[2 * threadIdx.x] = top;
+                    mls[2 * threadIdx.x + 1] = sum;
+                }
+                __syncthreads();
+                if (on && turn == 0) {
+                    for (int k = 1; k < turns; k++) {
+                        const int y = (int)threadIdx.x + k * items;
+                        const float most = fmaxf(top, mls[2 * y]), f0 = __builtin_amdgcn_exp2f(top - most),
+                                    f = __builtin_amdgcn_exp2f(mls[2 * y] - most);
+                        top = most;
+                        sum = sum * f0 + mls[2 * y + 1] * f;
+                        acc = acc * f0 + all[y] * f;
+                    }
+                }
+                __syncthreads();
+            }
+            if (on && turn == 0) store_row(a, r, h * a.G + qt * 16 + i, d, acc, top, sum);
+        }
     }
 
     // four channels of a head's result; no token counted: 0 and -infinity
@@ -375,9 +458,17 @@ struct Attn {
 
 extern __shared__ __attribute__((aligned(16))) float attn_lds[];
 
+// waves per SIMD that the registers allow
+#ifndef W64
+#define W64 3
+#define W128 2
+#endif
+template <int T, int DP>
+constexpr int kWaves = DP == 64 ? W64 : DP == 128 ? W128 : 1;
+
 // one block per pair
 template <int T, int DP, bool FULL, int NW>
-__global__ __launch_bounds__(64 * NW) void attn_pair_kernel(Params p) {
+__global__ __launch_bounds__(64 * NW, (kWaves<T, DP>)) void attn_pair_kernel(Params p) {
     using A = Attn<T, DP, FULL, NW>;
     A x;
     const int w = threadIdx.x >> 6;
@@ -387,49 +478,73 @@ __global__ __launch_bounds__(64 * NW) void attn_pair_kernel(Params p) {
     x.join(p, r, h, qt, -1, attn_lds);
 }
 
-// range blockIdx.x of P
-template <int T, int DP, bool FULL, int NW>
-__global__ __launch_bounds__(64 * NW) void attn_range_kernel(Params p) {
+// inclusive sum over the wave's lanes
+__device__ __forceinline__ int wave_scan(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int up = __shfl_up(v, d);
+        if (lane >= d) v += up;
+    }
+    return v;
+}
+
+// requests in front of unit pos / HQ, found by each wave for itself: lane i sums
+// the units of a stretch of requests
+struct Requests {
+    int all;      // units of all requests, for one of a request's pairs
+    int each, through, mine;
+    __device__ __forceinline__ Requests(const AttnArgs& a, int unit) : each((a.R + 63) / 64), mine(0) {
+        const int lane = threadIdx.x & 63;
+        for (int r = lane * each; r < (lane + 1) * each && r < a.R; r++) mine += units_of(extent_of(a, r), unit);
+        through = wave_scan(mine);
+        all = __shfl(through, 63);
+    }
+    // the request with unit `at`, and the units before it
+    __device__ __forceinline__ int find(const AttnArgs& a, int unit, int at, int& before) const {
+        const int lane = threadIdx.x & 63;
+        int s = __popcll(__ballot(through <= at)), r = s * each;
+        before = __shfl(through - mine, s);
+        for (; each > 1; r += 64) {
+            const int n = r + lane < a.R ? units_of(extent_of(a, r + lane), unit) : 0;
+            const int sum = before + wave_scan(n);
+            s = __popcll(__ballot(sum <= at));
+            if (s < 64) {
+                before = __shfl(sum - n, s);
+                r += s;
+                break;
+            }
+            before = __shfl(sum, 63);
+        }
+        return r;
+    }
+};
+
+// the ranges that hold a pair's units [from, from + n)
+struct Parts {
+    int w0, count, slot0, next;
+    __device__ __forceinline__ Parts(const Ranges& ranges, int from, int n) : w0(ranges.of(from)) {
+        count = ranges.of(from + n - 1) - w0 + 1;
+        slot0 = ranges.first(w0) == from ? 2 * w0 : 2 * w0 + 1;
+        next = 2 * (w0 + 1);
+    }
+};
+
+// range blockIdx.x of P; JOIN: the last of a cut pair's ranges to arrive joins it
+template <int T, int DP, bool FULL, int NW, bool JOIN>
+__global__ __launch_bounds__(64 * NW, (kWaves<T, DP>)) void attn_range_kernel(Params p) {
     using A = Attn<T, DP, FULL, NW>;
-    constexpr int NT = 64 * NW;
     const AttnArgs& a = p.a;
     const int w = threadIdx.x >> 6, me = blockIdx.x;
-    // units of the requests: thread i sums a stretch of them
-    __shared__ int64_t sums[NT], found[2];
-    const int each = (a.R + NT - 1) / NT, r0 = (int)threadIdx.x * each;
-    const int r1 = r0 + each < a.R ? r0 + each : a.R;
-    int64_t mine = 0;
-    for (int r = r0; r < r1; r++) mine += units_of(extent_of(a, r), A::kUnit);
-    sums[threadIdx.x] = mine;
-    __syncthreads();
-    int64_t before = 0, total = 0;
-    for (int i = 0; i < NT; i++) {
-        if (i < (int)threadIdx.x) before += sums[i];
-        total += sums[i];
-    }
-    const int64_t units = total * p.HQ;
-    const Ranges ranges(units, p.P);
-    int64_t pos = ranges.first(me);
-    const int64_t end = ranges.first(me + 1);
-    if (threadIdx.x == 0) reinterpret_cast<Cut*>(p.meta)[me].r = -1;
+    const Requests requests(a, A::kUnit);
+    const Ranges ranges(requests.all * p.HQ, p.P);
+    int pos = ranges.first(me);
+    const int end = ranges.first(me + 1);
     if (pos >= end) return;
-    if (r0 < r1 && pos >= before * p.HQ && pos < (before + mine) * p.HQ) {
-        int r = r0;
-        for (;; r++) {
-            const int n = units_of(extent_of(a, r), A::kUnit);
-            if (pos < (before + n) * p.HQ) break;
-            before += n;
-        }
-        found[0] = r;
-        found[1] = before * p.HQ;
-    }
-    __syncthreads();
-    int r = (int)found[0];
+    int before, r = requests.find(a, A::kUnit, (int)((uint32_t)pos / (uint32_t)p.HQ), before);
     Extent ex = extent_of(a, r);
     int n = units_of(ex, A::kUnit);
-    int hq = (int)((pos - found[1]) / n), u = (int)(pos - found[1] - (int64_t)hq * n);
-    if (threadIdx.x == 0 && u > 0 && pos - u >= ranges.first(me - 1))
-        reinterpret_cast<Cut*>(p.meta)[me] = Cut{r, hq, u, n, units, 0};
+    int hq = (int)((uint32_t)(pos - before * p.HQ) / (uint32_t)n), u = pos - before * p.HQ - hq * n;
     bool at_start = true;
     A x;
     while (pos < end) {
@@ -438,12 +553,29 @@ __global__ __launch_bounds__(64 * NW) void attn_range_kernel(Params p) {
             ex = extent_of(a, ++r);
             n = units_of(ex, A::kUnit);
         }
-        const int64_t left = end - pos;
-        const int u1 = left < n - u ? u + (int)left : n;
+        const int u1 = u + (end - pos) < n ? u + (end - pos) : n;
         const int h = hq / p.QT, qt = hq - h * p.QT;
         const int tiles = (ex.end - ex.base + A::kTile - 1) / A::kTile;
+        const bool part = u > 0 || u1 < n;
         x.run(a, ex, r, h, qt, u * NW + w, u1 * NW < tiles ? u1 * NW : tiles);
-        x.join(p, r, h, qt, u == 0 && u1 == n ? -1 : 2 * me + (at_start ? 0 : 1), attn_lds);
+        x.join(p, r, h, qt, !part ? -1 : 2 * me + (at_start ? 0 : 1), attn_lds);
+        if (JOIN && part) {
+            // only one pair goes past the end of a range, so its first range
+            // numbers its counter
+            const Parts parts(ranges, pos - u, n);
+            int* last = reinterpret_cast<int*>(attn_lds + A::lds_floats(p.rows));
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                uint32_t* c = a.count + parts.w0;
+                const bool l = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(parts.count - 1);
+                if (l) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                *last = l;
+            }
+            __syncthreads();
+            if (*last) A::finish(p, r, h, qt, 0, A::items_of(a, qt), parts.slot0, parts.next, parts.count, attn_lds);
+            __syncthreads();
+        }
         at_start = false;
         pos += u1 - u;
         u = 0;
@@ -451,55 +583,26 @@ __global__ __launch_bounds__(64 * NW) void attn_range_kernel(Params p) {
     }
 }
 
-// joins the partial results of the pair that the cut at range blockIdx.x's
-// start goes through first; block (x, y) takes query row y
-template <int T, int DP>
-__global__ __launch_bounds__(256) void attn_join_kernel(Params p) {
+// second launch: block (x, y) joins the y-th kJoinItems items of pair x, if a cut
+// went through it
+constexpr int kJoinItems = 32;
+template <int T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void attn_join_kernel(Params p) {
+    using A = Attn<T, DP, true, NW>;
+    __shared__ __attribute__((aligned(16))) float lds[6 * A::NT];
     const AttnArgs& a = p.a;
-    const int me = blockIdx.x, i = blockIdx.y;
-    const Cut c = reinterpret_cast<const Cut*>(p.meta)[me];
-    if (c.r < 0) return;
-    const int h = c.hq / p.QT, qt = c.hq - h * p.QT;
-    if (qt * 16 + i >= a.G) return;
-    const Ranges ranges(c.units, p.P);
-    const int64_t from = ranges.first(me) - c.u0;
-    const int parts = ranges.of(from + c.n - 1) - (me - 1) + 1;
-    const int slot0 = 2 * (me - 1) + (ranges.first(me - 1) == from ? 0 : 1);
-    auto slot = [&](int s) { return (int64_t)(s == 0 ? slot0 : 2 * (me - 1 + s)) * p.rows + i; };
-    __shared__ float red[256];
-    __shared__ f4 sum_o[256];
-    float top = kLowest;
-    for (int s = threadIdx.x; s < parts; s += 256) top = fmaxf(top, p.part_ml[slot(s) * 2]);
-    red[threadIdx.x] = top;
-    __syncthreads();
-    for (int k = 128; k > 0; k >>= 1) {
-        if ((int)threadIdx.x < k) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + k]);
-        __syncthreads();
-    }
-    top = red[0];
-    __syncthreads();
-    // DP / 4 threads across a row, 1024 / DP of them in turn over the parts
-    constexpr int across = DP / 4, turns = 256 / across;
-    const int d = (int)threadIdx.x % across * 4, turn = (int)threadIdx.x / across;
-    float sum = 0.f;
-    f4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int s = turn; s < parts; s += turns) {
-        const int64_t at = slot(s);
-        const float f = __builtin_amdgcn_exp2f(p.part_ml[at * 2] - top);
-        sum += p.part_ml[at * 2 + 1] * f;
-        if (d < a.D) acc += *reinterpret_cast<const f4*>(p.part_o + at * a.D + d) * f;
-    }
-    red[threadIdx.x] = sum;
-    sum_o[threadIdx.x] = acc;
-    __syncthreads();
-    if (turn == 0 && d < a.D) {
-#pragma unroll
-        for (int y = 1; y < turns; y++) {
-            sum += red[y * across + threadIdx.x];
-            acc += sum_o[y * across + threadIdx.x];
-        }
-        Attn<T, DP, true, 1>::store_row(a, c.r, h * a.G + qt * 16 + i, d, acc, top, sum);
-    }
+    const int r = blockIdx.x / p.HQ, hq = blockIdx.x - r * p.HQ, h = hq / p.QT, qt = hq - h * p.QT;
+    const int x0 = blockIdx.y * kJoinItems, items = A::items_of(a, qt);
+    if (x0 >= items) return;
+    const Requests requests(a, A::kUnit);
+    const Ranges ranges(requests.all * p.HQ, p.P);
+    const int stretch = r / requests.each;
+    int before = __shfl(requests.through - requests.mine, stretch);
+    for (int i = stretch * requests.each; i < r; i++) before += units_of(extent_of(a, i), A::kUnit);
+    const int n = units_of(extent_of(a, r), A::kUnit);
+    const Parts parts(ranges, before * p.HQ + hq * n, n);
+    if (parts.count > 1)
+        A::finish(p, r, h, qt, x0, x0 + kJoinItems < items ? x0 + kJoinItems : items, parts.slot0, parts.next, parts.count, lds);
 }
 
 template <int T, int DP, bool FULL>
@@ -508,25 +611,39 @@ LuxStatus launch_d(Params& p, hipStream_t st) {
     using A = Attn<T, DP, FULL, NW>;
     const size_t lds = A::lds_bytes(p.rows);
     const int64_t pairs = (int64_t)p.a.R * p.HQ;
-    static const hipError_t attr_p = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_pair_kernel<T, DP, FULL, NW>),
-                                                         hipFuncAttributeMaxDynamicSharedMemorySize, (int)A::lds_bytes(16));
-    static const hipError_t attr_r = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_range_kernel<T, DP, FULL, NW>),
-                                                         hipFuncAttributeMaxDynamicSharedMemorySize, (int)A::lds_bytes(16));
-    if (attr_p != hipSuccess || attr_r != hipSuccess) return LuxStatus::Internal;
-    // ranges: two blocks per CU, as many as the workspace has room for
-    int P = 2 * p.a.cus;
-    const size_t one = (size_t)p.rows * (p.a.D + 2) * 2 * 4 + sizeof(Cut);
+    auto pair = attn_pair_kernel<T, DP, FULL, NW>;
+    auto range = attn_range_kernel<T, DP, FULL, NW, true>, range_only = attn_range_kernel<T, DP, FULL, NW, false>;
+    static const bool attr = [&] {
+        for (const void* k : {(const void*)pair, (const void*)range, (const void*)range_only})
+            if (hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)A::lds_bytes(16)) != hipSuccess) return false;
+        return true;
+    }();
+    if (!attr) return LuxStatus::Internal;
+    // ranges: as many blocks as run at once, and the workspace has room for
+    int P = kWaves<T, DP> * p.a.cus;
+    const size_t one = (size_t)p.rows * (p.a.D + 2) * 2 * 4;
     if ((size_t)P * one > p.a.ws_bytes) P = (int)(p.a.ws_bytes / one);
-    const bool whole = P < 2 || p.a.columns * (int64_t)p.a.page <= A::kUnit;
+    if (P > p.a.counts) P = p.a.counts;
+    const int64_t longest = ((int64_t)p.a.columns * p.a.page + A::kUnit - 1) / A::kUnit + 1;  // units of a pair
+    const bool whole = P < 2 || longest <= 2 || longest * pairs >= (1ll << 31);
     if (whole) {
-        hipLaunchKernelGGL((attn_pair_kernel<T, DP, FULL, NW>), dim3((unsigned)pairs), dim3(64 * NW), lds, st, p);
+        hipLaunchKernelGGL(pair, dim3((unsigned)pairs), dim3(64 * NW), lds, st, p);
+        return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
+    }
+    p.P = P;
+    p.part_ml = p.a.ws;
+    p.part_ml_bytes = (uint32_t)P * 2 * p.rows * 8;
+    p.part_o = p.part_ml + p.part_ml_bytes / 4;
+    p.part_o_bytes = (uint32_t)P * 2 * p.rows * p.a.D * 4;
+    // one block joins a pair's parts within the launch, unless they are so
+    // many bytes that a second launch over more blocks is sooner done
+    const int64_t parts = longest < P / pairs ? longest : P / pairs;
+    if (parts * p.rows * p.a.D * 4 <= 256 * 1024) {
+        hipLaunchKernelGGL(range, dim3(P), dim3(64 * NW), lds, st, p);
     } else {
-        p.P = P;
-        p.meta = reinterpret_cast<int64_t*>(p.a.ws);
-        p.part_ml = p.a.ws + (size_t)P * sizeof(Cut) / 4;
-        p.part_o = p.part_ml + (size_t)P * 4 * p.rows;
-        hipLaunchKernelGGL((attn_range_kernel<T, DP, FULL, NW>), dim3(P), dim3(64 * NW), lds, st, p);
-        hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3(P, p.rows), dim3(256), 0, st, p);
+        hipLaunchKernelGGL(range_only, dim3(P), dim3(64 * NW), lds, st, p);
+        hipLaunchKernelGGL((attn_join_kernel<T, DP, NW>), dim3((unsigned)pairs, (unsigned)((p.rows * p.a.D / 4 + kJoinItems - 1) / kJoinItems)),
+                           dim3(64 * NW), 0, st, p);
     }
     return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
 }

@@ -56,6 +56,8 @@ struct AttnArgs {
     DivBy div;
     float* ws;  // partial results
     size_t ws_bytes;
+    uint32_t* count;  // `counts` words, zero between launches
+    int counts;
     int cus;
 };
 LuxStatus launch_paged_attention(const AttnArgs& a, hipStream_t st);

@@ -161,6 +161,8 @@ LuxBackendError op_paged_attention(LuxBackendContext* c, const lux_paged_attenti
     a.div = lxq::DivBy(p->page_size);
     a.ws = ctx->ws_bytes > lxq::kWorkspaceWords ? reinterpret_cast<float*>(static_cast<char*>(ctx->ws) + lxq::kWorkspaceWords) : nullptr;
     a.ws_bytes = a.ws ? ctx->ws_bytes - lxq::kWorkspaceWords : 0;
+    a.count = static_cast<uint32_t*>(ctx->counts);
+    a.counts = ctx->counts ? kCountWords : 0;
     a.cus = ctx->compute_units;
     if (hipSetDevice(ctx->device) != hipSuccess) return LUX_BACKEND_ERROR_DEVICE_LOST;
     return map_status(lxq::launch_paged_attention(a, ctx->stream));
