@@ -42,17 +42,20 @@ struct Params {
     AttnArgs a;
     int HQ;           // heads of keys times query tiles of a group
     int QT, rows;     // query tiles of a group; rows of a tile kept in partial results
-    int P;            // ranges
+    DivBy P, by_hq;   // ranges; division by HQ
+    bool join;        // the ranges join the pairs they share
     float* part_o;    // [2 P, rows, D]
     float* part_ml;   // [2 P, rows, 2]
     uint32_t part_o_bytes, part_ml_bytes;
 };
 
+__device__ __forceinline__ int div_by(int t, const DivBy& d) { return (int)(((uint64_t)(uint32_t)t * d.mul) >> (31 + d.sh)); }
+
 // of `units` units, range w of P starts at first(w): the first units % P
 // ranges are one unit longer
 struct Ranges {
     int base, rem;
-    __device__ Ranges(int units, int P) : base((int)((uint32_t)units / (uint32_t)P)), rem(units - base * P) {}
+    __device__ Ranges(int units, const DivBy& P) : base(div_by(units, P)), rem(units - base * P.d) {}
     __device__ int first(int w) const { return w * base + (w < rem ? w : rem); }
     __device__ int of(int u) const {
         const int long_ones = rem * (base + 1);
@@ -60,19 +63,19 @@ struct Ranges {
     }
 };
 
-__device__ __forceinline__ int div_by(int t, const DivBy& d) { return (int)(((uint64_t)(uint32_t)t * d.mul) >> (31 + d.sh)); }
-
 // the tokens of request r that count: [start, end), and where tiles begin
 struct Extent {
     int start, end, base;
 };
-__device__ __forceinline__ Extent extent_of(const AttnArgs& a, int r) {
+__device__ __forceinline__ Extent extent_of(const AttnArgs& a, int n) {
     const int cap = a.pool > 0 ? a.columns * a.page : 0;
-    int n = a.lens[r];
     n = n < 0 ? 0 : n > cap ? cap : n;
     const int s = a.window > 0 && n > a.window ? n - a.window : 0;
     return Extent{s, n, s & ~31};
 }
+// values that all lanes share, kept in scalar registers
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ Extent extent_at(const AttnArgs& a, int r) { return extent_of(a, uniform(a.lens[r])); }
 // units of `tokens` tokens; a request with none has one, which writes its zeros
 __device__ __forceinline__ int units_of(const Extent& e, int tokens) {
     const int n = (int)(((int64_t)e.end - e.base + tokens - 1) / tokens);
@@ -107,9 +110,18 @@ __device__ __forceinline__ float group_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
+// a wave's part of a pair
+struct Piece {
+    int r, h, qt;
+    int first, last;  // tiles
+    Extent ex;
+};
+
 // T: type of q, cache and out; DP: head_dim rounded up to 64, 128 or 256;
-// FULL: head_dim is DP
-template <int T, int DP, bool FULL, int NW>
+// FULL: head_dim is DP; WHOLE: pages hold whole runs of 16 tokens, so that a run
+// has one page and its rows one scalar base (else each lane finds its token's
+// row and the others take it from there); ONCE: cache loads that leave no copy
+template <int T, int DP, bool FULL, bool WHOLE, bool ONCE, int NW>
 struct Attn {
     static constexpr int ES = T == DT_F32 ? 4 : 2, E = 16 / ES;  // bytes; elements per 16 bytes
     static constexpr int SUB = T == DT_F32 ? 1 : 2, kTile = 16 * SUB;
@@ -128,18 +140,66 @@ struct Attn {
     }
     static constexpr size_t lds_bytes(int rows) { return lds_floats(rows) * 4 + 16; }
 
+    __device__ __forceinline__ static int dim(const AttnArgs& a) { return FULL ? DP : a.D; }
+
     u4 q[NC], k[SUB][NC];
     uv v[4 * SUB][NV];
     f4 o[NV][VE];
     float m, l;
+    int page[SUB], row[SUB];  // pages of the next tile, rows of the one in k and v: per run of 16, or the lane's token's in [0]
+    uint32_t bits;            // the tokens that count of the tile in k and v
 
-    // lane's token of a tile: its row of the cache, or -1
-    __device__ __forceinline__ static int page_at(const AttnArgs& a, const Extent& e, int r, int t) {
-        return t >= e.start && t < e.end ? a.table[(int64_t)r * a.columns + div_by(t, a.div)] : -1;
+    __device__ __forceinline__ Attn() {
+        if constexpr (!FULL) {  // the channels past head_dim, which no load touches
+#pragma unroll
+            for (int i = 0; i < SUB; i++)
+#pragma unroll
+                for (int c = 0; c < NC; c++) k[i][c] = u4{0, 0, 0, 0};
+        }
     }
-    __device__ __forceinline__ static int row_at(const AttnArgs& a, int h, int t, int page) {
-        const int at = t - div_by(t, a.div) * a.page;
-        return (uint32_t)page < (uint32_t)a.pool ? (page * a.Hk + h) * a.page + at : -1;
+
+    static constexpr uint32_t kAll = SUB == 2 ? 0xffffffffu : 0xffffu;
+
+    // pages of the tile at token t0
+    __device__ __forceinline__ void look(const AttnArgs& a, const Extent& e, int r, int t0) {
+        if constexpr (WHOLE) {
+            // (address space 4: scalar loads)
+            const auto* table = (const __attribute__((address_space(4))) int32_t*)a.table + (int64_t)r * a.columns;
+#pragma unroll
+            for (int s = 0; s < SUB; s++) {
+                const int t = t0 + 16 * s;
+                page[s] = t < e.end && t + 16 > e.start ? table[div_by(t, a.div)] : -1;
+            }
+        } else {
+            const int t = t0 + (int)(threadIdx.x & (kTile - 1));
+            page[0] = t >= e.start && t < e.end ? a.table[(int64_t)r * a.columns + div_by(t, a.div)] : -1;
+        }
+    }
+    // the rows they stand for; masked ones read row 0
+    __device__ __forceinline__ void resolve(const AttnArgs& a, const Extent& e, int h, int t0) {
+        if constexpr (WHOLE) {
+            const int lo = e.start > t0 ? e.start - t0 : 0, n = e.end - t0;
+            bits = (n >= kTile ? kAll : (1u << n) - 1u) & (kAll << lo);
+#pragma unroll
+            for (int s = 0; s < SUB; s++) {
+                const int t = t0 + 16 * s, at = t - div_by(t, a.div) * a.page;
+                const bool there = (uint32_t)page[s] < (uint32_t)a.pool;
+                row[s] = there ? (page[s] * a.Hk + h) * a.page + at : 0;
+                if (!there) bits &= ~(0xffffu << (16 * s));
+            }
+        } else {
+            const int t = t0 + (int)(threadIdx.x & (kTile - 1)), at = t - div_by(t, a.div) * a.page;
+            const bool there = (uint32_t)page[0] < (uint32_t)a.pool;
+            row[0] = there ? (page[0] * a.Hk + h) * a.page + at : 0;
+            bits = (uint32_t)__ballot(there) & kAll;
+        }
+    }
+    // the row of token i (of lane's choice in [0, 16)) of run s, in bytes from the cache's start: scalar and lane part
+    __device__ __forceinline__ const char* at_row(const AttnArgs& a, const void* cache, int s, int i) const {
+        const char* p = static_cast<const char*>(cache);
+        const uint32_t len = (uint32_t)(dim(a) * ES);
+        if constexpr (WHOLE) return p + (uint64_t)(uint32_t)row[s] * len + (uint32_t)i * len;
+        else return p + (uint64_t)(uint32_t)__shfl(row[0], 16 * s + i) * len;
     }
 
     __device__ __forceinline__ void load_q(const AttnArgs& a, int r, int h, int qt) {
@@ -148,34 +208,37 @@ struct Attn {
         for (int c = 0; c < NC; c++) {
             const int d = (4 * c + (lane >> 4)) * E;
             q[c] = u4{0, 0, 0, 0};
-            if (i < a.G && (FULL || d < a.D)) {
-                const char* p = static_cast<const char*>(a.q) + (r * a.q_row + (int64_t)(h * a.G + i) * a.D + d) * ES;
+            if (i < a.G && (FULL || d < dim(a))) {
+                const char* p = static_cast<const char*>(a.q) + (r * a.q_row + (int64_t)(h * a.G + i) * dim(a) + d) * ES;
                 q[c] = *reinterpret_cast<const u4h*>(p);
             }
         }
     }
-    // rows of masked tokens read row 0; channels past head_dim stay zero
-    __device__ __forceinline__ void load_k(const AttnArgs& a, int row) {
+    template <class V>
+    __device__ __forceinline__ static V load(const char* p) {
+        if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+        else return *reinterpret_cast<const V*>(p);
+    }
+    // channels past head_dim stay zero
+    __device__ __forceinline__ void load_k(const AttnArgs& a) {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int s = 0; s < SUB; s++) {
-            const int rw = __shfl(row, 16 * s + (lane & 15));
-            const char* p = static_cast<const char*>(a.kc) + (uint64_t)(uint32_t)(rw < 0 ? 0 : rw) * (uint32_t)(a.D * ES) + (lane >> 4) * 16;
+            const char* p = at_row(a, a.kc, s, lane & 15) + (lane >> 4) * 16;
 #pragma unroll
             for (int c = 0; c < NC; c++)
-                if (FULL || (4 * c + (lane >> 4)) * E < a.D) k[s][c] = *reinterpret_cast<const u4*>(p + c * 64);
+                if (FULL || (4 * c + (lane >> 4)) * E < dim(a)) k[s][c] = load<u4>(p + c * 64);
         }
     }
-    __device__ __forceinline__ void load_v(const AttnArgs& a, int row) {
+    __device__ __forceinline__ void load_v(const AttnArgs& a) {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int t = 0; t < 4 * SUB; t++) {
-            const int rw = __shfl(row, 16 * (t / 4) + 4 * (lane >> 4) + t % 4);
-            const char* p = static_cast<const char*>(a.vc) + (uint64_t)(uint32_t)(rw < 0 ? 0 : rw) * (uint32_t)(a.D * ES);
+            const char* p = at_row(a, a.vc, t / 4, 4 * (lane >> 4) + t % 4);
 #pragma unroll
             for (int c = 0; c < NV; c++) {
                 const int d = (16 * c + (lane & 15)) * VE;  // past head_dim: channels that are not stored
-                v[t][c] = *reinterpret_cast<const uv*>(p + (FULL || d < a.D ? d * ES : 0));
+                v[t][c] = load<uv>(p + (FULL || d < dim(a) ? d * ES : 0));
             }
         }
     }
@@ -191,21 +254,32 @@ struct Attn {
 
     // s (scores) to exp2 of their distance to the running maximum; bits: the
     // tile's tokens that count
-    __device__ __forceinline__ void soften(const AttnArgs& a, f4* s, uint64_t bits) {
+    __device__ __forceinline__ void soften(const AttnArgs& a, f4* s, uint32_t bits) {
         const int g = (threadIdx.x & 63) >> 4;
-        const float scale = a.scale * kLog2e;
+        if (a.softcap > 0.f) {
+            // cap tanh(y) = cap (1 - 2 / (1 + exp(2 y))), off by 2^-22 cap at most
+            const float in = 2.f * kLog2e * a.scale / a.softcap, cap = a.softcap * kLog2e;
+#pragma unroll
+            for (int i = 0; i < SUB; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    s[i][j] = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[i][j] * in)), -2.f * cap, cap);
+        } else {
+            const float scale = a.scale * kLog2e;
+#pragma unroll
+            for (int i = 0; i < SUB; i++) s[i] *= scale;
+        }
+        if (bits != kAll) {
+#pragma unroll
+            for (int i = 0; i < SUB; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[i][j] = (bits >> (16 * i + 4 * g + j)) & 1 ? s[i][j] : -INFINITY;
+        }
         float mx = kLowest;
 #pragma unroll
         for (int i = 0; i < SUB; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float x = s[i][j];
-                if (a.softcap > 0.f) x = a.softcap * kLog2e * tanhf(x * a.scale / a.softcap);
-                else x *= scale;
-                x = (bits >> (16 * i + 4 * g + j)) & 1 ? x : -INFINITY;
-                s[i][j] = x;
-                mx = fmaxf(mx, x);
-            }
+            for (int j = 0; j < 4; j++) mx = fmaxf(mx, s[i][j]);
         mx = fmaxf(group_max(mx), m);
         if (__any(mx > m)) {
             const float f = __builtin_amdgcn_exp2f(m - mx);
@@ -226,7 +300,7 @@ struct Attn {
     }
 
     // values of tokens that do not count are anything, NaN included: 0 instead
-    __device__ __forceinline__ void drop_values(uint64_t bits) {
+    __device__ __forceinline__ void drop_values(uint32_t bits) {
         const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
         for (int t = 0; t < 4 * SUB; t++) {
@@ -265,47 +339,43 @@ struct Attn {
         }
     }
 
-    // tiles first, first + NW, ... below last of one pair
-    __device__ __forceinline__ void run(const AttnArgs& a, const Extent& ex, int r, int h, int qt, int first, int last) {
-        const int lane = threadIdx.x & 63, in_tile = lane & (kTile - 1);
+    // One wave's tiles of a piece: first, first + NW, ... below last.  At its
+    // last tile it loads the first tile of `next`, so that the card does not
+    // wait between pieces; `primed`: so did the piece before this one.
+    __device__ __forceinline__ void run(const AttnArgs& a, const Piece& c, const Piece& next, bool& primed) {
         m = kLowest;
         l = 0.f;
 #pragma unroll
-        for (int c = 0; c < NV; c++)
+        for (int i = 0; i < NV; i++)
 #pragma unroll
-            for (int e = 0; e < VE; e++) o[c][e] = f4{0.f, 0.f, 0.f, 0.f};
-        if (first >= last) return;
-        if constexpr (!FULL) {
-#pragma unroll
-            for (int i = 0; i < SUB; i++)
-#pragma unroll
-                for (int c = 0; c < NC; c++) k[i][c] = u4{0, 0, 0, 0};
-        }
-        int t = ex.base + first * kTile + in_tile;
-        int row = row_at(a, h, t, page_at(a, ex, r, t));
-        load_q(a, r, h, qt);
-        load_k(a, row);
-        int page = page_at(a, ex, r, t + kUnit);
-        load_v(a, row);
-        for (int j = first; j < last; j += NW) {
-            const bool more = j + NW < last;
-            const uint64_t bits = __ballot(row >= 0);
+            for (int e = 0; e < VE; e++) o[i][e] = f4{0.f, 0.f, 0.f, 0.f};
+        if (c.first >= c.last) return;
+        // a first turn that only loads, unless the tile is there already
+        int j = primed ? c.first : c.first - NW;
+        primed = next.first < next.last;
+        for (; j < c.last; j += NW) {
+            const bool real = j >= c.first, more = j + NW < c.last;
+            const uint32_t now = bits;
             f4 s[SUB];
-            scores(s);
-            int next = 0;
-            t += kUnit;
-            if (more) {
-                next = row_at(a, h, t, page);
-                load_k(a, next);
-                page = page_at(a, ex, r, t + kUnit);
+            if (real) scores(s);
+            if (more || primed) {
+                const Extent ex{more ? c.ex.start : next.ex.start, more ? c.ex.end : next.ex.end, more ? c.ex.base : next.ex.base};
+                const int r = more ? c.r : next.r, h = more ? c.h : next.h;
+                const int t = ex.base + (more ? j + NW : next.first) * kTile;
+                if (!real || !more) {
+                    look(a, ex, r, t);
+                    load_q(a, r, h, more ? c.qt : next.qt);
+                }
+                resolve(a, ex, h, t);
+                load_k(a);
+                look(a, ex, r, t + kUnit);
             }
-            soften(a, s, bits);
-            if (bits != ~0ull) drop_values(bits);
-            gather(s);
-            if (more) {
-                load_v(a, next);
-                row = next;
+            if (real) {
+                soften(a, s, now);
+                if (now != kAll) drop_values(now);
+                gather(s);
             }
+            if (more || primed) load_v(a);
         }
         l = group_sum(l);
     }
@@ -313,7 +383,7 @@ struct Attn {
     // the waves' results of one pair: out and lse, or (slot >= 0) a partial result
     __device__ __forceinline__ void join(const Params& p, int r, int h, int qt, int slot, float* lds) {
         const AttnArgs& a = p.a;
-        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, qi = lane & 15, g = lane >> 4;
+        const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), qi = lane & 15, g = lane >> 4;
         float* ml = lds + NW * p.rows * LS;  // [NW][16][2]
         const int rows = a.G - qt * 16 < 16 ? a.G - qt * 16 : 16;
         if (lane < 16) {
@@ -331,7 +401,7 @@ struct Attn {
                             f4{o[c][e][i], o[c][e + 1][i], o[c][e + 2][i], o[c][e + 3][i]};
         }
         __syncthreads();
-        const int per = a.D / 4;
+        const int per = dim(a) / 4;
         for (int x = threadIdx.x; x < rows * per; x += NW * 64) {
             const int i = x / per, d = (x - i * per) * 4;
             float top = kLowest;
@@ -348,7 +418,7 @@ struct Attn {
             if (slot >= 0) {
                 // device scope: the block that joins them may be on another die
                 const uint32_t at = (uint32_t)(slot * p.rows + i);
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, acc), o_rsrc(p), (at * a.D + d) * 4, 0, kDevice);
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, acc), o_rsrc(p), (at * dim(a) + d) * 4, 0, kDevice);
                 if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(top), __float_as_uint(sum)}, ml_rsrc(p), at * 8, 0, kDevice);
             } else {
                 store_row(a, r, h * a.G + qt * 16 + i, d, acc, top, sum);
@@ -366,7 +436,7 @@ struct Attn {
 
     // a pair's items: four channels of a row each
     __device__ __forceinline__ static int items_of(const AttnArgs& a, int qt) {
-        return (a.G - qt * 16 < 16 ? a.G - qt * 16 : 16) * (a.D / 4);
+        return (a.G - qt * 16 < 16 ? a.G - qt * 16 : 16) * (dim(a) / 4);
     }
 
     // Joins the `parts` partial results of items [x0, last) of one pair: slot0,
@@ -375,7 +445,7 @@ struct Attn {
     __device__ __forceinline__ static void finish(const Params& p, int r, int h, int qt, int x0, int last, int slot0, int next, int parts,
                                                   float* lds) {
         const AttnArgs& a = p.a;
-        const int per = a.D / 4, items = last - x0;
+        const int per = dim(a) / 4, items = last - x0;
         const int turns = items < NT ? NT / items : 1;
         const int turn = turns > 1 ? (int)threadIdx.x / items : 0;
         const __amdgpu_buffer_rsrc_t ro = o_rsrc(p), rm = ml_rsrc(p);
@@ -385,7 +455,7 @@ struct Attn {
             const int i = x / per, d = (x - i * per) * 4;
             float top = kLowest, sum = 0.f;
             f4 acc = {0.f, 0.f, 0.f, 0.f};
-            constexpr int kBatch = 8;  // parts whose loads are in flight together
+            constexpr int kBatch = 16;  // parts whose loads are in flight together
             for (int s0 = turn; s0 < parts && on; s0 += kBatch * turns) {
                 u2 ml[kBatch];
                 u4 o[kBatch];
@@ -395,7 +465,7 @@ struct Attn {
                     const uint32_t at = (uint32_t)((s == 0 ? slot0 : next + 2 * (s - 1)) * p.rows + i);
                     // parts past the last: offsets past the end, which read zeros
                     ml[k] = __builtin_amdgcn_raw_buffer_load_b64(rm, s < parts ? at * 8 : 0x80000000u, 0, kDevice);
-                    o[k] = __builtin_amdgcn_raw_buffer_load_b128(ro, s < parts ? (at * a.D + d) * 4 : 0x80000000u, 0, kDevice);
+                    o[k] = __builtin_amdgcn_raw_buffer_load_b128(ro, s < parts ? (at * dim(a) + d) * 4 : 0x80000000u, 0, kDevice);
                 }
                 float most = top;
 #pragma unroll
@@ -442,7 +512,7 @@ struct Attn {
     // four channels of a head's result; no token counted: 0 and -infinity
     __device__ __forceinline__ static void store_row(const AttnArgs& a, int r, int head, int d, f4 acc, float top, float sum) {
         const float f = sum == 0.f ? 0.f : 1.f / sum;
-        const int64_t at = r * a.out_row + (int64_t)head * a.D + d;
+        const int64_t at = r * a.out_row + (int64_t)head * dim(a) + d;
         if (sum == 0.f) acc = f4{0.f, 0.f, 0.f, 0.f};
         if constexpr (T == DT_F32) {
             typedef float f4s __attribute__((ext_vector_type(4), aligned(4)));
@@ -459,22 +529,19 @@ struct Attn {
 extern __shared__ __attribute__((aligned(16))) float attn_lds[];
 
 // waves per SIMD that the registers allow
-#ifndef W64
-#define W64 3
-#define W128 2
-#endif
 template <int T, int DP>
-constexpr int kWaves = DP == 64 ? W64 : DP == 128 ? W128 : 1;
+constexpr int kWaves = DP == 64 ? 3 : DP == 128 ? 2 : 1;
 
 // one block per pair
-template <int T, int DP, bool FULL, int NW>
+template <int T, int DP, bool FULL, bool WHOLE, bool ONCE, int NW>
 __global__ __launch_bounds__(64 * NW, (kWaves<T, DP>)) void attn_pair_kernel(Params p) {
-    using A = Attn<T, DP, FULL, NW>;
+    using A = Attn<T, DP, FULL, WHOLE, ONCE, NW>;
     A x;
-    const int w = threadIdx.x >> 6;
+    const int w = uniform(threadIdx.x >> 6);
     const int r = blockIdx.x / p.HQ, hq = blockIdx.x - r * p.HQ, h = hq / p.QT, qt = hq - h * p.QT;
-    const Extent ex = extent_of(p.a, r);
-    x.run(p.a, ex, r, h, qt, w, (ex.end - ex.base + A::kTile - 1) / A::kTile);
+    const Extent ex = extent_at(p.a, r);
+    bool primed = false;
+    x.run(p.a, Piece{r, h, qt, w, (ex.end - ex.base + A::kTile - 1) / A::kTile, ex}, Piece{}, primed);
     x.join(p, r, h, qt, -1, attn_lds);
 }
 
@@ -494,27 +561,34 @@ __device__ __forceinline__ int wave_scan(int v) {
 struct Requests {
     int all;      // units of all requests, for one of a request's pairs
     int each, through, mine;
-    __device__ __forceinline__ Requests(const AttnArgs& a, int unit) : each((a.R + 63) / 64), mine(0) {
+    int len;      // of the lane's last request
+    __device__ __forceinline__ Requests(const AttnArgs& a, int unit) : each((a.R + 63) / 64), mine(0), len(0) {
         const int lane = threadIdx.x & 63;
-        for (int r = lane * each; r < (lane + 1) * each && r < a.R; r++) mine += units_of(extent_of(a, r), unit);
+        for (int r = lane * each; r < (lane + 1) * each && r < a.R; r++) {
+            len = a.lens[r];
+            mine += units_of(extent_of(a, len), unit);
+        }
         through = wave_scan(mine);
-        all = __shfl(through, 63);
+        all = __builtin_amdgcn_readlane(through, 63);
     }
-    // the request with unit `at`, and the units before it
-    __device__ __forceinline__ int find(const AttnArgs& a, int unit, int at, int& before) const {
+    // the request with unit `at`, the units before it and its length
+    __device__ __forceinline__ int find(const AttnArgs& a, int unit, int at, int& before, int& its) const {
         const int lane = threadIdx.x & 63;
         int s = __popcll(__ballot(through <= at)), r = s * each;
-        before = __shfl(through - mine, s);
+        before = __builtin_amdgcn_readlane(through - mine, s);
+        its = __builtin_amdgcn_readlane(len, s);
         for (; each > 1; r += 64) {
-            const int n = r + lane < a.R ? units_of(extent_of(a, r + lane), unit) : 0;
+            const int at_lane = r + lane < a.R ? a.lens[r + lane] : 0;
+            const int n = r + lane < a.R ? units_of(extent_of(a, at_lane), unit) : 0;
             const int sum = before + wave_scan(n);
             s = __popcll(__ballot(sum <= at));
             if (s < 64) {
-                before = __shfl(sum - n, s);
+                before = __builtin_amdgcn_readlane(sum - n, s);
+                its = __builtin_amdgcn_readlane(at_lane, s);
                 r += s;
                 break;
             }
-            before = __shfl(sum, 63);
+            before = __builtin_amdgcn_readlane(sum, 63);
         }
         return r;
     }
@@ -530,39 +604,57 @@ struct Parts {
     }
 };
 
-// range blockIdx.x of P; JOIN: the last of a cut pair's ranges to arrive joins it
-template <int T, int DP, bool FULL, int NW, bool JOIN>
+// a pair whose parts are all there
+struct Join {
+    int r, h, qt, slot0, next, count;
+};
+
+// range blockIdx.x of P; p.join: the last of a cut pair's ranges to arrive joins it
+template <int T, int DP, bool FULL, bool WHOLE, bool ONCE, int NW>
 __global__ __launch_bounds__(64 * NW, (kWaves<T, DP>)) void attn_range_kernel(Params p) {
-    using A = Attn<T, DP, FULL, NW>;
+    using A = Attn<T, DP, FULL, WHOLE, ONCE, NW>;
     const AttnArgs& a = p.a;
-    const int w = threadIdx.x >> 6, me = blockIdx.x;
+    const int w = uniform(threadIdx.x >> 6), me = blockIdx.x;
     const Requests requests(a, A::kUnit);
     const Ranges ranges(requests.all * p.HQ, p.P);
     int pos = ranges.first(me);
     const int end = ranges.first(me + 1);
     if (pos >= end) return;
-    int before, r = requests.find(a, A::kUnit, (int)((uint32_t)pos / (uint32_t)p.HQ), before);
-    Extent ex = extent_of(a, r);
+    int before, len;
+    int r = requests.find(a, A::kUnit, div_by(pos, p.by_hq), before, len);
+    Extent ex = extent_of(a, len);
     int n = units_of(ex, A::kUnit);
     int hq = (int)((uint32_t)(pos - before * p.HQ) / (uint32_t)n), u = pos - before * p.HQ - hq * n;
-    bool at_start = true;
+    bool at_start = true, primed = false;
     A x;
+    // the piece of pair (r, hq) from unit u on, as far as the range goes
+    auto piece = [&] {
+        const int h = p.QT == 1 ? hq : hq / p.QT, tiles = (ex.end - ex.base + A::kTile - 1) / A::kTile;
+        const int last = (u + (end - pos) < n ? u + (end - pos) : n) * NW;
+        return Piece{r, h, hq - h * p.QT, u * NW + w, last < tiles ? last : tiles, ex};
+    };
+    Piece c = piece();
+    Join first = {}, second = {};
     while (pos < end) {
-        if (hq == p.HQ) {
-            hq = 0;
-            ex = extent_of(a, ++r);
-            n = units_of(ex, A::kUnit);
+        const int from = pos - u, all = n, u0 = u, u1 = u + (end - pos) < n ? u + (end - pos) : n;
+        const bool part = u0 > 0 || u1 < n;
+        pos += u1 - u0;
+        u = 0;
+        Piece next = {};
+        if (pos < end) {
+            if (++hq == p.HQ) {
+                hq = 0;
+                ex = extent_at(a, ++r);
+                n = units_of(ex, A::kUnit);
+            }
+            next = piece();
         }
-        const int u1 = u + (end - pos) < n ? u + (end - pos) : n;
-        const int h = hq / p.QT, qt = hq - h * p.QT;
-        const int tiles = (ex.end - ex.base + A::kTile - 1) / A::kTile;
-        const bool part = u > 0 || u1 < n;
-        x.run(a, ex, r, h, qt, u * NW + w, u1 * NW < tiles ? u1 * NW : tiles);
-        x.join(p, r, h, qt, !part ? -1 : 2 * me + (at_start ? 0 : 1), attn_lds);
-        if (JOIN && part) {
+        x.run(a, c, next, primed);
+        x.join(p, c.r, c.h, c.qt, !part ? -1 : 2 * me + (at_start ? 0 : 1), attn_lds);
+        if (p.join && part) {
             // only one pair goes past the end of a range, so its first range
             // numbers its counter
-            const Parts parts(ranges, pos - u, n);
+            const Parts parts(ranges, from, all);
             int* last = reinterpret_cast<int*>(attn_lds + A::lds_floats(p.rows));
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
@@ -573,22 +665,34 @@ __global__ __launch_bounds__(64 * NW, (kWaves<T, DP>)) void attn_range_kernel(Pa
                 *last = l;
             }
             __syncthreads();
-            if (*last) A::finish(p, r, h, qt, 0, A::items_of(a, qt), parts.slot0, parts.next, parts.count, attn_lds);
+            if (uniform(*last)) {
+                // joined at the end of the range, when the tiles' registers
+                // are free; a range has at most two cut pairs
+                const Join j{c.r, c.h, c.qt, parts.slot0, parts.next, parts.count};
+                if (at_start) first = j;
+                else second = j;
+            }
             __syncthreads();
         }
         at_start = false;
-        pos += u1 - u;
-        u = 0;
-        hq++;
+        c = next;
+    }
+    if (p.join) {
+#pragma unroll 1
+        for (int i = 0; i < 2; i++) {
+            const Join j{i ? second.r : first.r, i ? second.h : first.h, i ? second.qt : first.qt, i ? second.slot0 : first.slot0,
+                         i ? second.next : first.next, i ? second.count : first.count};
+            if (j.count) A::finish(p, j.r, j.h, j.qt, 0, A::items_of(a, j.qt), j.slot0, j.next, j.count, attn_lds);
+        }
     }
 }
 
 // second launch: block (x, y) joins the y-th kJoinItems items of pair x, if a cut
 // went through it
 constexpr int kJoinItems = 32;
-template <int T, int DP, int NW>
+template <int T, int DP, bool FULL, int NW>
 __global__ __launch_bounds__(64 * NW) void attn_join_kernel(Params p) {
-    using A = Attn<T, DP, true, NW>;
+    using A = Attn<T, DP, FULL, true, false, NW>;
     __shared__ __attribute__((aligned(16))) float lds[6 * A::NT];
     const AttnArgs& a = p.a;
     const int r = blockIdx.x / p.HQ, hq = blockIdx.x - r * p.HQ, h = hq / p.QT, qt = hq - h * p.QT;
@@ -597,24 +701,24 @@ __global__ __launch_bounds__(64 * NW) void attn_join_kernel(Params p) {
     const Requests requests(a, A::kUnit);
     const Ranges ranges(requests.all * p.HQ, p.P);
     const int stretch = r / requests.each;
-    int before = __shfl(requests.through - requests.mine, stretch);
-    for (int i = stretch * requests.each; i < r; i++) before += units_of(extent_of(a, i), A::kUnit);
-    const int n = units_of(extent_of(a, r), A::kUnit);
+    int before = __builtin_amdgcn_readlane(requests.through - requests.mine, stretch);
+    for (int i = stretch * requests.each; i < r; i++) before += units_of(extent_at(a, i), A::kUnit);
+    const int n = units_of(extent_at(a, r), A::kUnit);
     const Parts parts(ranges, before * p.HQ + hq * n, n);
     if (parts.count > 1)
         A::finish(p, r, h, qt, x0, x0 + kJoinItems < items ? x0 + kJoinItems : items, parts.slot0, parts.next, parts.count, lds);
 }
 
-template <int T, int DP, bool FULL>
+template <int T, int DP, bool FULL, bool WHOLE, bool ONCE>
 LuxStatus launch_d(Params& p, hipStream_t st) {
     constexpr int NW = 4;
-    using A = Attn<T, DP, FULL, NW>;
+    using A = Attn<T, DP, FULL, WHOLE, ONCE, NW>;
     const size_t lds = A::lds_bytes(p.rows);
     const int64_t pairs = (int64_t)p.a.R * p.HQ;
-    auto pair = attn_pair_kernel<T, DP, FULL, NW>;
-    auto range = attn_range_kernel<T, DP, FULL, NW, true>, range_only = attn_range_kernel<T, DP, FULL, NW, false>;
+    auto pair = attn_pair_kernel<T, DP, FULL, WHOLE, ONCE, NW>;
+    auto range = attn_range_kernel<T, DP, FULL, WHOLE, ONCE, NW>;
     static const bool attr = [&] {
-        for (const void* k : {(const void*)pair, (const void*)range, (const void*)range_only})
+        for (const void* k : {(const void*)pair, (const void*)range})
             if (hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)A::lds_bytes(16)) != hipSuccess) return false;
         return true;
     }();
@@ -630,7 +734,8 @@ LuxStatus launch_d(Params& p, hipStream_t st) {
         hipLaunchKernelGGL(pair, dim3((unsigned)pairs), dim3(64 * NW), lds, st, p);
         return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
     }
-    p.P = P;
+    p.P = DivBy(P);
+    p.by_hq = DivBy(p.HQ);
     p.part_ml = p.a.ws;
     p.part_ml_bytes = (uint32_t)P * 2 * p.rows * 8;
     p.part_o = p.part_ml + p.part_ml_bytes / 4;
@@ -638,14 +743,31 @@ LuxStatus launch_d(Params& p, hipStream_t st) {
     // one block joins a pair's parts within the launch, unless they are so
     // many bytes that a second launch over more blocks is sooner done
     const int64_t parts = longest < P / pairs ? longest : P / pairs;
-    if (parts * p.rows * p.a.D * 4 <= 256 * 1024) {
-        hipLaunchKernelGGL(range, dim3(P), dim3(64 * NW), lds, st, p);
-    } else {
-        hipLaunchKernelGGL(range_only, dim3(P), dim3(64 * NW), lds, st, p);
-        hipLaunchKernelGGL((attn_join_kernel<T, DP, NW>), dim3((unsigned)pairs, (unsigned)((p.rows * p.a.D / 4 + kJoinItems - 1) / kJoinItems)),
-                           dim3(64 * NW), 0, st, p);
-    }
+    p.join = parts * p.rows * p.a.D * 4 <= 256 * 1024;
+    hipLaunchKernelGGL(range, dim3(P), dim3(64 * NW), lds, st, p);
+    if (!p.join)
+        hipLaunchKernelGGL((attn_join_kernel<T, DP, FULL, NW>),
+                           dim3((unsigned)pairs, (unsigned)((p.rows * p.a.D / 4 + kJoinItems - 1) / kJoinItems)), dim3(64 * NW), 0, st, p);
     return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
+}
+
+template <int T, int DP, bool FULL>
+LuxStatus launch_full(Params& p, hipStream_t st) {
+    if (p.a.page % 16) return launch_d<T, DP, FULL, false, false>(p, st);
+    // Rows that end on cache lines, of a pool that the last-level cache (256 MB)
+    // cannot hold: loads that leave no copy (8 requests of 131072 tokens 701 ->
+    // 625 us, 64 ragged ones up to 8192 203 -> 180).  A smaller pool may still
+    // be there from the call before (256 requests up to 128 tokens 18.5 us with
+    // such loads, 16.4 without; out of HBM 19.6 and 20.2), and a line that two
+    // rows share is wanted twice (head_dim 80, 64 requests up to 2048 tokens
+    // 46.1 and 41.1).
+    const int64_t row = (int64_t)p.a.D * (T == DT_F32 ? 4 : 2);
+    const bool once = row % 128 == 0 && 2 * row * p.a.pool * p.a.page * p.a.Hk >= (256ll << 20);
+    return once ? launch_d<T, DP, FULL, true, true>(p, st) : launch_d<T, DP, FULL, true, false>(p, st);
+}
+template <int T, int DP>
+LuxStatus launch_dp(Params& p, hipStream_t st) {
+    return p.a.D == DP ? launch_full<T, DP, true>(p, st) : launch_full<T, DP, false>(p, st);
 }
 
 template <int T>
@@ -655,9 +777,8 @@ LuxStatus launch_t(const AttnArgs& a, hipStream_t st) {
     p.QT = (a.G + 15) / 16;
     p.HQ = a.Hk * p.QT;
     p.rows = a.G < 16 ? a.G : 16;
-    if (a.D <= 64) return a.D == 64 ? launch_d<T, 64, true>(p, st) : launch_d<T, 64, false>(p, st);
-    if (a.D <= 128) return a.D == 128 ? launch_d<T, 128, true>(p, st) : launch_d<T, 128, false>(p, st);
-    return a.D == 256 ? launch_d<T, 256, true>(p, st) : launch_d<T, 256, false>(p, st);
+    if (a.D <= 64) return launch_dp<T, 64>(p, st);
+    return a.D <= 128 ? launch_dp<T, 128>(p, st) : launch_dp<T, 256>(p, st);
 }
 
 extern template LuxStatus launch_t<DT_F32>(const AttnArgs&, hipStream_t);
