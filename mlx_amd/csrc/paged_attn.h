@@ -39,6 +39,8 @@ constexpr float kLowest = -3.0e38f;  // the maximum of no score
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 
 struct Params {
+    // a.scale and a.softcap as the kernels take them: scores by log2 e are s *
+    // scale, or softcap tanh(y) with 2 y = s * scale
     AttnArgs a;
     int HQ;           // heads of keys times query tiles of a group
     int QT, rows;     // query tiles of a group; rows of a tile kept in partial results
@@ -78,7 +80,7 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ Extent extent_at(const AttnArgs& a, int r) { return extent_of(a, uniform(a.lens[r])); }
 // units of `tokens` tokens; a request with none has one, which writes its zeros
 __device__ __forceinline__ int units_of(const Extent& e, int tokens) {
-    const int n = (int)(((int64_t)e.end - e.base + tokens - 1) / tokens);
+    const int n = (int)((uint32_t)(e.end - e.base + tokens - 1) / (uint32_t)tokens);
     return n < 1 ? 1 : n;
 }
 
@@ -94,6 +96,24 @@ __device__ __forceinline__ f4 mfma_qk(const u4& k, const u4& q, f4 c) {
             c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[j]), __uint_as_float(q[j]), c, 0, 0, 0);
         return c;
     }
+}
+
+// slot of the s-th part of a pair that starts in range w0: a range keeps the part
+// that its first units continue in slot 2 w, the one that its last units start in
+// slot 2 w + 1
+__device__ __forceinline__ uint32_t slot(int w0, int s) { return (uint32_t)(2 * (w0 + s) + (s == 0)); }
+
+// x / d for whole numbers below 2^15: the half keeps the quotient off the next one
+__device__ __forceinline__ int small_div(int x, int d) {
+    return (int)(((float)x + 0.5f) * __builtin_amdgcn_rcpf((float)d));
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp_f<0xB1>(v));
+    v = fmaxf(v, dpp_f<0x4E>(v));
+    v = fmaxf(v, dpp_f<0x141>(v));
+    v = fmaxf(v, dpp_f<0x140>(v));
+    return fmaxf(fmaxf(lane_f(v, 0), lane_f(v, 16)), fmaxf(lane_f(v, 32), lane_f(v, 48)));
 }
 
 // max / sum over the four lanes that hold one query's tokens: both halves of a
@@ -134,9 +154,10 @@ struct Attn {
     typedef uint32_t uv __attribute__((ext_vector_type(VW)));
 
     static constexpr int NT = 64 * NW;
-    // the waves' results, or what finish() keeps per thread; a word
+    static constexpr int kChunk = 64, kFinish = 16 * (kChunk + 4) + 4 * NT;
+    // the waves' results, or what finish() keeps; a word
     static constexpr size_t lds_floats(int rows) {
-        return (size_t)NW * (rows * LS + 32) > 6 * NT ? (size_t)NW * (rows * LS + 32) : 6 * NT;
+        return (size_t)NW * (rows * LS + 32) > kFinish ? (size_t)NW * (rows * LS + 32) : kFinish;
     }
     static constexpr size_t lds_bytes(int rows) { return lds_floats(rows) * 4 + 16; }
 
@@ -202,18 +223,17 @@ struct Attn {
         else return p + (uint64_t)(uint32_t)__shfl(row[0], 16 * s + i) * len;
     }
 
+    // columns past the group's end take its first query: nobody reads their results
     __device__ __forceinline__ void load_q(const AttnArgs& a, int r, int h, int qt) {
         const int lane = threadIdx.x & 63, i = qt * 16 + (lane & 15);
+        const char* p = static_cast<const char*>(a.q) + (r * a.q_row + (int64_t)(h * a.G + (i < a.G ? i : 0)) * dim(a)) * ES;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             const int d = (4 * c + (lane >> 4)) * E;
-            q[c] = u4{0, 0, 0, 0};
-            if (i < a.G && (FULL || d < dim(a))) {
-                const char* p = static_cast<const char*>(a.q) + (r * a.q_row + (int64_t)(h * a.G + i) * dim(a) + d) * ES;
-                q[c] = *reinterpret_cast<const u4h*>(p);
-            }
+            q[c] = *reinterpret_cast<const u4h*>(p + (FULL || d < dim(a) ? d * ES : 0));
         }
     }
+
     template <class V>
     __device__ __forceinline__ static V load(const char* p) {
         if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
@@ -243,6 +263,7 @@ struct Attn {
         }
     }
 
+    // (channels past head_dim: keys of 0, against values of q that count anyway)
     __device__ __forceinline__ void scores(f4* s) const {
 #pragma unroll
         for (int i = 0; i < SUB; i++) s[i] = f4{0.f, 0.f, 0.f, 0.f};
@@ -258,16 +279,14 @@ struct Attn {
         const int g = (threadIdx.x & 63) >> 4;
         if (a.softcap > 0.f) {
             // cap tanh(y) = cap (1 - 2 / (1 + exp(2 y))), off by 2^-22 cap at most
-            const float in = 2.f * kLog2e * a.scale / a.softcap, cap = a.softcap * kLog2e;
 #pragma unroll
             for (int i = 0; i < SUB; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    s[i][j] = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[i][j] * in)), -2.f * cap, cap);
+                    s[i][j] = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[i][j] * a.scale)), -2.f * a.softcap, a.softcap);
         } else {
-            const float scale = a.scale * kLog2e;
 #pragma unroll
-            for (int i = 0; i < SUB; i++) s[i] *= scale;
+            for (int i = 0; i < SUB; i++) s[i] *= a.scale;
         }
         if (bits != kAll) {
 #pragma unroll
@@ -339,6 +358,13 @@ struct Attn {
         }
     }
 
+    // a tile's scores into the running maximum, sum and result
+    __device__ __forceinline__ void take(const AttnArgs& a, f4* s, uint32_t now) {
+        soften(a, s, now);
+        if (now != kAll) drop_values(now);
+        gather(s);
+    }
+
     // One wave's tiles of a piece: first, first + NW, ... below last.  At its
     // last tile it loads the first tile of `next`, so that the card does not
     // wait between pieces; `primed`: so did the piece before this one.
@@ -350,33 +376,41 @@ struct Attn {
 #pragma unroll
             for (int e = 0; e < VE; e++) o[i][e] = f4{0.f, 0.f, 0.f, 0.f};
         if (c.first >= c.last) return;
-        // a first turn that only loads, unless the tile is there already
-        int j = primed ? c.first : c.first - NW;
-        primed = next.first < next.last;
-        for (; j < c.last; j += NW) {
-            const bool real = j >= c.first, more = j + NW < c.last;
-            const uint32_t now = bits;
-            f4 s[SUB];
-            if (real) scores(s);
-            if (more || primed) {
-                const Extent ex{more ? c.ex.start : next.ex.start, more ? c.ex.end : next.ex.end, more ? c.ex.base : next.ex.base};
-                const int r = more ? c.r : next.r, h = more ? c.h : next.h;
-                const int t = ex.base + (more ? j + NW : next.first) * kTile;
-                if (!real || !more) {
-                    look(a, ex, r, t);
-                    load_q(a, r, h, more ? c.qt : next.qt);
-                }
-                resolve(a, ex, h, t);
-                load_k(a);
-                look(a, ex, r, t + kUnit);
-            }
-            if (real) {
-                soften(a, s, now);
-                if (now != kAll) drop_values(now);
-                gather(s);
-            }
-            if (more || primed) load_v(a);
+        int t = c.ex.base + c.first * kTile;
+        if (!primed) {
+            look(a, c.ex, c.r, t);
+            load_q(a, c.r, c.h, c.qt);
+            resolve(a, c.ex, c.h, t);
+            load_k(a);
+            look(a, c.ex, c.r, t + kUnit);
+            load_v(a);
         }
+        f4 s[SUB];
+        for (int j = c.first + NW; j < c.last; j += NW) {
+            const uint32_t now = bits;
+            scores(s);
+            t += kUnit;
+            resolve(a, c.ex, c.h, t);
+            load_k(a);
+            look(a, c.ex, c.r, t + kUnit);
+            take(a, s, now);
+            load_v(a);
+        }
+        // the last tile: no branch between its scores and the loads of the loop
+        // above, which would have the scores wait for the values too
+        const uint32_t now = bits;
+        scores(s);
+        primed = next.first < next.last;
+        if (primed) {
+            t = next.ex.base + next.first * kTile;
+            look(a, next.ex, next.r, t);
+            load_q(a, next.r, next.h, next.qt);
+            resolve(a, next.ex, next.h, t);
+            load_k(a);
+            look(a, next.ex, next.r, t + kUnit);
+        }
+        take(a, s, now);
+        if (primed) load_v(a);
         l = group_sum(l);
     }
 
@@ -439,74 +473,104 @@ struct Attn {
         return (a.G - qt * 16 < 16 ? a.G - qt * 16 : 16) * (dim(a) / 4);
     }
 
-    // Joins the `parts` partial results of items [x0, last) of one pair: slot0,
-    // then every second slot from next on.  Where the items are fewer than the
-    // threads, several share the parts of one item and meet in LDS.
-    __device__ __forceinline__ static void finish(const Params& p, int r, int h, int qt, int x0, int last, int slot0, int next, int parts,
-                                                  float* lds) {
+    // Joins the `parts` partial results of items [x0, last) of the pair that
+    // starts in range w0.  A wave takes whole rows of (m, l), a part per lane,
+    // and leaves the parts' weights in LDS; then a thread adds up its item's
+    // four channels, and where the items are fewer than the threads, several
+    // threads share an item's parts and meet in LDS.  Items past NT come with at
+    // most kChunk parts.
+    __device__ __forceinline__ static void finish(const Params& p, int r, int h, int qt, int x0, int last, int w0, int parts, float* lds) {
         const AttnArgs& a = p.a;
-        const int per = dim(a) / 4, items = last - x0;
-        const int turns = items < NT ? NT / items : 1;
-        const int turn = turns > 1 ? (int)threadIdx.x / items : 0;
+        const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
+        const int per = dim(a) / 4, items = last - x0, first = x0;
+        const int turns = items < NT ? small_div(NT, items) : 1;
+        const int turn = turns > 1 ? small_div(threadIdx.x, items) : 0;
+        const int row0 = small_div(x0, per), rows = small_div(last - 1, per) + 1 - row0;
         const __amdgpu_buffer_rsrc_t ro = o_rsrc(p), rm = ml_rsrc(p);
+        float* weight = lds;                                       // [16][kChunk]
+        float* of_row = lds + 16 * kChunk;                         // [16][4]: maximum, sum, rescaling
+        f4* all = reinterpret_cast<f4*>(lds + 16 * (kChunk + 4));  // [NT]
         for (; x0 < last; x0 += NT) {
             const int x = x0 + (int)threadIdx.x - turn * items;
             const bool on = x < last && turn < turns;
-            const int i = x / per, d = (x - i * per) * 4;
-            float top = kLowest, sum = 0.f;
+            const int i = on ? small_div(x, per) : row0, d = on ? (x - i * per) * 4 : 0;
             f4 acc = {0.f, 0.f, 0.f, 0.f};
-            constexpr int kBatch = 16;  // parts whose loads are in flight together
-            for (int s0 = turn; s0 < parts && on; s0 += kBatch * turns) {
-                u2 ml[kBatch];
+            for (int c0 = 0; c0 < parts; c0 += kChunk) {
+                const int n = parts - c0 < kChunk ? parts - c0 : kChunk;
+                const bool weigh = c0 > 0 || x0 == first;
+                u2 ml[16 / NW];
+                if (weigh)
+#pragma unroll
+                    for (int k = 0; k < 16 / NW; k++) {
+                        const int y = w + k * NW;
+                        if (y >= rows) break;
+                        ml[k] = __builtin_amdgcn_raw_buffer_load_b64(
+                            rm, lane < n ? (slot(w0, c0 + lane) * p.rows + row0 + y) * 8 : 0x80000000u, 0, kDevice);
+                    }
+                // up to kBatch of the thread's parts in flight together, in
+                // groups of 8 as far as there are any
+                constexpr int kBatch = 16;
                 u4 o[kBatch];
+                const uint32_t step = (uint32_t)(p.rows * dim(a)) * 4, hop = 2 * turns * step;
+                auto load_o = [&](int s0) {
+                    int s = s0 + turn;
+                    uint32_t at = (uint32_t)(i * dim(a) + d) * 4 + slot(w0, c0 + s) * step;
 #pragma unroll
-                for (int k = 0; k < kBatch; k++) {
-                    const int s = s0 + k * turns;
-                    const uint32_t at = (uint32_t)((s == 0 ? slot0 : next + 2 * (s - 1)) * p.rows + i);
-                    // parts past the last: offsets past the end, which read zeros
-                    ml[k] = __builtin_amdgcn_raw_buffer_load_b64(rm, s < parts ? at * 8 : 0x80000000u, 0, kDevice);
-                    o[k] = __builtin_amdgcn_raw_buffer_load_b128(ro, s < parts ? (at * dim(a) + d) * 4 : 0x80000000u, 0, kDevice);
-                }
-                float most = top;
+                    for (int q = 0; q < kBatch; q += 8) {
+                        if (s0 + q * turns >= n) break;
 #pragma unroll
-                for (int k = 0; k < kBatch; k++) {
-                    if (s0 + k * turns >= parts) ml[k][0] = __float_as_uint(kLowest);
-                    most = fmaxf(most, __uint_as_float(ml[k][0]));
-                }
-                const float f0 = __builtin_amdgcn_exp2f(top - most);
-                top = most;
-                sum *= f0;
-                acc *= f0;
+                        for (int k = q; k < q + 8; k++) {
+                            // past the last: an offset past the end, which reads zeros
+                            o[k] = __builtin_amdgcn_raw_buffer_load_b128(ro, s < n ? at : 0x80000000u, 0, kDevice);
+                            at += hop - (k == 0 && c0 + s == 0 ? step : 0);
+                            s += turns;
+                        }
+                    }
+                };
+                load_o(0);
+                if (weigh)
 #pragma unroll
-                for (int k = 0; k < kBatch; k++) {
-                    const float f = __builtin_amdgcn_exp2f(__uint_as_float(ml[k][0]) - top);
-                    sum = fmaf(__uint_as_float(ml[k][1]), f, sum);
-                    acc += __builtin_bit_cast(f4, o[k]) * f;
-                }
-            }
-            if (turns > 1) {
-                f4* all = reinterpret_cast<f4*>(lds);  // [NT] sums, then [NT][2]
-                float* mls = lds + 4 * NT;
-                if (on) {
-                    all[threadIdx.x] = acc;
-                    mls[2 * threadIdx.x] = top;
-                    mls[2 * threadIdx.x + 1] = sum;
-                }
+                    for (int k = 0; k < 16 / NW; k++) {
+                        const int y = w + k * NW;
+                        if (y >= rows) break;
+                        float* mine = of_row + 4 * y;
+                        const float m = lane < n ? __uint_as_float(ml[k][0]) : kLowest, was = c0 ? mine[0] : kLowest;
+                        const float top = fmaxf(was, wave_max(m)), f = lane < n ? __builtin_amdgcn_exp2f(m - top) : 0.f;
+                        const float sum = wave_sum(f * __uint_as_float(ml[k][1])), f0 = __builtin_amdgcn_exp2f(was - top);
+                        weight[y * kChunk + lane] = f;
+                        if (lane == 0) {
+                            mine[1] = (c0 ? mine[1] * f0 : 0.f) + sum;
+                            mine[0] = top;
+                            mine[2] = f0;
+                        }
+                    }
                 __syncthreads();
-                if (on && turn == 0) {
-                    for (int k = 1; k < turns; k++) {
-                        const int y = (int)threadIdx.x + k * items;
-                        const float most = fmaxf(top, mls[2 * y]), f0 = __builtin_amdgcn_exp2f(top - most),
-                                    f = __builtin_amdgcn_exp2f(mls[2 * y] - most);
-                        top = most;
-                        sum = sum * f0 + mls[2 * y + 1] * f;
-                        acc = acc * f0 + all[y] * f;
+                acc *= of_row[4 * (i - row0) + 2];
+                for (int s0 = 0; s0 < n; s0 += kBatch * turns) {
+                    if (s0) load_o(s0);
+#pragma unroll
+                    for (int q = 0; q < kBatch; q += 8) {
+                        if (s0 + q * turns >= n) break;
+#pragma unroll
+                        for (int k = q; k < q + 8; k++) {
+                            const int s = s0 + turn + k * turns;
+                            acc += __builtin_bit_cast(f4, o[k]) * weight[(i - row0) * kChunk + (s < kChunk ? s : kChunk - 1)];
+                        }
                     }
                 }
                 __syncthreads();
             }
-            if (on && turn == 0) store_row(a, r, h * a.G + qt * 16 + i, d, acc, top, sum);
+            if (turns > 1) {
+                all[threadIdx.x] = acc;
+                __syncthreads();
+                if (on && turn == 0)
+                    for (int k = 1; k < turns; k++) acc += all[threadIdx.x + k * items];
+                __syncthreads();
+            }
+            if (on && turn == 0)
+                store_row(a, r, h * a.G + qt * 16 + i, d, acc, of_row[4 * (i - row0)], of_row[4 * (i - row0) + 1]);
         }
+        __syncthreads();
     }
 
     // four channels of a head's result; no token counted: 0 and -infinity
@@ -528,13 +592,15 @@ struct Attn {
 
 extern __shared__ __attribute__((aligned(16))) float attn_lds[];
 
-// waves per SIMD that the registers allow
-template <int T, int DP>
-constexpr int kWaves = DP == 64 ? 3 : DP == 128 ? 2 : 1;
+// waves per SIMD that the registers allow (three at 64 and 128 channels were as
+// fast or slower: 64 heads on 4, up to 4096 tokens of 64 channels 60.6 us with
+// two, 63.4 with three)
+template <int DP>
+constexpr int kWaves = DP == 256 ? 1 : 2;
 
 // one block per pair
 template <int T, int DP, bool FULL, bool WHOLE, bool ONCE, int NW>
-__global__ __launch_bounds__(64 * NW, (kWaves<T, DP>)) void attn_pair_kernel(Params p) {
+__global__ __launch_bounds__(64 * NW, (kWaves<DP>)) void attn_pair_kernel(Params p) {
     using A = Attn<T, DP, FULL, WHOLE, ONCE, NW>;
     A x;
     const int w = uniform(threadIdx.x >> 6);
@@ -545,15 +611,19 @@ __global__ __launch_bounds__(64 * NW, (kWaves<T, DP>)) void attn_pair_kernel(Par
     x.join(p, r, h, qt, -1, attn_lds);
 }
 
-// inclusive sum over the wave's lanes
+// inclusive sum over the wave's lanes: shifts within rows of 16, then each
+// row's last lane to the rows behind it
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
 __device__ __forceinline__ int wave_scan(int v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int up = __shfl_up(v, d);
-        if (lane >= d) v += up;
-    }
-    return v;
+    v = dpp_add<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);     // row_bcast:15 into rows 1 and 3
+    return dpp_add<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
 }
 
 // requests in front of unit pos / HQ, found by each wave for itself: lane i sums
@@ -596,22 +666,15 @@ struct Requests {
 
 // the ranges that hold a pair's units [from, from + n)
 struct Parts {
-    int w0, count, slot0, next;
+    int w0, count;
     __device__ __forceinline__ Parts(const Ranges& ranges, int from, int n) : w0(ranges.of(from)) {
         count = ranges.of(from + n - 1) - w0 + 1;
-        slot0 = ranges.first(w0) == from ? 2 * w0 : 2 * w0 + 1;
-        next = 2 * (w0 + 1);
     }
-};
-
-// a pair whose parts are all there
-struct Join {
-    int r, h, qt, slot0, next, count;
 };
 
 // range blockIdx.x of P; p.join: the last of a cut pair's ranges to arrive joins it
 template <int T, int DP, bool FULL, bool WHOLE, bool ONCE, int NW>
-__global__ __launch_bounds__(64 * NW, (kWaves<T, DP>)) void attn_range_kernel(Params p) {
+__global__ __launch_bounds__(64 * NW, (kWaves<DP>)) void attn_range_kernel(Params p) {
     using A = Attn<T, DP, FULL, WHOLE, ONCE, NW>;
     const AttnArgs& a = p.a;
     const int w = uniform(threadIdx.x >> 6), me = blockIdx.x;
@@ -634,23 +697,20 @@ __global__ __launch_bounds__(64 * NW, (kWaves<T, DP>)) void attn_range_kernel(Pa
         return Piece{r, h, hq - h * p.QT, u * NW + w, last < tiles ? last : tiles, ex};
     };
     Piece c = piece();
-    Join first = {}, second = {};
+    int r0 = 0, h0 = 0, qt0 = 0, w0 = 0, count0 = 0, r1 = 0, h1 = 0, qt1 = 0, w1 = 0, count1 = 0;
     while (pos < end) {
         const int from = pos - u, all = n, u0 = u, u1 = u + (end - pos) < n ? u + (end - pos) : n;
         const bool part = u0 > 0 || u1 < n;
         pos += u1 - u0;
         u = 0;
-        Piece next = {};
-        if (pos < end) {
-            if (++hq == p.HQ) {
-                hq = 0;
-                ex = extent_at(a, ++r);
-                n = units_of(ex, A::kUnit);
-            }
-            next = piece();
+        if (pos < end && ++hq == p.HQ) {
+            hq = 0;
+            ex = extent_at(a, ++r);
+            n = units_of(ex, A::kUnit);
         }
+        const Piece next = piece();  // at the range's end: no tiles
         x.run(a, c, next, primed);
-        x.join(p, c.r, c.h, c.qt, !part ? -1 : 2 * me + (at_start ? 0 : 1), attn_lds);
+        x.join(p, c.r, c.h, c.qt, !part ? -1 : 2 * me + (u0 == 0), attn_lds);
         if (p.join && part) {
             // only one pair goes past the end of a range, so its first range
             // numbers its counter
@@ -668,9 +728,8 @@ __global__ __launch_bounds__(64 * NW, (kWaves<T, DP>)) void attn_range_kernel(Pa
             if (uniform(*last)) {
                 // joined at the end of the range, when the tiles' registers
                 // are free; a range has at most two cut pairs
-                const Join j{c.r, c.h, c.qt, parts.slot0, parts.next, parts.count};
-                if (at_start) first = j;
-                else second = j;
+                if (at_start) r0 = c.r, h0 = c.h, qt0 = c.qt, w0 = parts.w0, count0 = parts.count;
+                else r1 = c.r, h1 = c.h, qt1 = c.qt, w1 = parts.w0, count1 = parts.count;
             }
             __syncthreads();
         }
@@ -680,9 +739,8 @@ __global__ __launch_bounds__(64 * NW, (kWaves<T, DP>)) void attn_range_kernel(Pa
     if (p.join) {
 #pragma unroll 1
         for (int i = 0; i < 2; i++) {
-            const Join j{i ? second.r : first.r, i ? second.h : first.h, i ? second.qt : first.qt, i ? second.slot0 : first.slot0,
-                         i ? second.next : first.next, i ? second.count : first.count};
-            if (j.count) A::finish(p, j.r, j.h, j.qt, 0, A::items_of(a, j.qt), j.slot0, j.next, j.count, attn_lds);
+            if (count0) A::finish(p, r0, h0, qt0, 0, A::items_of(a, qt0), w0, count0, attn_lds);
+            r0 = r1, h0 = h1, qt0 = qt1, w0 = w1, count0 = count1;
         }
     }
 }
@@ -693,7 +751,7 @@ constexpr int kJoinItems = 32;
 template <int T, int DP, bool FULL, int NW>
 __global__ __launch_bounds__(64 * NW) void attn_join_kernel(Params p) {
     using A = Attn<T, DP, FULL, true, false, NW>;
-    __shared__ __attribute__((aligned(16))) float lds[6 * A::NT];
+    __shared__ __attribute__((aligned(16))) float lds[A::kFinish];
     const AttnArgs& a = p.a;
     const int r = blockIdx.x / p.HQ, hq = blockIdx.x - r * p.HQ, h = hq / p.QT, qt = hq - h * p.QT;
     const int x0 = blockIdx.y * kJoinItems, items = A::items_of(a, qt);
@@ -706,7 +764,7 @@ __global__ __launch_bounds__(64 * NW) void attn_join_kernel(Params p) {
     const int n = units_of(extent_at(a, r), A::kUnit);
     const Parts parts(ranges, before * p.HQ + hq * n, n);
     if (parts.count > 1)
-        A::finish(p, r, h, qt, x0, x0 + kJoinItems < items ? x0 + kJoinItems : items, parts.slot0, parts.next, parts.count, lds);
+        A::finish(p, r, h, qt, x0, x0 + kJoinItems < items ? x0 + kJoinItems : items, parts.w0, parts.count, lds);
 }
 
 template <int T, int DP, bool FULL, bool WHOLE, bool ONCE>
@@ -724,7 +782,7 @@ LuxStatus launch_d(Params& p, hipStream_t st) {
     }();
     if (!attr) return LuxStatus::Internal;
     // ranges: as many blocks as run at once, and the workspace has room for
-    int P = kWaves<T, DP> * p.a.cus;
+    int P = kWaves<DP> * p.a.cus;
     const size_t one = (size_t)p.rows * (p.a.D + 2) * 2 * 4;
     if ((size_t)P * one > p.a.ws_bytes) P = (int)(p.a.ws_bytes / one);
     if (P > p.a.counts) P = p.a.counts;
@@ -777,6 +835,8 @@ LuxStatus launch_t(const AttnArgs& a, hipStream_t st) {
     p.QT = (a.G + 15) / 16;
     p.HQ = a.Hk * p.QT;
     p.rows = a.G < 16 ? a.G : 16;
+    p.a.scale = a.softcap > 0.f ? 2.f * kLog2e * a.scale / a.softcap : kLog2e * a.scale;
+    p.a.softcap = a.softcap * kLog2e;
     if (a.D <= 64) return launch_dp<T, 64>(p, st);
     return a.D <= 128 ? launch_dp<T, 128>(p, st) : launch_dp<T, 256>(p, st);
 }
