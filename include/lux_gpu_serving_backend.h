@@ -108,7 +108,7 @@ typedef struct lux_paged_append_args {
  * they hold.  Scores, sums and the running statistics are fp32; with 16-bit
  * types exp(s - max) is rounded to that type before the product with v.
  * head_dim: a multiple of 8, at most 256; heads a multiple of kv_heads;
- * num_pages * kv_heads * page_size below 2^31.
+ * num_pages * kv_heads * page_size below 2^31; the caches start on 16 bytes.
  */
 typedef struct lux_paged_attention_args {
     uint32_t struct_size;
@@ -146,7 +146,7 @@ typedef enum {
  * x is a block's output, post_norm the norm after it, pre_norm the norm before
  * the next block.  In fp32, h unrounded into pre_norm; each output is rounded
  * once.  A NULL weight is 1, a NULL bias 0.  residual NULL: h = gate *
- * post_norm(x).  residual_out or out may be NULL, not both.  residual_out may
+ * post_norm(x).  Rows of gate are gate_row_stride apart (GATE_ROW: its values).  residual_out or out may be NULL, not both.  residual_out may
  * be residual itself, and out may be x (same place, stride and dtype).  dim:
  * at most 65536.
  */

@@ -37,16 +37,22 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, float* v) {
         }
     }
 }
-template <int DT>
+// AWAY: past the caches
+template <bool AWAY, class P>
+__device__ __forceinline__ void put(void* p, P v) {
+    if constexpr (AWAY) __builtin_nontemporal_store(v, static_cast<P*>(p));
+    else *static_cast<P*>(p) = v;
+}
+template <int DT, bool AWAY>
 __device__ __forceinline__ void store8(void* p, int64_t i, const float* v) {
     if constexpr (DT == DT_F32) {
-        *reinterpret_cast<f4u*>(static_cast<float*>(p) + i) = f4u{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f4u*>(static_cast<float*>(p) + i + 4) = f4u{v[4], v[5], v[6], v[7]};
+        put<AWAY>(static_cast<float*>(p) + i, f4u{v[0], v[1], v[2], v[3]});
+        put<AWAY>(static_cast<float*>(p) + i + 4, f4u{v[4], v[5], v[6], v[7]});
     } else {
         u4u a;
 #pragma unroll
         for (int e = 0; e < 4; e++) a[e] = pack2<DT>(v[2 * e], v[2 * e + 1]);
-        *reinterpret_cast<u4u*>(static_cast<uint16_t*>(p) + i) = a;
+        put<AWAY>(static_cast<uint16_t*>(p) + i, a);
     }
 }
 
@@ -60,10 +66,10 @@ __device__ __forceinline__ void load_part(const void* p, int64_t i, int n, float
         for (int e = 0; e < 8; e++) v[e] = e < n ? load_f(p, i + e, DT) : 0.f;
     }
 }
-template <int DT>
+template <int DT, bool AWAY>
 __device__ __forceinline__ void store_part(void* p, int64_t i, int n, const float* v) {
     if (n >= 8) {
-        store8<DT>(p, i, v);
+        store8<DT, AWAY>(p, i, v);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; e++)
@@ -141,7 +147,7 @@ __device__ __forceinline__ void normalize(float (*v)[8], const int* n, int kind,
 }
 
 // a block per row
-template <int NT, int V, int XT, int RT>
+template <int NT, int V, bool AWAY, int XT, int RT>
 __global__ __launch_bounds__(NT) void block_norm_kernel(NormArgs a) {
     __shared__ float part[16];
     constexpr int hop = NT * 8;
@@ -182,13 +188,13 @@ __global__ __launch_bounds__(NT) void block_norm_kernel(NormArgs a) {
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) v[i][e] = e < n[i] ? v[i][e] : 0.f;
-        if (a.h) store_part<RT>(a.h, t * a.h_row + c, n[i], v[i]);
+        if (a.h) store_part<RT, AWAY>(a.h, t * a.h_row + c, n[i], v[i]);
     }
     if (!a.out) return;
     if (a.pre != NORM_NONE) normalize<NT, V>(v, n, a.pre, inv_d, a.eps, a.nw, a.nb, a.w_dt, col, part);
 #pragma unroll
     for (int i = 0; i < V; i++)
-        if (n[i] > 0) store_part<XT>(a.out, t * a.o_row + col + i * hop, n[i], v[i]);
+        if (n[i] > 0) store_part<XT, AWAY>(a.out, t * a.o_row + col + i * hop, n[i], v[i]);
 }
 
 // Rows too long for the registers (past 32768): x and the residual are read again
@@ -269,31 +275,46 @@ __global__ __launch_bounds__(1024) void block_norm_long_kernel(NormArgs a) {
         const int n = a.D - c;
         float v[8];
         h_at(c, n, v);
-        if (a.h) store_part<RT>(a.h, t * a.h_row + c, n, v);
+        if (a.h) store_part<RT, false>(a.h, t * a.h_row + c, n, v);
         if (!a.out) continue;
         if (a.pre != NORM_NONE) affine(v, c, n, mean2, scale2, a.nw, a.nb);
-        store_part<XT>(a.out, t * a.o_row + c, n, v);
+        store_part<XT, false>(a.out, t * a.o_row + c, n, v);
     }
 }
 
 // NT threads and V vectors of 8 per thread; NT = 0: the long form
-template <int NT, int V, int XT, int RT>
+template <int NT, int V, bool AWAY, int XT, int RT>
 void launch_xr(const NormArgs& a, hipStream_t st) {
     if constexpr (NT == 0) hipLaunchKernelGGL((block_norm_long_kernel<XT, RT>), dim3(a.T), dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL((block_norm_kernel<NT, V, XT, RT>), dim3(a.T), dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((block_norm_kernel<NT, V, AWAY, XT, RT>), dim3(a.T), dim3(NT), 0, st, a);
 }
-template <int NT, int V, int XT>
+template <int NT, int V, bool AWAY, int XT>
 void launch_x(const NormArgs& a, hipStream_t st) {
-    if (a.r_dt == DT_F32) launch_xr<NT, V, XT, DT_F32>(a, st);
-    else if (a.r_dt == DT_F16) launch_xr<NT, V, XT, DT_F16>(a, st);
-    else launch_xr<NT, V, XT, DT_BF16>(a, st);
+    if (a.r_dt == DT_F32) launch_xr<NT, V, AWAY, XT, DT_F32>(a, st);
+    else if (a.r_dt == DT_F16) launch_xr<NT, V, AWAY, XT, DT_F16>(a, st);
+    else launch_xr<NT, V, AWAY, XT, DT_BF16>(a, st);
 }
-template <int NT, int V>
+template <int NT, int V, bool AWAY>
 LuxStatus launch(const NormArgs& a, hipStream_t st) {
-    if (a.x_dt == DT_F32) launch_x<NT, V, DT_F32>(a, st);
-    else if (a.x_dt == DT_F16) launch_x<NT, V, DT_F16>(a, st);
-    else launch_x<NT, V, DT_BF16>(a, st);
+    if (a.x_dt == DT_F32) launch_x<NT, V, AWAY, DT_F32>(a, st);
+    else if (a.x_dt == DT_F16) launch_x<NT, V, AWAY, DT_F16>(a, st);
+    else launch_x<NT, V, AWAY, DT_BF16>(a, st);
     return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
+}
+
+// many rows: by the vectors of 8 in a row
+template <bool AWAY>
+LuxStatus launch_many(const NormArgs& a, int v, hipStream_t st) {
+    if (v <= 64) return launch<64, 1, AWAY>(a, st);
+    if (v <= 64 * 2) return launch<64, 2, AWAY>(a, st);
+    if (v <= 128 * 2) return launch<128, 2, AWAY>(a, st);
+    if (v <= 128 * 3) return launch<128, 3, AWAY>(a, st);
+    if (v <= 256 * 2 && a.x_dt != DT_F32) return launch<256, 2, AWAY>(a, st);
+    if (v <= 512) return launch<512, 1, AWAY>(a, st);
+    if (v <= 256 * 3) return launch<256, 3, AWAY>(a, st);
+    if (v <= 512 * 2) return launch<512, 2, AWAY>(a, st);
+    if (v <= 512 * 3) return launch<512, 3, AWAY>(a, st);
+    return launch<1024, 2, AWAY>(a, st);
 }
 
 }  // namespace
@@ -306,24 +327,21 @@ LuxStatus launch(const NormArgs& a, hipStream_t st) {
 // 2100 f16: 128 x 3 43.9, 256 x 2 49.6; of 4096 bf16: 256 x 2 54.9, 512 x 1
 // 56.2; of 4096 f32: 512 x 1 97, 256 x 2 104; 2048 rows of 16384 f16: 1024 x 2
 // 63.7, 512 x 4 78).
+// Results that the L2s (32 MB) cannot hold leave past the caches: 4096 rows of
+// 4608 bf16 51.6 us with plain stores, 34.6 so, 8192 of 2100 f16 44.2 and 31.7,
+// 8192 of 4096 bf16 54.4 and 53.5.
 LuxStatus launch_block_norm(const NormArgs& a, hipStream_t st) {
-    const int v = (a.D + 7) / 8;  // vectors of a row
-    if (v <= 64) return launch<64, 1>(a, st);
-    if (a.T > 512) {
-        if (v <= 64 * 2) return launch<64, 2>(a, st);
-        if (v <= 128 * 2) return launch<128, 2>(a, st);
-        if (v <= 128 * 3) return launch<128, 3>(a, st);
-        if (v <= 256 * 2 && a.x_dt != DT_F32) return launch<256, 2>(a, st);
-        if (v <= 512) return launch<512, 1>(a, st);
-        if (v <= 256 * 3) return launch<256, 3>(a, st);
-        if (v <= 512 * 2) return launch<512, 2>(a, st);
-        if (v <= 512 * 3) return launch<512, 3>(a, st);
+    const int v = (a.D + 7) / 8;
+    if (a.T > 512 && v <= 1024 * 2) {
+        const int64_t each = (a.h ? (a.r_dt == DT_F32 ? 4 : 2) : 0) + (a.out ? (a.x_dt == DT_F32 ? 4 : 2) : 0);
+        return each * a.T * a.D >= (32 << 20) ? launch_many<true>(a, v, st) : launch_many<false>(a, v, st);
     }
-    if (v <= 512) return launch<512, 1>(a, st);
-    if (v <= 1024) return launch<1024, 1>(a, st);
-    if (v <= 1024 * 2) return launch<1024, 2>(a, st);
-    if (v <= 1024 * 4) return launch<1024, 4>(a, st);
-    return launch<0, 0>(a, st);
+    if (v <= 64) return launch<64, 1, false>(a, st);
+    if (v <= 512) return launch<512, 1, false>(a, st);
+    if (v <= 1024) return launch<1024, 1, false>(a, st);
+    if (v <= 1024 * 2) return launch<1024, 2, false>(a, st);
+    if (v <= 1024 * 4) return launch<1024, 4, false>(a, st);
+    return launch<0, 0, false>(a, st);
 }
 
 }  // namespace lxq

@@ -21,8 +21,7 @@
 // a cut goes through leaves partial (m, l, O) in the workspace, which the last of
 // its blocks to arrive joins.  Bound by HBM.
 #pragma once
-#include "qcommon.h"
-#include "serving.h"
+#include "serving_device.h"
 
 namespace lxq {
 namespace attn {
@@ -50,8 +49,6 @@ struct Params {
     float* part_ml;   // [2 P, rows, 2]
     uint32_t part_o_bytes, part_ml_bytes;
 };
-
-__device__ __forceinline__ int div_by(int t, const DivBy& d) { return (int)(((uint64_t)(uint32_t)t * d.mul) >> (31 + d.sh)); }
 
 // of `units` units, range w of P starts at first(w): the first units % P
 // ranges are one unit longer
@@ -231,6 +228,7 @@ struct Attn {
         for (int c = 0; c < NC; c++) {
             const int d = (4 * c + (lane >> 4)) * E;
             q[c] = *reinterpret_cast<const u4h*>(p + (FULL || d < dim(a) ? d * ES : 0));
+            if (!FULL && d >= dim(a)) q[c] = u4{0, 0, 0, 0};
         }
     }
 
@@ -263,7 +261,6 @@ struct Attn {
         }
     }
 
-    // (channels past head_dim: keys of 0, against values of q that count anyway)
     __device__ __forceinline__ void scores(f4* s) const {
 #pragma unroll
         for (int i = 0; i < SUB; i++) s[i] = f4{0.f, 0.f, 0.f, 0.f};
@@ -609,21 +606,6 @@ __global__ __launch_bounds__(64 * NW, (kWaves<DP>)) void attn_pair_kernel(Params
     bool primed = false;
     x.run(p.a, Piece{r, h, qt, w, (ex.end - ex.base + A::kTile - 1) / A::kTile, ex}, Piece{}, primed);
     x.join(p, r, h, qt, -1, attn_lds);
-}
-
-// inclusive sum over the wave's lanes: shifts within rows of 16, then each
-// row's last lane to the rows behind it
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
-}
-__device__ __forceinline__ int wave_scan(int v) {
-    v = dpp_add<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
-    v = dpp_add<0x112, 0xF>(v);
-    v = dpp_add<0x114, 0xF>(v);
-    v = dpp_add<0x118, 0xF>(v);
-    v = dpp_add<0x142, 0xA>(v);     // row_bcast:15 into rows 1 and 3
-    return dpp_add<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
 }
 
 // requests in front of unit pos / HQ, found by each wave for itself: lane i sums

@@ -7,21 +7,24 @@
 // per token finds its request (the last one that starts at or before it) and
 // writes its slot; the token at the start of a page that its request did not
 // hold writes the page's table entry: a new page's first token is new itself.
-#include "qcommon.h"
-#include "serving.h"
+//
+// All latency.  Up to kMost requests every block sums them all by itself, into
+// LDS, and goes on to its tokens: one launch and two trips to memory.  More are
+// summed by a launch of their own.
+#include "serving_device.h"
 
 namespace lxq {
 namespace {
 
-__device__ __forceinline__ int div_by(int t, const DivBy& d) { return (int)(((uint64_t)(uint32_t)t * d.mul) >> (31 + d.sh)); }
+// where the first new token's page is in the list: 0 before the list
+__device__ __forceinline__ int head_of(const PlanArgs& a) { return a.head[0] < 0 ? 0 : a.head[0]; }
 
 struct Request {
     int seq, fresh, have, need;
 };
-__device__ __forceinline__ Request request_at(const PlanArgs& a, int r) {
+__device__ __forceinline__ Request request_of(const PlanArgs& a, int s, int n) {
     Request q;
     const int cap = a.columns * a.page;  // below 2^31
-    const int s = a.seq[r], n = a.fresh[r];
     q.seq = s < 0 ? 0 : s > cap ? cap : s;
     q.fresh = n < 0 ? 0 : n;
     q.have = div_by(q.seq, a.div);
@@ -34,15 +37,14 @@ __device__ __forceinline__ Request request_at(const PlanArgs& a, int r) {
     return q;
 }
 
+__device__ __forceinline__ Request request_at(const PlanArgs& a, int r) { return request_of(a, a.seq[r], a.fresh[r]); }
+
 // inclusive sums of two values over a block of NW waves; `total`: the block's
 template <int NW>
 __device__ __forceinline__ void block_scan(int& x, int& y, int& tx, int& ty, int (*part)[2]) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int px = __shfl_up(x, d), py = __shfl_up(y, d);
-        if (lane >= d) { x += px; y += py; }
-    }
+    x = wave_scan(x);
+    y = wave_scan(y);
     __syncthreads();  // the last round's readers
     if (lane == 63) { part[w][0] = x; part[w][1] = y; }
     __syncthreads();
@@ -71,8 +73,7 @@ __device__ __forceinline__ void write_request(const PlanArgs& a, int r, const Re
 }
 
 // token t of request r, whose tokens start at `start` and pages at `first`
-__device__ __forceinline__ void write_token(const PlanArgs& a, int t, int r, int start, int64_t first) {
-    const Request q = request_at(a, r);
+__device__ __forceinline__ void write_token(const PlanArgs& a, int t, int r, const Request& q, int start, int64_t first) {
     const int64_t p64 = (int64_t)q.seq + (t - start);
     const int pos = (int)p64;
     const int got = pages_there(first, q.need, a.F);
@@ -101,10 +102,91 @@ __device__ __forceinline__ void write_no_token(const PlanArgs& a, int t) {
     if (a.request) a.request[t] = -1;
 }
 
-// first launch: one block walks the requests
+// one launch for up to kMost requests; thread i sums a stretch of them
+constexpr int kMost = 2048;
+__global__ __launch_bounds__(256) void plan_kernel(PlanArgs a) {
+    __shared__ int part[4][2];
+    __shared__ int starts[kMost + 1], firsts[kMost], seqs[kMost];
+    constexpr int kEach = kMost / 256;
+    const int each = (a.R + 255) / 256, r0 = (int)threadIdx.x * each;
+    const int head = head_of(a);
+    int s[kEach], n[kEach];
+    auto load = [&](int i) {
+        const int r = r0 + i;
+        s[i] = r < a.R ? a.seq[r] : 0;
+        n[i] = r < a.R ? a.fresh[r] : 0;
+    };
+    load(0);
+    if (each > 1) {  // no branch between them: one trip for all
+#pragma unroll
+        for (int i = 1; i < kEach; i++) {
+            s[i] = n[i] = 0;
+            if (i < each) load(i);
+        }
+    }
+    int tokens = 0, pages = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        if (i >= each) break;
+        const Request q = request_of(a, s[i], n[i]);
+        tokens += q.fresh;
+        pages += q.need;
+    }
+    int x = tokens, y = pages, all_tokens, all_pages;
+    block_scan<4>(x, y, all_tokens, all_pages, part);
+    int start = x - tokens, first = y - pages, past_all = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        if (i >= each) break;
+        const int r = r0 + i;
+        if (r < a.R) {
+            const Request q = request_of(a, s[i], n[i]);
+            starts[r] = start;
+            firsts[r] = first;
+            seqs[r] = q.seq;
+            if (blockIdx.x == 0) {
+                int got, past;
+                write_request(a, r, q, start, (int64_t)head + first, got, past);
+                past_all += past;
+            }
+            start += q.fresh;
+            first += q.need;
+        }
+    }
+    if (threadIdx.x == 0) starts[a.R] = all_tokens;
+    if (blockIdx.x == 0) {
+        int none = 0, tp, tn;
+        block_scan<4>(past_all, none, tp, tn, part);
+        if (threadIdx.x == 0) {
+            const int got = pages_there(head, all_pages, a.F);
+            a.starts[a.R] = all_tokens;
+            a.counts[0] = head + got;
+            a.counts[1] = all_tokens;
+            a.counts[2] = all_pages - got;
+            a.counts[3] = tp;
+        }
+    }
+    __syncthreads();
+    const int64_t most = all_tokens > a.T ? all_tokens : a.T, step = (int64_t)gridDim.x * 256;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < most; t += step) {
+        if (t >= all_tokens) {
+            write_no_token(a, (int)t);
+            continue;
+        }
+        int lo = 0, hi = a.R - 1;  // the last request that starts at or before t: none after it is empty
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (starts[mid] <= (int)t) lo = mid;
+            else hi = mid - 1;
+        }
+        write_token(a, (int)t, lo, request_of(a, seqs[lo], starts[lo + 1] - starts[lo]), starts[lo], (int64_t)head + firsts[lo]);
+    }
+}
+
+// more requests, first launch: one block walks the requests
 __global__ __launch_bounds__(1024) void plan_requests_kernel(PlanArgs a) {
     __shared__ int part[16][2];
-    const int head = a.head[0] < 0 ? 0 : a.head[0];
+    const int head = head_of(a);
     int tokens = 0;
     int64_t pages = 0;
     int got_all = 0, past_all = 0;
@@ -138,7 +220,7 @@ __global__ __launch_bounds__(1024) void plan_requests_kernel(PlanArgs a) {
 
 // second launch: a thread per token
 __global__ __launch_bounds__(256) void plan_tokens_kernel(PlanArgs a) {
-    const int head = a.head[0] < 0 ? 0 : a.head[0];
+    const int head = head_of(a);
     const int total = a.starts[a.R];
     const int64_t most = total > a.T ? total : a.T, step = (int64_t)gridDim.x * 256;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < most; t += step) {
@@ -152,17 +234,22 @@ __global__ __launch_bounds__(256) void plan_tokens_kernel(PlanArgs a) {
             if (a.starts[mid] <= (int)t) lo = mid;
             else hi = mid - 1;
         }
-        write_token(a, (int)t, lo, a.starts[lo], (int64_t)head + a.ws[lo]);
+        write_token(a, (int)t, lo, request_at(a, lo), a.starts[lo], (int64_t)head + a.ws[lo]);
     }
 }
 
 }  // namespace
 
 LuxStatus launch_paged_plan(const PlanArgs& a, hipStream_t st) {
-    if ((size_t)a.R > a.ws_words) return LuxStatus::NotSupported;
-    hipLaunchKernelGGL(plan_requests_kernel, dim3(1), dim3(1024), 0, st, a);
-    const int blocks = a.T < 256 * 2048 ? (a.T + 255) / 256 : 2048;
-    hipLaunchKernelGGL(plan_tokens_kernel, dim3(blocks < 1 ? 1 : blocks), dim3(256), 0, st, a);
+    const int blocks = a.T < 256 * 1024 ? (a.T + 255) / 256 : 1024;
+    const dim3 g(blocks < 1 ? 1 : blocks);
+    if (a.R <= kMost) {
+        hipLaunchKernelGGL(plan_kernel, g, dim3(256), 0, st, a);
+    } else {
+        if ((size_t)a.R > a.ws_words) return LuxStatus::NotSupported;
+        hipLaunchKernelGGL(plan_requests_kernel, dim3(1), dim3(1024), 0, st, a);
+        hipLaunchKernelGGL(plan_tokens_kernel, g, dim3(256), 0, st, a);
+    }
     return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
 }
 
