@@ -113,6 +113,21 @@ __device__ __forceinline__ float wave_max(float v) {
     return fmaxf(fmaxf(lane_f(v, 0), lane_f(v, 16)), fmaxf(lane_f(v, 32), lane_f(v, 48)));
 }
 
+// tanh(y) from z = 2 y log2 e: 1 - 2 / (1 + exp2(z)), off by 2^-22 at most.  In f32
+// scores that is more than the rest of the kernel is off where y is small:
+// there the series up to y^11, whose next term is below 2^-28 of y at 0.3.
+template <int T>
+__device__ __forceinline__ float tanh_of(float z) {
+    const float far = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z)), -2.f, 1.f);
+    if constexpr (T != DT_F32) return far;
+    const float y = z * (0.5f * kLn2), q = y * y;
+    float near = fmaf(q, -1382.f / 155925.f, 62.f / 2835.f);
+    near = fmaf(q, near, -17.f / 315.f);
+    near = fmaf(q, near, 2.f / 15.f);
+    near = fmaf(q, near, -1.f / 3.f);
+    return fabsf(y) < 0.3f ? fmaf(y * q, near, y) : far;
+}
+
 // max / sum over the four lanes that hold one query's tokens: both halves of a
 // row or wave swap are the pair's values, in either order
 __device__ __forceinline__ float group_max(float v) {
@@ -275,12 +290,10 @@ struct Attn {
     __device__ __forceinline__ void soften(const AttnArgs& a, f4* s, uint32_t bits) {
         const int g = (threadIdx.x & 63) >> 4;
         if (a.softcap > 0.f) {
-            // cap tanh(y) = cap (1 - 2 / (1 + exp(2 y))), off by 2^-22 cap at most
 #pragma unroll
             for (int i = 0; i < SUB; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    s[i][j] = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[i][j] * a.scale)), -2.f * a.softcap, a.softcap);
+                for (int j = 0; j < 4; j++) s[i][j] = a.softcap * tanh_of<T>(s[i][j] * a.scale);
         } else {
 #pragma unroll
             for (int i = 0; i < SUB; i++) s[i] *= a.scale;
