@@ -106,7 +106,8 @@ typedef struct lux_paged_append_args {
  * A request with no position gives out = 0 and lse = -infinity.  Cache places
  * that no position of a request names are never part of its result, whatever
  * they hold.  Scores, sums and the running statistics are fp32; with 16-bit
- * types exp(s - max) is rounded to that type before the product with v.
+ * types exp(s - max) enters the product with v as the sum of two values of
+ * that type.
  * head_dim: a multiple of 8, at most 256; heads a multiple of kv_heads;
  * num_pages * kv_heads * page_size below 2^31; the caches start on 16 bytes.
  */

@@ -6,9 +6,9 @@ Tolerances.  u = 2^-24, 2^-11, 2^-8 is the rounding of one value of f32, f16,
 bf16.  Attention: a score is a sum of D exact products (16-bit types) or of D
 fused multiply-adds in f32, so it is off by at most (D + 8) 2^-24 scale
 sum |q k|, and its exp by that much relative, as is the sum of exps; 64 2^-24
-covers exp2, the rescalings and the sums over a few hundred terms per lane; the
-rounding of exp(s - max) to the type adds u.  All of these weigh values of at
-most max |v|.  Norms: a mean over a row is a tree of at most 64 serial additions
+covers exp2, the rescalings and the sums over a few hundred terms per lane; exp(s -
+max) as the sum of two values of the type is off by u^2 of itself (and in f16 by half
+of its smallest step).  All of these weigh values of at most max |v|.  Norms: a mean over a row is a tree of at most 64 serial additions
 per thread and 20 more, 84 2^-24 relative to the sum of magnitudes, taken twice
 in a layer norm; 2^-24 times 256 covers it with the square root and the products.
 """
@@ -21,6 +21,7 @@ import torch
 F32, F16, BF16 = 0, 1, 2
 TORCH = {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16}
 ROUND = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
+WEIGHT_ROUND = {F32: 0.0, F16: 2.0 ** -22 + 2.0 ** -25, BF16: 2.0 ** -16}
 
 
 class Device:
@@ -108,8 +109,7 @@ def check_attention(got, lse, ref, v_max, dtype, what):
     R, H, D = out.shape
     got = got.double().view(R, H, D)
     assert torch.isfinite(got).all(), f"{what}: non-finite output"
-    p_round = ROUND[dtype] if dtype != F32 else 0.0
-    bound = (tol + p_round)[..., None] * v_max + ROUND[dtype] * out.abs()
+    bound = (tol + WEIGHT_ROUND[dtype])[..., None] * v_max + ROUND[dtype] * out.abs()
     if dtype == F16:
         bound = bound + 2.0 ** -25
     bad = (got - out).abs() > bound
