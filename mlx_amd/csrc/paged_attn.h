@@ -149,7 +149,7 @@ struct Piece {
     Extent ex;
 };
 
-// T: type of q, cache and out; DP: head_dim rounded up to 64, 128 or 256;
+// T: type of q, cache and out; DP: head_dim, or that rounded up to 64, 128 or 256;
 // FULL: head_dim is DP; WHOLE: pages hold whole runs of 16 tokens, so that a run
 // has one page and its rows one scalar base (else each lane finds its token's
 // row and the others take it from there); ONCE: cache loads that leave no copy
@@ -158,7 +158,7 @@ struct Attn {
     static constexpr int ES = T == DT_F32 ? 4 : 2, E = 16 / ES;  // bytes; elements per 16 bytes
     static constexpr int SUB = T == DT_F32 ? 1 : 2, kTile = 16 * SUB;
     static constexpr int NC = DP / (4 * E);                  // 16-byte chunks of a key row per lane
-    static constexpr int VE = E < DP / 16 ? E : DP / 16;     // channels of a value row per lane and load
+    static constexpr int VE = DP == 192 ? 4 : E < DP / 16 ? E : DP / 16;  // channels of a value row per lane and load
     static constexpr int NV = DP / (16 * VE);                // loads per value row
     static constexpr int VW = VE * ES / 4;                   // their words
     static constexpr int kUnit = kTile * NW;
@@ -842,7 +842,8 @@ LuxStatus launch_t(const AttnArgs& a, hipStream_t st) {
     p.a.scale = a.softcap > 0.f ? 2.f * kLog2e * a.scale / a.softcap : kLog2e * a.scale;
     p.a.softcap = a.softcap * kLog2e;
     if (a.D <= 64) return launch_dp<T, 64>(p, st);
-    return a.D <= 128 ? launch_dp<T, 128>(p, st) : launch_dp<T, 256>(p, st);
+    if (a.D <= 128) return launch_dp<T, 128>(p, st);
+    return a.D == 192 ? launch_full<T, 192, true>(p, st) : launch_dp<T, 256>(p, st);
 }
 
 extern template LuxStatus launch_t<DT_F32>(const AttnArgs&, hipStream_t);
