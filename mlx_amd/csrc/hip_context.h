@@ -24,8 +24,8 @@ struct HipContext {
     // launches on ws so far: each GEMM launch gets the next number as its
     // epoch (the split tiles meet by it; never 0)
     uint32_t epoch = 0;
-    // arrival counters of the attention's split pairs, zero between launches;
-    // without them the attention is not split
+    // arrival counters of the attention's split pairs (three per range), zero
+    // between launches; without them the attention is not split
     void* counts = nullptr;
 };
 constexpr int kCountWords = 2048;

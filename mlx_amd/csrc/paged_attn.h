@@ -19,7 +19,15 @@
 // few or too uneven for the card, the tokens of all pairs are laid end to end
 // in units of NW tiles and cut into P equal ranges, one per block: a pair that
 // a cut goes through leaves partial (m, l, O) in the workspace, which the last of
-// its blocks to arrive joins.  Bound by HBM.
+// its blocks to arrive joins.  At its last tile of a pair a wave already loads
+// the first of the next one (256 requests up to 1024 tokens 107.5 us without,
+// 103 with).
+//
+// Bound by HBM where the cache is long: 8 requests of 131072 tokens, 8 heads of
+// 128 bf16 (4.3 GB) in 624 us, 6.9 TB/s; 64 ragged ones up to 8192 (1.1 GB) 181
+// us, 6.2 TB/s.  Short calls are a chain of trips to memory (lengths, table,
+// keys, partial results, counter, their join): one request of 4096 tokens, 32
+// heads on 8 of 128 f16 (17 MB) 9.6 us.
 #pragma once
 #include "serving_device.h"
 
@@ -44,7 +52,6 @@ struct Params {
     int HQ;           // heads of keys times query tiles of a group
     int QT, rows;     // query tiles of a group; rows of a tile kept in partial results
     DivBy P, by_hq;   // ranges; division by HQ
-    bool join;        // the ranges join the pairs they share
     float* part_o;    // [2 P, rows, D]
     float* part_ml;   // [2 P, rows, 2]
     uint32_t part_o_bytes, part_ml_bytes;
@@ -469,10 +476,7 @@ struct Attn {
                 acc += *reinterpret_cast<const f4*>(lds + (y * p.rows + i) * LS + d) * f;
             }
             if (slot >= 0) {
-                // device scope: the block that joins them may be on another die
-                const uint32_t at = (uint32_t)(slot * p.rows + i);
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, acc), o_rsrc(p), (at * dim(a) + d) * 4, 0, kDevice);
-                if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(top), __float_as_uint(sum)}, ml_rsrc(p), at * 8, 0, kDevice);
+                store_part(p, slot, i, d, acc, top, sum);
             } else {
                 store_row(a, r, h * a.G + qt * 16 + i, d, acc, top, sum);
             }
@@ -487,36 +491,40 @@ struct Attn {
         return __builtin_amdgcn_make_buffer_rsrc(p.part_ml, 0, (int)p.part_ml_bytes, 0x00020000);
     }
 
-    // a pair's items: four channels of a row each
-    __device__ __forceinline__ static int items_of(const AttnArgs& a, int qt) {
-        return (a.G - qt * 16 < 16 ? a.G - qt * 16 : 16) * (dim(a) / 4);
+    // four channels of a row of a partial result, at device scope: the block that
+    // joins it may be on another die
+    __device__ __forceinline__ static void store_part(const Params& p, int slot, int i, int d, f4 acc, float top, float sum) {
+        const uint32_t at = (uint32_t)(slot * p.rows + i);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, acc), o_rsrc(p), (at * dim(p.a) + d) * 4, 0, kDevice);
+        if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(top), __float_as_uint(sum)}, ml_rsrc(p), at * 8, 0, kDevice);
     }
 
-    // Joins the `parts` partial results of items [x0, last) of the pair that
-    // starts in range w0.  A wave takes whole rows of (m, l), a part per lane,
-    // and leaves the parts' weights in LDS; then a thread adds up its item's
-    // four channels, and where the items are fewer than the threads, several
-    // threads share an item's parts and meet in LDS.  Items past NT come with at
-    // most kChunk parts.
-    __device__ __forceinline__ static void finish(const Params& p, int r, int h, int qt, int x0, int last, int w0, int parts, float* lds) {
+    // Joins parts at, at + hop, ... (`parts` of them) of the pair that starts in
+    // range w0 into the result, or (to >= 0) into the partial result in slot
+    // `to`, which may be the first one's.  An item is four channels of a row.  A
+    // wave takes whole rows of (m, l), a part per lane, and leaves the parts'
+    // weights in LDS; then a thread adds up its item, and where the items are
+    // fewer than the threads, several threads share an item's parts and meet in
+    // LDS.  Items past NT come with at most kChunk parts.
+    __device__ __forceinline__ static void finish(const Params& p, int r, int h, int qt, int w0, int at, int hop, int parts, int to,
+                                                  float* lds) {
         const AttnArgs& a = p.a;
         const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
-        const int per = dim(a) / 4, items = last - x0, first = x0;
+        const int rows = a.G - qt * 16 < 16 ? a.G - qt * 16 : 16, per = dim(a) / 4, items = rows * per;
         const int turns = items < NT ? small_div(NT, items) : 1;
         const int turn = turns > 1 ? small_div(threadIdx.x, items) : 0;
-        const int row0 = small_div(x0, per), rows = small_div(last - 1, per) + 1 - row0;
         const __amdgpu_buffer_rsrc_t ro = o_rsrc(p), rm = ml_rsrc(p);
         float* weight = lds;                                       // [16][kChunk]
         float* of_row = lds + 16 * kChunk;                         // [16][4]: maximum, sum, rescaling
         f4* all = reinterpret_cast<f4*>(lds + 16 * (kChunk + 4));  // [NT]
-        for (; x0 < last; x0 += NT) {
+        for (int x0 = 0; x0 < items; x0 += NT) {
             const int x = x0 + (int)threadIdx.x - turn * items;
-            const bool on = x < last && turn < turns;
-            const int i = on ? small_div(x, per) : row0, d = on ? (x - i * per) * 4 : 0;
+            const bool on = x < items && turn < turns;
+            const int i = on ? small_div(x, per) : 0, d = on ? (x - i * per) * 4 : 0;
             f4 acc = {0.f, 0.f, 0.f, 0.f};
             for (int c0 = 0; c0 < parts; c0 += kChunk) {
                 const int n = parts - c0 < kChunk ? parts - c0 : kChunk;
-                const bool weigh = c0 > 0 || x0 == first;
+                const bool weigh = c0 > 0 || x0 == 0;
                 u2 ml[16 / NW];
                 if (weigh)
 #pragma unroll
@@ -524,24 +532,24 @@ struct Attn {
                         const int y = w + k * NW;
                         if (y >= rows) break;
                         ml[k] = __builtin_amdgcn_raw_buffer_load_b64(
-                            rm, lane < n ? (slot(w0, c0 + lane) * p.rows + row0 + y) * 8 : 0x80000000u, 0, kDevice);
+                            rm, lane < n ? (slot(w0, at + (c0 + lane) * hop) * p.rows + y) * 8 : 0x80000000u, 0, kDevice);
                     }
                 // up to kBatch of the thread's parts in flight together, in
                 // groups of 8 as far as there are any
                 constexpr int kBatch = 16;
                 u4 o[kBatch];
-                const uint32_t step = (uint32_t)(p.rows * dim(a)) * 4, hop = 2 * turns * step;
+                const uint32_t step = (uint32_t)(p.rows * dim(a)) * 4, stride = 2 * turns * hop * step;
                 auto load_o = [&](int s0) {
                     int s = s0 + turn;
-                    uint32_t at = (uint32_t)(i * dim(a) + d) * 4 + slot(w0, c0 + s) * step;
+                    uint32_t from = (uint32_t)(i * dim(a) + d) * 4 + slot(w0, at + (c0 + s) * hop) * step;
 #pragma unroll
                     for (int q = 0; q < kBatch; q += 8) {
                         if (s0 + q * turns >= n) break;
 #pragma unroll
                         for (int k = q; k < q + 8; k++) {
                             // past the last: an offset past the end, which reads zeros
-                            o[k] = __builtin_amdgcn_raw_buffer_load_b128(ro, s < n ? at : 0x80000000u, 0, kDevice);
-                            at += hop - (k == 0 && c0 + s == 0 ? step : 0);
+                            o[k] = __builtin_amdgcn_raw_buffer_load_b128(ro, s < n ? from : 0x80000000u, 0, kDevice);
+                            from += stride - (k == 0 && at + (c0 + s) * hop == 0 ? step : 0);
                             s += turns;
                         }
                     }
@@ -564,7 +572,7 @@ struct Attn {
                         }
                     }
                 __syncthreads();
-                acc *= of_row[4 * (i - row0) + 2];
+                acc *= of_row[4 * i + 2];
                 for (int s0 = 0; s0 < n; s0 += kBatch * turns) {
                     if (s0) load_o(s0);
 #pragma unroll
@@ -573,7 +581,7 @@ struct Attn {
 #pragma unroll
                         for (int k = q; k < q + 8; k++) {
                             const int s = s0 + turn + k * turns;
-                            acc += __builtin_bit_cast(f4, o[k]) * weight[(i - row0) * kChunk + (s < kChunk ? s : kChunk - 1)];
+                            acc += __builtin_bit_cast(f4, o[k]) * weight[i * kChunk + (s < kChunk ? s : kChunk - 1)];
                         }
                     }
                 }
@@ -586,8 +594,10 @@ struct Attn {
                     for (int k = 1; k < turns; k++) acc += all[threadIdx.x + k * items];
                 __syncthreads();
             }
-            if (on && turn == 0)
-                store_row(a, r, h * a.G + qt * 16 + i, d, acc, of_row[4 * (i - row0)], of_row[4 * (i - row0) + 1]);
+            if (on && turn == 0) {
+                if (to >= 0) store_part(p, to, i, d, acc, of_row[4 * i], of_row[4 * i + 1]);
+                else store_row(a, r, h * a.G + qt * 16 + i, d, acc, of_row[4 * i], of_row[4 * i + 1]);
+            }
         }
         __syncthreads();
     }
@@ -668,15 +678,40 @@ struct Requests {
     }
 };
 
-// the ranges that hold a pair's units [from, from + n)
+// The ranges that hold a pair's units [from, from + n).  Parts of up to 256 KB are
+// joined at once; more in groups of about their square root, each by the last of
+// its ranges to arrive, and the groups by the last group (16 heads of 256 f16 on
+// one, a request of 65536 tokens beside 63 of 20: some 250 parts of 16 KB, 92 us
+// at once, 35 in groups).
 struct Parts {
     int w0, count;
     __device__ __forceinline__ Parts(const Ranges& ranges, int from, int n) : w0(ranges.of(from)) {
         count = ranges.of(from + n - 1) - w0 + 1;
     }
 };
+// parts of a group: all, or a power of two
+__device__ __forceinline__ int group_of(const Params& p, int count) {
+    if (count * (int64_t)(p.rows * p.a.D * 4) <= 256 * 1024) return count;
+    int n = 8;
+    while (n * n < count) n *= 2;
+    return n;
+}
 
-// range blockIdx.x of P; p.join: the last of a cut pair's ranges to arrive joins it
+// thread 0 counts one in; true for all threads of the last of `all`, which
+// leaves the counter at 0
+__device__ __forceinline__ bool count_in(uint32_t* c, int all, int* word) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's partial results are out
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const bool last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(all - 1);
+        if (last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *word = last;
+    }
+    __syncthreads();
+    return uniform(*word);
+}
+
+// range blockIdx.x of P
 template <int T, int DP, bool FULL, bool WHOLE, bool ONCE, int NW>
 __global__ __launch_bounds__(64 * NW, (kWaves<DP>)) void attn_range_kernel(Params p) {
     using A = Attn<T, DP, FULL, WHOLE, ONCE, NW>;
@@ -692,7 +727,7 @@ __global__ __launch_bounds__(64 * NW, (kWaves<DP>)) void attn_range_kernel(Param
     Extent ex = extent_of(a, len);
     int n = units_of(ex, A::kUnit);
     int hq = (int)((uint32_t)(pos - before * p.HQ) / (uint32_t)n), u = pos - before * p.HQ - hq * n;
-    bool at_start = true, primed = false;
+    bool primed = false;
     A x;
     // the piece of pair (r, hq) from unit u on, as far as the range goes
     auto piece = [&] {
@@ -701,7 +736,8 @@ __global__ __launch_bounds__(64 * NW, (kWaves<DP>)) void attn_range_kernel(Param
         return Piece{r, h, hq - h * p.QT, u * NW + w, last < tiles ? last : tiles, ex};
     };
     Piece c = piece();
-    int r0 = 0, h0 = 0, qt0 = 0, w0 = 0, count0 = 0, r1 = 0, h1 = 0, qt1 = 0, w1 = 0, count1 = 0;
+    int r0 = 0, h0 = 0, qt0 = 0, w0 = 0, n0 = 0, r1 = 0, h1 = 0, qt1 = 0, w1 = 0, n1 = 0;  // the pairs to join, of n parts
+    int* word = reinterpret_cast<int*>(attn_lds + A::lds_floats(p.rows));
     while (pos < end) {
         const int from = pos - u, all = n, u0 = u, u1 = u + (end - pos) < n ? u + (end - pos) : n;
         const bool part = u0 > 0 || u1 < n;
@@ -715,60 +751,43 @@ __global__ __launch_bounds__(64 * NW, (kWaves<DP>)) void attn_range_kernel(Param
         const Piece next = piece();  // at the range's end: no tiles
         x.run(a, c, next, primed);
         x.join(p, c.r, c.h, c.qt, !part ? -1 : 2 * me + (u0 == 0), attn_lds);
-        if (p.join && part) {
-            // only one pair goes past the end of a range, so its first range
-            // numbers its counter
+        if (part) {
+            // counters: P for the pairs that start in a range and go past its
+            // end (only one does) and its first group, P for the group that
+            // starts in a range behind that one, P for the pairs' groups
             const Parts parts(ranges, from, all);
-            int* last = reinterpret_cast<int*>(attn_lds + A::lds_floats(p.rows));
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                uint32_t* c = a.count + parts.w0;
-                const bool l = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(parts.count - 1);
-                if (l) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                *last = l;
+            const int group = group_of(p, parts.count);
+            int g = 0, in_group = parts.count;
+            if (group < parts.count) {
+                g = (me - parts.w0) & -group;
+                in_group = parts.count - g < group ? parts.count - g : group;
             }
-            __syncthreads();
-            if (uniform(*last)) {
+            if (count_in(a.count + (g ? p.P.d + parts.w0 + g : parts.w0), in_group, word)) {
                 // joined at the end of the range, when the tiles' registers
                 // are free; a range has at most two cut pairs
-                if (at_start) r0 = c.r, h0 = c.h, qt0 = c.qt, w0 = parts.w0, count0 = parts.count;
-                else r1 = c.r, h1 = c.h, qt1 = c.qt, w1 = parts.w0, count1 = parts.count;
+                if (u0 > 0) r0 = c.r, h0 = c.h, qt0 = c.qt, w0 = parts.w0, n0 = parts.count;
+                else r1 = c.r, h1 = c.h, qt1 = c.qt, w1 = parts.w0, n1 = parts.count;
             }
             __syncthreads();
         }
-        at_start = false;
         c = next;
     }
-    if (p.join) {
 #pragma unroll 1
-        for (int i = 0; i < 2; i++) {
-            if (count0) A::finish(p, r0, h0, qt0, 0, A::items_of(a, qt0), w0, count0, attn_lds);
-            r0 = r1, h0 = h1, qt0 = qt1, w0 = w1, count0 = count1;
+    for (int i = 0; i < 2; i++) {
+        if (n0) {
+            const int group = group_of(p, n0);
+            int parts = n0, hop = 1;
+            if (group < n0) {
+                const int g = (me - w0) & -group, groups = (n0 + group - 1) / group;
+                A::finish(p, r0, h0, qt0, w0, g, 1, n0 - g < group ? n0 - g : group, (int)slot(w0, g), attn_lds);
+                parts = count_in(a.count + 2 * p.P.d + w0, groups, word) ? groups : 0;
+                hop = group;
+            }
+            if (parts) A::finish(p, r0, h0, qt0, w0, 0, hop, parts, -1, attn_lds);
         }
+        r0 = r1, h0 = h1, qt0 = qt1, w0 = w1, n0 = n1;
+        n1 = 0;
     }
-}
-
-// second launch: block (x, y) joins the y-th kJoinItems items of pair x, if a cut
-// went through it
-constexpr int kJoinItems = 32;
-template <int T, int DP, bool FULL, int NW>
-__global__ __launch_bounds__(64 * NW) void attn_join_kernel(Params p) {
-    using A = Attn<T, DP, FULL, true, false, NW>;
-    __shared__ __attribute__((aligned(16))) float lds[A::kFinish];
-    const AttnArgs& a = p.a;
-    const int r = blockIdx.x / p.HQ, hq = blockIdx.x - r * p.HQ, h = hq / p.QT, qt = hq - h * p.QT;
-    const int x0 = blockIdx.y * kJoinItems, items = A::items_of(a, qt);
-    if (x0 >= items) return;
-    const Requests requests(a, A::kUnit);
-    const Ranges ranges(requests.all * p.HQ, p.P);
-    const int stretch = r / requests.each;
-    int before = __builtin_amdgcn_readlane(requests.through - requests.mine, stretch);
-    for (int i = stretch * requests.each; i < r; i++) before += units_of(extent_at(a, i), A::kUnit);
-    const int n = units_of(extent_at(a, r), A::kUnit);
-    const Parts parts(ranges, before * p.HQ + hq * n, n);
-    if (parts.count > 1)
-        A::finish(p, r, h, qt, x0, x0 + kJoinItems < items ? x0 + kJoinItems : items, parts.w0, parts.count, lds);
 }
 
 template <int T, int DP, bool FULL, bool WHOLE, bool ONCE>
@@ -789,7 +808,7 @@ LuxStatus launch_d(Params& p, hipStream_t st) {
     int P = kWaves<DP> * p.a.cus;
     const size_t one = (size_t)p.rows * (p.a.D + 2) * 2 * 4;
     if ((size_t)P * one > p.a.ws_bytes) P = (int)(p.a.ws_bytes / one);
-    if (P > p.a.counts) P = p.a.counts;
+    if (P > p.a.counts / 3) P = p.a.counts / 3;
     const int64_t longest = ((int64_t)p.a.columns * p.a.page + A::kUnit - 1) / A::kUnit + 1;  // units of a pair
     const bool whole = P < 2 || longest <= 2 || longest * pairs >= (1ll << 31);
     if (whole) {
@@ -802,14 +821,7 @@ LuxStatus launch_d(Params& p, hipStream_t st) {
     p.part_ml_bytes = (uint32_t)P * 2 * p.rows * 8;
     p.part_o = p.part_ml + p.part_ml_bytes / 4;
     p.part_o_bytes = (uint32_t)P * 2 * p.rows * p.a.D * 4;
-    // one block joins a pair's parts within the launch, unless they are so
-    // many bytes that a second launch over more blocks is sooner done
-    const int64_t parts = longest < P / pairs ? longest : P / pairs;
-    p.join = parts * p.rows * p.a.D * 4 <= 256 * 1024;
     hipLaunchKernelGGL(range, dim3(P), dim3(64 * NW), lds, st, p);
-    if (!p.join)
-        hipLaunchKernelGGL((attn_join_kernel<T, DP, FULL, NW>),
-                           dim3((unsigned)pairs, (unsigned)((p.rows * p.a.D / 4 + kJoinItems - 1) / kJoinItems)), dim3(64 * NW), 0, st, p);
     return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
 }
 

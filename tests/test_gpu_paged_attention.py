@@ -117,6 +117,14 @@ def test_long_and_ragged(ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_pairs_of_very_many_parts(ctx, dtype):
+    """Wide partial results of one pair over most of the card's ranges, alone and beside short requests."""
+    check(ctx, 260 + dtype, dtype, [9000], 16, 1, 256, 32, poison=False)
+    check(ctx, 263 + dtype, dtype, [5, 0, 20000, 17, 1, 300] + [40] * 20, 12, 1, 256, 16, poison=False)
+    check(ctx, 266 + dtype, dtype, [30000, 2], 16, 2, 128, 64, poison=False)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_many_short_requests(ctx, dtype):
     gen = torch.Generator().manual_seed(9)
     check(ctx, 270 + dtype, dtype, torch.randint(0, 90, (700,), generator=gen).tolist(), 2, 1, 64, 16)
