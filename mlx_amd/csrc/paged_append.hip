@@ -3,8 +3,9 @@
 //
 // A copy with at most one rounding.  A thread moves 8 elements of a token's keys
 // and the same 8 of its values; consecutive threads take a token's row in
-// order, so both sides run in whole lines.  Bound by HBM, and by the launch
-// where there are few tokens.
+// order, so both sides run in whole lines.  Bound by HBM (8192 tokens of 8 heads
+// of 128, f32 to f16, 101 MB: 15.9 us, 6.3 TB/s with part of the input cached),
+// and by the launch where there are few tokens (64 tokens, bf16: 3.6 us).
 #include "serving_device.h"
 
 namespace lxq {

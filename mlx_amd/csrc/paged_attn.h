@@ -680,9 +680,10 @@ struct Requests {
 
 // The ranges that hold a pair's units [from, from + n).  Parts of up to 256 KB are
 // joined at once; more in groups of about their square root, each by the last of
-// its ranges to arrive, and the groups by the last group (16 heads of 256 f16 on
-// one, a request of 65536 tokens beside 63 of 20: some 250 parts of 16 KB, 92 us
-// at once, 35 in groups).
+// its ranges to arrive, and the groups by the last group.  16 heads of 256 f16 on
+// one, parts of 16 KB: a request of 65536 tokens beside 63 of 20 (some 250 parts)
+// 92 us at once, 35 in groups; 4 of 16384 (64 parts) 32.8 and 26.3; 10 (26 parts)
+// 47.1 and 48.1; 16 (16 parts) 53.4 and 57.2.
 struct Parts {
     int w0, count;
     __device__ __forceinline__ Parts(const Ranges& ranges, int from, int n) : w0(ranges.of(from)) {
