@@ -107,7 +107,9 @@ typedef struct lux_paged_append_args {
  * that no position of a request names are never part of its result, whatever
  * they hold.  Scores, sums and the running statistics are fp32; with 16-bit
  * types exp(s - max) enters the product with v as the sum of two values of
- * that type.
+ * that type, neither of them 0 (in f16 from 2^-38 of the largest on).  So an
+ * infinite value in a place that counts is the channel's result, two opposite
+ * ones NaN.
  * head_dim: a multiple of 8, at most 256; heads a multiple of kv_heads;
  * num_pages * kv_heads * page_size below 2^31; the caches start on 16 bytes.
  */

@@ -102,6 +102,20 @@ __device__ __forceinline__ f4 mfma_qk(const u4& k, const u4& q, f4 c) {
     }
 }
 
+// two values >= 0 of the type, of x and y without their last bits
+template <int T>
+__device__ __forceinline__ uint32_t cut2(float x, float y) {
+    if constexpr (T == DT_F16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+    else return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+}
+// the type's smallest value (bf16: its smallest normal one) where they are below it
+template <int T>
+__device__ __forceinline__ uint32_t least2(uint32_t v) {
+    typedef uint16_t h2 __attribute__((ext_vector_type(2)));
+    constexpr uint16_t least = T == DT_F16 ? 0x0001 : 0x0080;
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(h2, v), h2{least, least}));
+}
+
 // slot of the s-th part of a pair that starts in range w0: a range keeps the part
 // that its first units continue in slot 2 w, the one that its last units start in
 // slot 2 w + 1
@@ -364,17 +378,21 @@ struct Attn {
                     for (int t = 0; t < 4; t++)
                         o[c][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[t][c][e]), s[0][t], o[c][e], 0, 0, 0);
         } else {
-            // the weights as the sum of two values of the type (one alone is off
+            // The weights as the sum of two values of the type (one alone is off
             // by as much as the output's own rounding: 8 requests of 131072
-            // tokens bf16 2.3e-3 off in 64 bits, 1.7e-3 so, 621.8 and 622.8 us)
+            // tokens bf16 2.3e-3 off in 64 bits, 1.7e-3 so, 621.8 and 622.8 us).
+            // Both are above 0, so that an infinite value of v stays one: the
+            // first is cut, not rounded, and neither is below the type's smallest
+            // (bf16: normal) value, a weight of 2^-38 in f16 and 2^-126 in bf16.
             u4 p[2];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float x = s[i / 2][i % 2 * 2], y = s[i / 2][i % 2 * 2 + 1];
-                p[0][i] = pack2<T>(x, y);
-                const float hx = T == DT_F16 ? f16_to_f32(p[0][i] & 0xffffu) : __uint_as_float(p[0][i] << 16);
-                const float hy = T == DT_F16 ? f16_to_f32(p[0][i] >> 16) : __uint_as_float(p[0][i] & 0xffff0000u);
-                p[1][i] = pack2<T>(x - hx, y - hy);
+                const uint32_t high = cut2<T>(x, y);
+                p[0][i] = least2<T>(high);
+                const float hx = T == DT_F16 ? f16_to_f32(high & 0xffffu) : __uint_as_float(high << 16);
+                const float hy = T == DT_F16 ? f16_to_f32(high >> 16) : __uint_as_float(high & 0xffff0000u);
+                p[1][i] = least2<T>(pack2<T>(x - hx, y - hy));
             }
 #pragma unroll
             for (int c = 0; c < NV; c++)

@@ -2,10 +2,11 @@
 import pytest
 import torch
 
-from serving_util import BF16, F16, F32, ROUND, TORCH
-from test_gpu_paged_attention import attend
+from serving_util import BF16, F16, F32, ROUND, TORCH, attention_reference, check_attention
+from test_gpu_paged_attention import attend, problem
 
 pytestmark = pytest.mark.gpu
+INF = float("inf")
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
@@ -35,3 +36,46 @@ def test_very_many_small_weights(ctx, dtype, far):
         bound = bound + 1.25 * N * 2.0 ** -36 / p.sum() + 2.0 ** -25
     assert ((got.double() - want).abs() <= bound).all(), float(((got.double() - want).abs() / bound).max())
     assert ((lse.double() - (far + torch.log(p.sum()))).abs() <= (3 * far + 64 + N / 16) * 2.0 ** -24).all()
+
+
+def check_with_infinities(got, lse, ref, v_max, dtype, what):
+    """Infinities and NaN where the definition has them; the rest as in the other tests."""
+    out, want_lse, tol = ref
+    got = got.double().view(out.shape)
+    assert torch.equal(torch.isnan(got), torch.isnan(out)), what
+    odd = ~torch.isfinite(out)
+    assert torch.equal(torch.isinf(got), torch.isinf(out)) and torch.equal(got[torch.isinf(out)], out[torch.isinf(out)]), what
+    check_attention(torch.where(odd, 0.0, got).to(TORCH[dtype]), lse, (torch.where(odd, 0.0, out), want_lse, tol), v_max, dtype, what)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lens", [[1, 1, 2, 40], [3000, 1, 500, 33]])
+def test_infinite_values(ctx, dtype, lens):
+    """The weight of a counted token is above 0, so an infinite value is the channel's result, and two opposite ones NaN."""
+    H, Hk, D, page = 8, 2, 64, 16
+    q, kc, vc, table, n = problem(600 + dtype, dtype, lens, H, Hk, D, page, poison=False)
+    at = lambda r, t: (int(table[r, t // page]), slice(None), t % page)  # noqa: E731
+    v_max = float(vc.double().abs().max())
+    vc[at(0, 0)][:, 3], vc[at(1, 0)][:, 5] = INF, -INF
+    vc[at(2, 1)][:, 0], vc[at(3, 17)][:, 9], vc[at(3, 20)][:, 9], vc[at(3, 30)][0, 10] = INF, INF, -INF, -INF
+    got, lse = attend(ctx, q, kc, vc, table, n, H, dtype)
+    ref = attention_reference(q, kc, vc, table, n, H, scale=D ** -0.5)
+    assert torch.isinf(ref[0]).sum() == 8 + 8 + 8 + 4 and torch.isnan(ref[0]).sum() == 8
+    check_with_infinities(got, lse, ref, v_max, dtype, "infinite values")
+
+
+@pytest.mark.parametrize("dtype,far", [(F32, 60), (F16, 12), (F16, 20), (F16, 60), (BF16, 20), (BF16, 60)])
+def test_infinite_values_of_small_weight(ctx, dtype, far):
+    """An infinite value whose weight is exp(-far) of the largest."""
+    D, page = 64, 16
+    q, kc, vc, table, n = problem(630, dtype, [100], 1, 1, D, page, poison=False)
+    q[0] = 0
+    q[0, 0] = 8
+    kc[..., 0] = 0
+    kc[int(table[0, 2]), 0, 5, 0] = far  # its score: far; all others 0
+    v_max = float(vc.double().abs().max())
+    vc[int(table[0, 0]), 0, 1, 7] = -INF
+    got, lse = attend(ctx, q, kc, vc, table, n, 1, dtype)
+    ref = attention_reference(q, kc, vc, table, n, 1, scale=D ** -0.5)
+    assert torch.isinf(ref[0]).sum() == 1
+    check_with_infinities(got, lse, ref, v_max, dtype, "small weight")
