@@ -134,13 +134,11 @@ __device__ __forceinline__ float wave_max(float v) {
     return fmaxf(fmaxf(lane_f(v, 0), lane_f(v, 16)), fmaxf(lane_f(v, 32), lane_f(v, 48)));
 }
 
-// tanh(y) from z = 2 y log2 e: 1 - 2 / (1 + exp2(z)), off by 2^-22 at most.  In f32
-// scores that is more than the rest of the kernel is off where y is small:
-// there the series up to y^11, whose next term is below 2^-28 of y at 0.3.
-template <int T>
+// tanh(y) from z = 2 y log2 e: 1 - 2 / (1 + exp2(z)), off by 2^-22 at most.  Where y
+// is small that is a large share of it, and times a large cap a large part of the
+// score: there the series up to y^11, whose next term is below 2^-28 of y at 0.3.
 __device__ __forceinline__ float tanh_of(float z) {
     const float far = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z)), -2.f, 1.f);
-    if constexpr (T != DT_F32) return far;
     const float y = z * (0.5f * kLn2), q = y * y;
     float near = fmaf(q, -1382.f / 155925.f, 62.f / 2835.f);
     near = fmaf(q, near, -17.f / 315.f);
@@ -319,7 +317,7 @@ struct Attn {
 #pragma unroll
             for (int i = 0; i < SUB; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[i][j] = a.softcap * tanh_of<T>(s[i][j] * a.scale);
+                for (int j = 0; j < 4; j++) s[i][j] = a.softcap * tanh_of(s[i][j] * a.scale);
         } else {
 #pragma unroll
             for (int i = 0; i < SUB; i++) s[i] *= a.scale;

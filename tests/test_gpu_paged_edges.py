@@ -79,3 +79,17 @@ def test_infinite_values_of_small_weight(ctx, dtype, far):
     ref = attention_reference(q, kc, vc, table, n, 1, scale=D ** -0.5)
     assert torch.isinf(ref[0]).sum() == 1
     check_with_infinities(got, lse, ref, v_max, dtype, "small weight")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [2.0 ** -60, 0.01, 1.0, 50.0, 1e3, 1e5, 1e6, 1e9, 2.0 ** 90])
+def test_caps_of_any_size(ctx, dtype, cap):
+    """A score far below its cap is itself, whatever the cap: nothing may be off by a share of the cap."""
+    D, H = 64, 8
+    q, kc, vc, table, n = problem(660 + dtype, dtype, [1, 60, 333, 1500], H, 2, D, 16, poison=False)
+    got, lse = attend(ctx, q, kc, vc, table, n, H, dtype, softcap=cap)
+    out, want_lse, _ = attention_reference(q, kc, vc, table, n, H, scale=D ** -0.5, softcap=cap)
+    tol = attention_reference(q, kc, vc, table, n, H, scale=D ** -0.5)[2]
+    # the cap's own steps: at most 16 roundings of the capped score, none of which is above 8 here or above the cap
+    tol = tol + 2 * 16 * 2.0 ** -24 * min(cap, 8.0)
+    check_attention(got, lse, (out, want_lse, tol), float(vc.double().abs().max()), dtype, f"cap {cap}")
