@@ -101,7 +101,8 @@ typedef struct lux_paged_append_args {
  * of [max(0, n - window), n), n = kv_lens[r] cut to [0, max_pages *
  * page_size] (window 0: all of [0, n)), but those whose page is none:
  *   s_t = scale * q . k_t, or softcap * tanh(scale * q . k_t / softcap) where
- *   softcap > 0;  out = sum_t exp(s_t) v_t / sum_t exp(s_t);
+ *   softcap > 0 (2^-100 to 2^100; others but 0 are INVALID_ARGUMENT);
+ *   out = sum_t exp(s_t) v_t / sum_t exp(s_t);
  *   lse = log(sum_t exp(s_t))
  * A request with no position gives out = 0 and lse = -infinity.  Cache places
  * that no position of a request names are never part of its result, whatever

@@ -126,11 +126,14 @@ LuxBackendError op_paged_append(LuxBackendContext* c, const lux_paged_append_arg
     return map_status(lxq::launch_paged_append(a, ctx->stream));
 }
 
+// none, or a cap whose quotients and products with a score's factors stay in fp32
+bool cap_ok(float c) { return c == 0.f || (c >= 0x1p-100f && c <= 0x1p100f); }
+
 LuxBackendError op_paged_attention(LuxBackendContext* c, const lux_paged_attention_args* p) {
     HipContext* ctx = C(c);
     if (!ctx || !p || p->struct_size != sizeof(*p)) return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     if (p->requests < 0 || p->heads <= 0 || !cache_ok(p->kv_heads, p->head_dim, p->page_size, p->num_pages) ||
-        p->heads % p->kv_heads || p->max_pages <= 0 || p->window < 0 || !(p->softcap >= 0.f))
+        p->heads % p->kv_heads || p->max_pages <= 0 || p->window < 0 || !cap_ok(p->softcap))
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     const int64_t row = (int64_t)p->heads * p->head_dim;
     if (!stride_ok(p->q_row_stride, row) || !stride_ok(p->out_row_stride, row) || !offset_ok(p->q_offset) ||

@@ -2,8 +2,9 @@
 import pytest
 import torch
 
-from serving_util import BF16, F16, F32, ROUND, TORCH, attention_reference, check_attention
-from test_gpu_paged_attention import attend, problem
+from mlx_amd import abi
+from serving_util import BF16, F16, F32, ROUND, TORCH, Device, attention_reference, check_attention
+from test_gpu_paged_attention import _record, attend, problem
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -93,3 +94,13 @@ def test_caps_of_any_size(ctx, dtype, cap):
     # the cap's own steps: at most 16 roundings of the capped score, none of which is above 8 here or above the cap
     tol = tol + 2 * 16 * 2.0 ** -24 * min(cap, 8.0)
     check_attention(got, lse, (out, want_lse, tol), float(vc.double().abs().max()), dtype, f"cap {cap}")
+
+
+def test_caps_that_are_refused(ctx):
+    """Infinite ones, whose scores would be infinity times 0, and those that scores divided or multiplied by leave f32."""
+    with Device(ctx) as dev:
+        call = lambda cap: ctx.s.op_paged_attention(ctx.handle, _record(dev, softcap=cap))  # noqa: E731
+        for cap in (INF, -INF, 3e38, 2.0 ** 101, 2.0 ** -101, 1e-40, -1e-40):
+            assert call(cap) == abi.ERR_INVALID_ARGUMENT, cap
+        for cap in (0.0, -0.0, 2.0 ** 100, 2.0 ** -100):
+            assert call(cap) == abi.OK, cap
