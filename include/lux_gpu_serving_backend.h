@@ -104,7 +104,8 @@ typedef struct lux_paged_append_args {
  *   softcap > 0 (2^-100 to 2^100; others but 0 are INVALID_ARGUMENT);
  *   out = sum_t exp(s_t) v_t / sum_t exp(s_t);
  *   lse = log(sum_t exp(s_t))
- * A request with no position gives out = 0 and lse = -infinity.  Cache places
+ * A request with no position gives out = 0 and lse = -infinity.  A score
+ * that leaves fp32 when multiplied by log2 e is infinite (2.36e38).  Cache places
  * that no position of a request names are never part of its result, whatever
  * they hold.  Scores, sums and the running statistics are fp32; with 16-bit
  * types exp(s - max) enters the product with v as the sum of two values of

@@ -42,7 +42,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kDevice = 16;  // cache policy of the partial results: device scope (sc1)
-constexpr float kLowest = -3.0e38f;  // the maximum of no score
+constexpr float kLowest = -0x1.fffffep127f;  // the maximum of no score: no finite score is below
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 
 struct Params {

@@ -104,3 +104,21 @@ def test_caps_that_are_refused(ctx):
             assert call(cap) == abi.ERR_INVALID_ARGUMENT, cap
         for cap in (0.0, -0.0, 2.0 ** 100, 2.0 ** -100):
             assert call(cap) == abi.OK, cap
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scores_near_the_lowest(ctx, dtype):
+    """Scores of -2.2e38, all there are: weights of 1, not none."""
+    D, page = 64, 16
+    q, kc, vc, table, n = problem(690 + dtype, dtype, [50, 20], 2, 2, D, page, poison=False)
+    q[:], kc[:] = 0, 0
+    q[:, 0::D], kc[..., 0] = -2.0 ** 60, 2.0 ** 64
+    scale = 2.2e38 / 2.0 ** 124
+    got, lse = attend(ctx, q, kc, vc, table, n, 2, dtype, scale=scale)
+    got = got.double().view(2, 2, D)
+    for r in range(2):
+        for h in range(2):
+            t = torch.arange(int(n[r]))
+            want = vc[table[r, t // page].long(), h, t % page].double().mean(0)
+            assert ((got[r, h] - want).abs() <= 2 * ROUND[dtype] * want.abs() + 2.0 ** -14).all()
+            assert abs(float(lse[r, h]) + 2.2e38) < 1e32
