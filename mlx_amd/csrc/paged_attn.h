@@ -82,9 +82,13 @@ __device__ __forceinline__ Extent extent_of(const AttnArgs& a, int n) {
 // values that all lanes share, kept in scalar registers
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ Extent extent_at(const AttnArgs& a, int r) { return extent_of(a, uniform(a.lens[r])); }
+// runs of `tokens` tokens (without a sign: a request may end just below 2^31)
+__device__ __forceinline__ int runs_of(const Extent& e, int tokens) {
+    return (int)(((uint32_t)(e.end - e.base) + (uint32_t)tokens - 1) / (uint32_t)tokens);
+}
 // units of `tokens` tokens; a request with none has one, which writes its zeros
 __device__ __forceinline__ int units_of(const Extent& e, int tokens) {
-    const int n = (int)((uint32_t)(e.end - e.base + tokens - 1) / (uint32_t)tokens);
+    const int n = runs_of(e, tokens);
     return n < 1 ? 1 : n;
 }
 
@@ -217,19 +221,19 @@ struct Attn {
 
     static constexpr uint32_t kAll = SUB == 2 ? 0xffffffffu : 0xffffu;
 
-    // pages of the tile at token t0
-    __device__ __forceinline__ void look(const AttnArgs& a, const Extent& e, int r, int t0) {
+    // pages of the tile at token t0, which may be past the request's end and past 2^31
+    __device__ __forceinline__ void look(const AttnArgs& a, const Extent& e, int r, uint32_t t0) {
         if constexpr (WHOLE) {
             // (address space 4: scalar loads)
             const auto* table = (const __attribute__((address_space(4))) int32_t*)a.table + (int64_t)r * a.columns;
 #pragma unroll
             for (int s = 0; s < SUB; s++) {
-                const int t = t0 + 16 * s;
-                page[s] = t < e.end && t + 16 > e.start ? table[div_by(t, a.div)] : -1;
+                const uint32_t t = t0 + 16 * s;
+                page[s] = t < (uint32_t)e.end && t + 16 > (uint32_t)e.start ? table[div_by((int)t, a.div)] : -1;
             }
         } else {
-            const int t = t0 + (int)(threadIdx.x & (kTile - 1));
-            page[0] = t >= e.start && t < e.end ? a.table[(int64_t)r * a.columns + div_by(t, a.div)] : -1;
+            const uint32_t t = t0 + (threadIdx.x & (kTile - 1));
+            page[0] = t >= (uint32_t)e.start && t < (uint32_t)e.end ? a.table[(int64_t)r * a.columns + div_by((int)t, a.div)] : -1;
         }
     }
     // the rows they stand for; masked ones read row 0
@@ -430,7 +434,7 @@ struct Attn {
             load_q(a, c.r, c.h, c.qt);
             resolve(a, c.ex, c.h, t);
             load_k(a);
-            look(a, c.ex, c.r, t + kUnit);
+            look(a, c.ex, c.r, (uint32_t)t + kUnit);
             load_v(a);
         }
         f4 s[SUB];
@@ -440,7 +444,7 @@ struct Attn {
             t += kUnit;
             resolve(a, c.ex, c.h, t);
             load_k(a);
-            look(a, c.ex, c.r, t + kUnit);
+            look(a, c.ex, c.r, (uint32_t)t + kUnit);
             take(a, s, now);
             load_v(a);
         }
@@ -455,7 +459,7 @@ struct Attn {
             load_q(a, next.r, next.h, next.qt);
             resolve(a, next.ex, next.h, t);
             load_k(a);
-            look(a, next.ex, next.r, t + kUnit);
+            look(a, next.ex, next.r, (uint32_t)t + kUnit);
         }
         take(a, s, now);
         if (primed) load_v(a);
@@ -658,7 +662,7 @@ __global__ __launch_bounds__(64 * NW, (kWaves<DP>)) void attn_pair_kernel(Params
     const int r = blockIdx.x / p.HQ, hq = blockIdx.x - r * p.HQ, h = hq / p.QT, qt = hq - h * p.QT;
     const Extent ex = extent_at(p.a, r);
     bool primed = false;
-    x.run(p.a, Piece{r, h, qt, w, (ex.end - ex.base + A::kTile - 1) / A::kTile, ex}, Piece{}, primed);
+    x.run(p.a, Piece{r, h, qt, w, runs_of(ex, A::kTile), ex}, Piece{}, primed);
     x.join(p, r, h, qt, -1, attn_lds);
 }
 
@@ -754,7 +758,7 @@ __global__ __launch_bounds__(64 * NW, (kWaves<DP>)) void attn_range_kernel(Param
     A x;
     // the piece of pair (r, hq) from unit u on, as far as the range goes
     auto piece = [&] {
-        const int h = p.QT == 1 ? hq : hq / p.QT, tiles = (ex.end - ex.base + A::kTile - 1) / A::kTile;
+        const int h = p.QT == 1 ? hq : hq / p.QT, tiles = runs_of(ex, A::kTile);
         const int last = (u + (end - pos) < n ? u + (end - pos) : n) * NW;
         return Piece{r, h, hq - h * p.QT, u * NW + w, last < tiles ? last : tiles, ex};
     };

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from mlx_amd import abi
-from serving_util import BF16, F16, F32, ROUND, TORCH, Device, attention_reference, check_attention
+from serving_util import BF16, F16, F32, ROUND, TORCH, Device, attention_reference, check_attention, randn
 from test_gpu_paged_attention import _record, attend, problem
 
 pytestmark = pytest.mark.gpu
@@ -122,3 +122,21 @@ def test_scores_near_the_lowest(ctx, dtype):
             want = vc[table[r, t // page].long(), h, t % page].double().mean(0)
             assert ((got[r, h] - want).abs() <= 2 * ROUND[dtype] * want.abs() + 2.0 ** -14).all()
             assert abs(float(lse[r, h]) + 2.2e38) < 1e32
+
+
+@pytest.mark.parametrize("page,columns", [(42966, 49981), (8176, 262657)])
+def test_length_just_below_31_bits(ctx, page, columns):
+    """A request that ends within a tile of 2^31: one page, named by every entry of its row, so that its places count alike.
+
+    Each lane adds up to 2^31 / 2048 / 4 terms (2048 waves, 8 of 32 tokens a lane), 2^18 roundings of 2^-24 of the sum."""
+    N, D = page * columns, 8
+    assert 2 ** 31 - 32 < N < 2 ** 31
+    gen = torch.Generator().manual_seed(1)
+    kc, vc = (0.5 * randn(gen, F16, 1, 1, page, D) for _ in range(2))
+    vc = vc.abs() + 1
+    q = randn(gen, F16, 1, D)
+    got, lse = attend(ctx, q, kc, vc, torch.zeros(1, columns, dtype=torch.int32), torch.tensor([N], dtype=torch.int32), 1, F16)
+    s = kc[0, 0].double() @ q[0].double() / D ** 0.5
+    want = torch.softmax(s, 0) @ vc[0, 0].double()
+    assert ((got[0].double() - want).abs() <= (2.0 ** -5 + ROUND[F16]) * want).all()
+    assert abs(float(lse) - float(torch.logsumexp(s, 0) + torch.log(torch.tensor(float(columns), dtype=torch.float64)))) <= 2.0 ** -5
