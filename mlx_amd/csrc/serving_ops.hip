@@ -2,21 +2,13 @@
 // (include/lux_gpu_serving_backend.h): argument checks, then one launcher.
 #include <new>
 
+#include "extent.h"
 #include "hip_context.h"
 #include "serving.h"
 
 using namespace lxh;
 
 namespace {
-
-// strides and offsets up to 2^40 elements keep every extent in 64 bits
-bool stride_ok(int64_t s, int64_t row) { return s == 0 || (s >= row && s <= (1ll << 40)); }
-bool offset_ok(int64_t o) { return o >= 0 && o <= (1ll << 40); }
-
-// bytes from an array's start to the end of the last of `rows` rows
-size_t extent(int64_t rows, int64_t stride, int64_t row, size_t esz) {
-    return rows <= 0 || row <= 0 ? 0 : (size_t)((rows - 1) * stride + row) * esz;
-}
 
 // the memory one argument covers
 struct Span {
@@ -34,7 +26,7 @@ struct Spans {
     bool ok = true;
     const void* add(LuxBackendBuffer* b, size_t skip, size_t bytes, size_t esz, bool out) {
         HipBuffer* h = B(b);
-        if (!fits(h, skip + bytes) || (bytes && reinterpret_cast<uintptr_t>(h->ptr) % esz)) {
+        if (!h || !holds(h->size, skip, bytes) || (bytes && reinterpret_cast<uintptr_t>(h->ptr) % esz)) {
             ok = false;
             return nullptr;
         }
