@@ -190,8 +190,12 @@ typedef struct lux_gpu_serving_vtbl {
      * part of another allocation, another library's tensor) and keeps until
      * buffer_free, which leaves the memory alone.  NULL where device_ptr is
      * no memory of the context's device.  Work of other streams on that memory
-     * is the caller's to order.  The serving ops read nothing past `bytes`;
-     * the quantized ops may read 256 bytes more. */
+     * is the caller's to order.  The serving ops read nothing past `bytes`.
+     * The quantized ops, which take operands in vectors, refuse a wrapped one
+     * (INVALID_ARGUMENT) that does not start on 16 bytes, and an input without 256
+     * readable bytes behind what they need of it: in the buffer or in the
+     * rest of the allocation that it lies in.  The base table's ops ask for 4
+     * bytes (matmul: and 12 readable ones behind its inputs). */
     LuxBackendBuffer* (*buffer_wrap)(LuxBackendContext* ctx, void* device_ptr, size_t bytes);
 
     void* _reserved[5];

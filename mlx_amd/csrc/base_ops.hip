@@ -13,6 +13,8 @@ namespace {
 
 enum : int { EW_ADD = 0, EW_SUB = 1, EW_MUL = 2, EW_DIV = 3 };
 
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // buffers and rows may be dword-aligned only
+
 // 4 elements per thread (a 16-byte load of each operand), grid-stride
 template <int OP>
 __global__ __launch_bounds__(256) void ew_kernel(const float* __restrict__ a, const float* __restrict__ b,
@@ -21,13 +23,16 @@ __global__ __launch_bounds__(256) void ew_kernel(const float* __restrict__ a, co
     const size_t n4 = n / 4;
     const size_t stride = (size_t)gridDim.x * blockDim.x;
     for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += stride) {
-        const float4 x = reinterpret_cast<const float4*>(a)[i], y = reinterpret_cast<const float4*>(b)[i];
-        float4 r;
-        if constexpr (OP == EW_ADD) r = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
-        else if constexpr (OP == EW_SUB) r = make_float4(x.x - y.x, x.y - y.y, x.z - y.z, x.w - y.w);
-        else if constexpr (OP == EW_MUL) r = make_float4(x.x * y.x, x.y * y.y, x.z * y.z, x.w * y.w);
-        else r = make_float4(x.x / y.x, x.y / y.y, x.z / y.z, x.w / y.w);
-        reinterpret_cast<float4*>(o)[i] = r;
+        const f4u x = reinterpret_cast<const f4u*>(a)[i], y = reinterpret_cast<const f4u*>(b)[i];
+        f4u r;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if constexpr (OP == EW_ADD) r[e] = x[e] + y[e];
+            else if constexpr (OP == EW_SUB) r[e] = x[e] - y[e];
+            else if constexpr (OP == EW_MUL) r[e] = x[e] * y[e];
+            else r[e] = x[e] / y[e];
+        }
+        reinterpret_cast<f4u*>(o)[i] = r;
     }
     // tail (n % 4 elements) by the first threads
     const size_t t = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -69,7 +74,6 @@ struct MmTile {
     static_assert(2 * 4 * (kA + kB) <= 64 * 1024, "static LDS");
 };
 
-typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // rows of A and B are dword-aligned only
 typedef float f4a __attribute__((ext_vector_type(4)));
 
 template <class T>

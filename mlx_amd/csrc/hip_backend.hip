@@ -332,11 +332,11 @@ LuxBackendError qmm_impl(LuxBackendContext* c, LuxBackendBuffer* x, LuxBackendBu
     if (e != LUX_BACKEND_OK) return e;
     if (bias && !dtype_ok(bias_dtype)) return LUX_BACKEND_ERROR_NOT_SUPPORTED;
     const size_t G = (size_t)(K / group_size);
-    if (!fits(B(x), (size_t)M * K * dtype_size(x_dtype)) ||
-        !fits(B(w_q), (size_t)N * K * bits / 8) || !fits(B(scales), (size_t)N * G * dtype_size(sb_dtype)) ||
-        !fits(B(biases), (size_t)N * G * dtype_size(sb_dtype)) ||
-        !fits(B(out), (size_t)M * N * dtype_size(out_dtype)) ||
-        (bias && !fits(B(bias), (size_t)N * dtype_size(bias_dtype))))
+    if (!read_by(B(x), (size_t)M * K * dtype_size(x_dtype)) || !read_by(B(w_q), (size_t)N * K * bits / 8) ||
+        !read_by(B(scales), (size_t)N * G * dtype_size(sb_dtype)) ||
+        !read_by(B(biases), (size_t)N * G * dtype_size(sb_dtype)) ||
+        !written_by(B(out), (size_t)M * N * dtype_size(out_dtype)) ||
+        (bias && !read_by(B(bias), (size_t)N * dtype_size(bias_dtype))))
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     if (M == 0 || N == 0) return LUX_BACKEND_OK;
 
@@ -401,9 +401,9 @@ LuxBackendError hip_op_dequantize(LuxBackendContext* c, LuxBackendBuffer* w_q,
     if (e != LUX_BACKEND_OK) return e;
     if (!dtype_ok(sb_dtype) || !dtype_ok(out_dtype)) return LUX_BACKEND_ERROR_NOT_SUPPORTED;
     const size_t G = (size_t)(K / group_size);
-    if (!fits(B(w_q), (size_t)N * K * bits / 8) || !fits(B(scales), (size_t)N * G * dtype_size(sb_dtype)) ||
-        !fits(B(biases), (size_t)N * G * dtype_size(sb_dtype)) ||
-        !fits(B(out), (size_t)N * K * dtype_size(out_dtype)))
+    if (!read_by(B(w_q), (size_t)N * K * bits / 8) || !read_by(B(scales), (size_t)N * G * dtype_size(sb_dtype)) ||
+        !read_by(B(biases), (size_t)N * G * dtype_size(sb_dtype)) ||
+        !written_by(B(out), (size_t)N * K * dtype_size(out_dtype)))
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     if (N == 0) return LUX_BACKEND_OK;
     if (hipSetDevice(ctx->device) != hipSuccess) return LUX_BACKEND_ERROR_DEVICE_LOST;
@@ -422,9 +422,9 @@ LuxBackendError hip_op_quantize(LuxBackendContext* c, LuxBackendBuffer* w, LuxBa
     if (e != LUX_BACKEND_OK) return e;
     if (!dtype_ok(w_dtype) || !dtype_ok(sb_dtype)) return LUX_BACKEND_ERROR_NOT_SUPPORTED;
     const size_t G = (size_t)(K / group_size);
-    if (!fits(B(w), (size_t)N * K * dtype_size(w_dtype)) || !fits(B(w_q), (size_t)N * K * bits / 8) ||
-        !fits(B(scales), (size_t)N * G * dtype_size(sb_dtype)) ||
-        !fits(B(biases), (size_t)N * G * dtype_size(sb_dtype)))
+    if (!read_by(B(w), (size_t)N * K * dtype_size(w_dtype)) || !written_by(B(w_q), (size_t)N * K * bits / 8) ||
+        !written_by(B(scales), (size_t)N * G * dtype_size(sb_dtype)) ||
+        !written_by(B(biases), (size_t)N * G * dtype_size(sb_dtype)))
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     if (N == 0) return LUX_BACKEND_OK;
     if (hipSetDevice(ctx->device) != hipSuccess) return LUX_BACKEND_ERROR_DEVICE_LOST;
@@ -440,7 +440,10 @@ LuxBackendError hip_op_quantize(LuxBackendContext* c, LuxBackendBuffer* w, LuxBa
 // kernel must not read or write past an allocation.
 // ---------------------------------------------------------------------------
 
-bool fits(LuxBackendBuffer* b, size_t floats) { return B(b) && floats <= B(b)->size / 4; }
+// (the matmul may read 12 bytes past A and B)
+bool fits(LuxBackendBuffer* b, size_t floats, size_t past = 0) {
+    return B(b) && floats <= B(b)->size / 4 && reaches(B(b), floats * 4, 4, past);
+}
 
 LuxBackendError elementwise(int op, LuxBackendContext* c, LuxBackendBuffer* a, LuxBackendBuffer* b,
                             LuxBackendBuffer* out, size_t n) {
@@ -472,7 +475,7 @@ LuxBackendError hip_op_matmul_f32(LuxBackendContext* c, LuxBackendBuffer* a, Lux
                                   LuxBackendBuffer* out, int M, int K, int N) {
     HipContext* ctx = C(c);
     if (!ctx || M < 0 || K < 0 || N < 0) return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
-    if (!fits(a, (size_t)M * K) || !fits(b, (size_t)K * N) || !fits(out, (size_t)M * N))
+    if (!fits(a, (size_t)M * K, 12) || !fits(b, (size_t)K * N, 12) || !fits(out, (size_t)M * N))
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     if (hipSetDevice(ctx->device) != hipSuccess) return LUX_BACKEND_ERROR_DEVICE_LOST;
     return map_status(lxq::launch_matmul_f32(static_cast<const float*>(B(a)->ptr), static_cast<const float*>(B(b)->ptr),

@@ -34,6 +34,7 @@ struct HipBuffer {
     void* ptr = nullptr;
     size_t size = 0;
     bool owned = true;  // false: a view of memory that the caller frees
+    size_t tail = lxq::kTailPad;  // readable bytes behind it (a view's: to its allocation's end)
 };
 
 inline HipContext* C(LuxBackendContext* c) { return reinterpret_cast<HipContext*>(c); }
@@ -66,6 +67,17 @@ inline bool dtype_ok(int dt) {
 }
 
 inline bool fits(HipBuffer* b, size_t need) { return b && (need == 0 || (b->ptr && b->size >= need)); }
+// an operand whose kernels take its first `need` bytes in vectors of `align`
+// bytes and may read `past` bytes behind them: an allocation of the plugin's
+// is made for that, a view may start and end anywhere
+inline bool reaches(HipBuffer* b, size_t need, size_t align, size_t past) {
+    if (!fits(b, need)) return false;
+    return need == 0 || b->owned ||
+           (reinterpret_cast<uintptr_t>(b->ptr) % align == 0 && b->size - need + b->tail >= past);
+}
+// operands of the quantized ops
+inline bool read_by(HipBuffer* b, size_t need) { return reaches(b, need, 16, lxq::kTailPad); }
+inline bool written_by(HipBuffer* b, size_t need) { return reaches(b, need, 16, 0); }
 
 }  // namespace lxh
 

@@ -232,6 +232,18 @@ bool on_device(const HipContext* ctx, const void* p) {
     return at.type == hipMemoryTypeDevice && at.device == ctx->device;
 }
 
+// readable bytes behind a view of device memory: to the end of the allocation it lies in
+size_t behind(char* p, size_t bytes) {
+    hipDeviceptr_t base = nullptr;
+    size_t size = 0;
+    if (hipMemGetAddressRange(&base, &size, p) != hipSuccess) {
+        (void)hipGetLastError();
+        return 0;
+    }
+    const char *end = static_cast<char*>(base) + size, *mine = p + bytes;
+    return end > mine ? (size_t)(end - mine) : 0;
+}
+
 LuxBackendBuffer* buffer_wrap(LuxBackendContext* c, void* ptr, size_t bytes) {
     HipContext* ctx = C(c);
     if (!ctx || (bytes && !ptr) || hipSetDevice(ctx->device) != hipSuccess) return nullptr;
@@ -241,6 +253,7 @@ LuxBackendBuffer* buffer_wrap(LuxBackendContext* c, void* ptr, size_t bytes) {
     b->ptr = bytes ? ptr : nullptr;
     b->size = bytes;
     b->owned = false;
+    b->tail = bytes ? behind(static_cast<char*>(ptr), bytes) : 0;
     return reinterpret_cast<LuxBackendBuffer*>(b);
 }
 
