@@ -7,6 +7,11 @@ nothing read back between steps.
 
 The lengths, the free list's head and the block table stay on the device: a
 step's kv_lens are the next one's seq_lens, its counts the next one's head.
+
+Rows.  The plan numbers a step's new tokens, the attention its requests.  Here row
+r is both, so the requests that take a token in a step stand in front of those
+that pause (feed()); a program with any other order gathers the rows of k and v by
+token_request, or those of q by token_starts.
 """
 import os
 import sys
@@ -78,8 +83,16 @@ class Block:
                                       post_weight=h(self.norms[1]), pre_weight=h(self.norms[2]), residual_out=h(self.h), out=h(self.next))
         self.turn = 0
 
+    def feed(self, x, new=None):
+        """A step's inputs, a row per request, and which of them take a token: all, or 1s and then 0s."""
+        new = np.ones(self.R, np.int32) if new is None else np.asarray(new, np.int32)
+        if new.shape != (self.R,) or ((new != 0) & (new != 1)).any() or (np.diff(new) > 0).any():
+            raise ValueError(f"one token or none per request, those with one first: {new.tolist()}")
+        self.x.upload(x.view(np.uint16))
+        self.new.upload(new)
+
     def step(self):
-        """One token for each request whose `new` is 1; the others' rows are computed and thrown away."""
+        """One token for each request that feed() gave one; the others' rows are computed and thrown away."""
         c, i = self.ctx, self.turn
         c.block_norm(self.first)
         self.qkv(self.normed, self.fused, self.R)
@@ -90,15 +103,16 @@ class Block:
         c.block_norm(self.last)
         self.turn = 1 - i
 
-    def reference(self, x, past):
-        """The same step in 64 bits; `past`: each request's keys and values so far, extended in place."""
+    def reference(self, x, past, new):
+        """The same step in 64 bits, rows that take no token 0; `past`: each request's keys and values so far, extended in place."""
         def rms(v, w):
             return v / np.sqrt((v * v).mean(-1, keepdims=True) + 1e-5) * w.astype(np.float64)
 
         x = x.astype(np.float64)
         fused = rms(x, self.norm_w[0]) @ self.qkv.weights.astype(np.float64).T
         att = np.zeros((self.R, self.q_len))
-        for r in range(self.R):
+        on = np.asarray(new, bool)
+        for r in np.flatnonzero(on):
             k, v = (fused[r, at:at + self.kv_len].reshape(self.Hk, 1, self.D) for at in (self.q_len, self.q_len + self.kv_len))
             past[r] = (k, v) if past[r] is None else tuple(np.concatenate([o, n], 1) for o, n in zip(past[r], (k, v)))
             q = fused[r, :self.q_len].reshape(self.Hk, -1, self.D)
@@ -106,7 +120,7 @@ class Block:
             p = np.exp(s - s.max(-1, keepdims=True))
             att[r] = ((p / p.sum(-1, keepdims=True)) @ past[r][1]).reshape(-1)
         h = x + rms(att @ self.proj.weights.astype(np.float64).T, self.norm_w[1])
-        return h, rms(h, self.norm_w[2])
+        return h * on[:, None], rms(h, self.norm_w[2]) * on[:, None]
 
     def free_all(self):
         for b in [*self.qkv.bufs, *self.proj.bufs, *self.norms, *self.lens, *self.counts, self.x, self.normed, self.fused, self.att, self.out,
@@ -114,22 +128,24 @@ class Block:
             b.free()
 
 
-def run(ctx, steps=20, requests=3, dim=512, heads=8, kv_heads=2, head_dim=64, page=4, seed=7):
-    """Decodes `steps` tokens for each request; returns the worst error of a step, relative to its largest value."""
+def run(ctx, steps=20, requests=3, dim=512, heads=8, kv_heads=2, head_dim=64, page=4, seed=7, running=None):
+    """Decodes `steps` tokens for each request; returns the worst error of a step, relative to its largest value.
+    running: at which steps only that many requests take a token ({step: n})."""
     pages = requests * -(-steps // page) + 2
     block = Block(ctx, dim, heads, kv_heads, head_dim, requests, pages, page, -(-steps // page), seed)
-    block.new.upload(np.ones(requests, np.int32))
-    rng, past, worst = np.random.default_rng(seed), [None] * requests, 0.0
+    rng, past, worst, lens = np.random.default_rng(seed), [None] * requests, 0.0, np.zeros(requests, np.int32)
     try:
-        for _ in range(steps):
+        for i in range(steps):
             x = rng.standard_normal((requests, dim)).astype(np.float16)
-            block.x.upload(x.view(np.uint16))
+            new = (np.arange(requests) < (running or {}).get(i, requests)).astype(np.int32)
+            block.feed(x, new)
             block.step()
-            for buf, want in zip((block.h, block.next), block.reference(x, past)):
-                got = buf.download(np.uint16, want.shape).view(np.float16).astype(np.float64)
-                worst = max(worst, float(np.abs(got - want).max() / np.abs(want).max()))
-        lens = block.lens[block.turn].download(np.int32, (requests,))
-        assert (lens == steps).all(), lens
+            lens += new
+            for buf, want in zip((block.h, block.next), block.reference(x, past, new)):
+                got = buf.download(np.uint16, want.shape).view(np.float16).astype(np.float64) * new[:, None]
+                worst = max(worst, float(np.abs(got - want).max() / max(np.abs(want).max(), 1e-30)))
+        got = block.lens[block.turn].download(np.int32, (requests,))
+        assert (got == lens).all(), (got, lens)
         return worst
     finally:
         block.free_all()

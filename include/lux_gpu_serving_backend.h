@@ -96,7 +96,9 @@ typedef struct lux_paged_append_args {
 } lux_paged_append_args;
 
 /*
- * Attention of one token per request over its cached tokens.  Head i reads
+ * Attention of one token per request over its cached tokens: row r of q is
+ * request r's.  (A plan numbers tokens; where some requests of a step get
+ * none, the token of request r is row token_starts[r] of its arrays.)  Head i reads
  * the keys and values of head i / (heads / kv_heads).  Over the positions t
  * of [max(0, n - window), n), n = kv_lens[r] cut to [0, max_pages *
  * page_size] (window 0: all of [0, n)), but those whose page is none:
