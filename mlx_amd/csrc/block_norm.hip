@@ -149,10 +149,10 @@ __device__ __forceinline__ void normalize(float (*v)[8], const int* n, int kind,
 
 // a block per row
 template <int NT, int V, bool AWAY, int XT, int RT>
-__global__ __launch_bounds__(NT) void block_norm_kernel(NormArgs a) {
+__global__ __launch_bounds__(NT) void block_norm_kernel(NormArgs a, int first) {
     __shared__ float part[16];
     constexpr int hop = NT * 8;
-    const int t = blockIdx.x, col = (int)threadIdx.x * 8;
+    const int t = first + (int)blockIdx.x, col = (int)threadIdx.x * 8;
     const float inv_d = 1.f / (float)a.D;
     const bool gates = a.gate_mode == GATE_CHANNEL || a.gate_mode == GATE_FULL;
     const int64_t g_at = a.gate_mode == GATE_FULL ? t * a.g_row : 0;
@@ -201,10 +201,10 @@ __global__ __launch_bounds__(NT) void block_norm_kernel(NormArgs a) {
 // Rows too long for the registers (past 32768): x and the residual are read again
 // for each sum, out of the caches; h and out are written by the last pass.
 template <int XT, int RT>
-__global__ __launch_bounds__(1024) void block_norm_long_kernel(NormArgs a) {
+__global__ __launch_bounds__(1024) void block_norm_long_kernel(NormArgs a, int first) {
     constexpr int NT = 1024;
     __shared__ float part[16];
-    const int t = blockIdx.x;
+    const int t = first + (int)blockIdx.x;
     const float inv_d = 1.f / (float)a.D;
     const float row_gate = a.gate_mode == GATE_ROW ? load_f(a.gate, t * a.g_row, XT) : 1.f;
     float mean1 = 0.f, scale1 = 1.f;
@@ -286,8 +286,10 @@ __global__ __launch_bounds__(1024) void block_norm_long_kernel(NormArgs a) {
 // NT threads and V vectors of 8 per thread; NT = 0: the long form
 template <int NT, int V, bool AWAY, int XT, int RT>
 void launch_xr(const NormArgs& a, hipStream_t st) {
-    if constexpr (NT == 0) hipLaunchKernelGGL((block_norm_long_kernel<XT, RT>), dim3(a.T), dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL((block_norm_kernel<NT, V, AWAY, XT, RT>), dim3(a.T), dim3(NT), 0, st, a);
+    launch_blocks(a.T, NT ? NT : 1024, [&](int first, unsigned n) {
+        if constexpr (NT == 0) hipLaunchKernelGGL((block_norm_long_kernel<XT, RT>), dim3(n), dim3(1024), 0, st, a, first);
+        else hipLaunchKernelGGL((block_norm_kernel<NT, V, AWAY, XT, RT>), dim3(n), dim3(NT), 0, st, a, first);
+    });
 }
 template <int NT, int V, bool AWAY, int XT>
 void launch_x(const NormArgs& a, hipStream_t st) {

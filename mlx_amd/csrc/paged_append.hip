@@ -69,9 +69,9 @@ __device__ __forceinline__ int page_of(const AppendArgs& a, int slot) {
 // `per` tokens per block, `vecs` vectors of 8 per token: 256 / vecs tokens, or
 // one in several rounds
 template <int IN, int OUT, bool AWAY>
-__global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int vecs, int per, int vecs_of_head) {
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int first, int vecs, int per, int vecs_of_head) {
     const int mine = vecs < 256 ? (int)threadIdx.x / vecs : 0;
-    const int t = (int)blockIdx.x * per + mine;
+    const int64_t t = (int64_t)(first + (int)blockIdx.x) * per + mine;
     if (mine >= per || t >= a.T) return;
     const int slot = a.slots[t], page = page_of(a, slot);
     if (page < 0) return;
@@ -86,8 +86,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int vecs, int
 
 // head_dim no multiple of 8, or a cache that starts off 16 bytes: one element per thread
 template <int IN, int OUT>
-__global__ __launch_bounds__(256) void append_any_kernel(AppendArgs a) {
-    const int row = a.Hk * a.D, t = blockIdx.x;
+__global__ __launch_bounds__(256) void append_any_kernel(AppendArgs a, int first) {
+    const int row = a.Hk * a.D, t = first + (int)blockIdx.x;
     const int slot = a.slots[t], page = page_of(a, slot);
     if (page < 0) return;
     const int at = slot - page * a.page;
@@ -103,18 +103,21 @@ template <int IN, int OUT>
 void launch(const AppendArgs& a, hipStream_t st) {
     const int row = a.Hk * a.D;
     if (a.D % 8 || (reinterpret_cast<uintptr_t>(a.kc) | reinterpret_cast<uintptr_t>(a.vc)) % 16) {
-        hipLaunchKernelGGL((append_any_kernel<IN, OUT>), dim3(a.T), dim3(256), 0, st, a);
+        launch_blocks(a.T, 256, [&](int first, unsigned n) {
+            hipLaunchKernelGGL((append_any_kernel<IN, OUT>), dim3(n), dim3(256), 0, st, a, first);
+        });
         return;
     }
     const int vecs = row / 8, per = vecs < 256 ? 256 / vecs : 1;
-    const dim3 g((a.T + per - 1) / per), b(256);
     // 16-bit results that the L2s (32 MB) cannot hold leave past the caches (8192
     // tokens of 8 heads of 128, f32 to f16 16.0 us, 18.0 with plain stores); the
     // two stores of 8 f32 values are half lines, which costs more than it gains
     // (8192 tokens of 16 heads of 128 54.3 us plain, 66.8 so)
     const bool away = OUT != DT_F32 && (int64_t)a.T * row * 4 >= (32 << 20);
-    if (away) hipLaunchKernelGGL((append_kernel<IN, OUT, OUT != DT_F32>), g, b, 0, st, a, vecs, per, a.D / 8);
-    else hipLaunchKernelGGL((append_kernel<IN, OUT, false>), g, b, 0, st, a, vecs, per, a.D / 8);
+    launch_blocks(((int64_t)a.T + per - 1) / per, 256, [&](int first, unsigned n) {
+        if (away) hipLaunchKernelGGL((append_kernel<IN, OUT, OUT != DT_F32>), dim3(n), dim3(256), 0, st, a, first, vecs, per, a.D / 8);
+        else hipLaunchKernelGGL((append_kernel<IN, OUT, false>), dim3(n), dim3(256), 0, st, a, first, vecs, per, a.D / 8);
+    });
 }
 template <int IN>
 void launch_in(const AppendArgs& a, hipStream_t st) {

@@ -655,11 +655,11 @@ constexpr int kWaves = DP == 256 ? 1 : 2;
 
 // one block per pair
 template <int T, int DP, bool FULL, bool WHOLE, bool ONCE, int NW>
-__global__ __launch_bounds__(64 * NW, (kWaves<DP>)) void attn_pair_kernel(Params p) {
+__global__ __launch_bounds__(64 * NW, (kWaves<DP>)) void attn_pair_kernel(Params p, int first) {
     using A = Attn<T, DP, FULL, WHOLE, ONCE, NW>;
     A x;
     const int w = uniform(threadIdx.x >> 6);
-    const int r = blockIdx.x / p.HQ, hq = blockIdx.x - r * p.HQ, h = hq / p.QT, qt = hq - h * p.QT;
+    const int pair = first + (int)blockIdx.x, r = pair / p.HQ, hq = pair - r * p.HQ, h = hq / p.QT, qt = hq - h * p.QT;
     const Extent ex = extent_at(p.a, r);
     bool primed = false;
     x.run(p.a, Piece{r, h, qt, w, runs_of(ex, A::kTile), ex}, Piece{}, primed);
@@ -839,7 +839,9 @@ LuxStatus launch_d(Params& p, hipStream_t st) {
     const int64_t longest = ((int64_t)p.a.columns * p.a.page + A::kUnit - 1) / A::kUnit + 1;  // units of a pair
     const bool whole = P < 2 || longest <= 2 || longest * pairs >= (1ll << 31);
     if (whole) {
-        hipLaunchKernelGGL(pair, dim3((unsigned)pairs), dim3(64 * NW), lds, st, p);
+        launch_blocks(pairs, 64 * NW, [&](int first, unsigned n) {
+            hipLaunchKernelGGL(pair, dim3(n), dim3(64 * NW), lds, st, p, first);
+        });
         return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
     }
     p.P = DivBy(P);

@@ -25,6 +25,16 @@ struct DivBy {
     }
 };
 
+// A launch has fewer than 2^32 threads (with more, those past a multiple of it run
+// and no error is reported): more blocks of `threads` go in several, launch(first,
+// blocks) each
+template <class F>
+void launch_blocks(int64_t blocks, int threads, F launch) {
+    const int64_t most = (1ll << 31) / threads;
+    for (int64_t first = 0; first < blocks; first += most)
+        launch((int)first, (unsigned)(blocks - first < most ? blocks - first : most));
+}
+
 struct PlanArgs {
     const int32_t *seq, *fresh, *free_pages, *head;
     int32_t *table, *slots, *positions, *request, *starts, *lens, *counts;
