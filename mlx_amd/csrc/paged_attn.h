@@ -172,7 +172,7 @@ struct Piece {
     Extent ex;
 };
 
-// T: type of q, cache and out; DP: head_dim, or that rounded up to 64, 128 or 256;
+// T: type of q, cache and out; DP: head_dim, or that rounded up to 64, 128, 192 or 256;
 // FULL: head_dim is DP; WHOLE: pages hold whole runs of 16 tokens, so that a run
 // has one page and its rows one scalar base (else each lane finds its token's
 // row and the others take it from there); ONCE: cache loads that leave no copy
@@ -884,7 +884,13 @@ LuxStatus launch_t(const AttnArgs& a, hipStream_t st) {
     p.a.softcap = a.softcap * kLog2e;
     if (a.D <= 64) return launch_dp<T, 64>(p, st);
     if (a.D <= 128) return launch_dp<T, 128>(p, st);
-    return a.D == 192 ? launch_full<T, 192, true>(p, st) : launch_dp<T, 256>(p, st);
+    // Padded to 192 channels instead of 256: two blocks per CU.  64 requests up to
+    // 4096 tokens, 32 heads on 8, bf16 / f32: 136 channels 121.8 / 226.6 us instead of
+    // 128.1 / 250.7, 160 132.8 / 255.6 (140.0 / 275.3), 184 153.8 / 294.1 (156.5 /
+    // 312.3); 16 of 2048 with a head each f32 160 71.2 (88.6).  Slower where there is
+    // one head of keys: 37 up to 5000, 16 heads on one f32 160 44.3 (42.7), 184 51.3
+    // (45.1; this form's f32 range kernel spills), bf16 184 28.5 (27.2).
+    return a.D <= 192 ? launch_dp<T, 192>(p, st) : launch_dp<T, 256>(p, st);
 }
 
 extern template LuxStatus launch_t<DT_F32>(const AttnArgs&, hipStream_t);
