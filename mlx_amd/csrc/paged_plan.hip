@@ -103,11 +103,11 @@ __device__ __forceinline__ void write_no_token(const PlanArgs& a, int t) {
     if (a.request) a.request[t] = -1;
 }
 
-// one launch for up to kMost requests; thread i sums a stretch of them.  With two
-// launches 1000 requests take 8.6 us instead of 5.1, 2048 with 32768 tokens 10.2
-// instead of 8.1; beyond that the one block's LDS (24 KB) and the stretches
-// per thread grow on.
-constexpr int kMost = 2048;
+// one launch for up to kMost requests; thread i sums a stretch of them.  With one
+// and with two launches, a token each (32768 tokens take as long): 600 requests 4.7
+// and 8.9 us, 1000 5.2 and 8.8, 2048 7.8 and 10.2, 3000 8.0 and 12.1, 4096 11.7 and
+// 12.9.  Beyond that the block's LDS (48 KB) and the stretches per thread grow on.
+constexpr int kMost = 4096;
 __global__ __launch_bounds__(256) void plan_kernel(PlanArgs a) {
     __shared__ int part[4][2];
     __shared__ int starts[kMost + 1], firsts[kMost], seqs[kMost];

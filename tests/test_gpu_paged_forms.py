@@ -82,3 +82,14 @@ def test_plan_of_many_tokens(ctx):
     check_plan(ctx, [5, 0, 100], [200000, 1, 150003], 64, 6000, seed=1)
     check_plan(ctx, [5, 0, 100], [200000, 1, 150003], 64, 6000, max_tokens=270001, spare=-100, seed=2)
     check_plan(ctx, [3] * 2500, [130] * 2500, 16, 20, seed=3)
+
+
+@pytest.mark.parametrize("R", [2047, 2048, 2049, 4095, 4096, 4097])
+def test_plan_of_very_many_requests(ctx, R):
+    """On both sides of what one launch takes, each thread's stretch of requests ragged at its end."""
+    gen = torch.Generator().manual_seed(R)
+    seq, new = torch.randint(0, 60, (R,), generator=gen).tolist(), torch.randint(0, 2, (R,), generator=gen).tolist()
+    new[-1], new[R // 3] = 70, 300
+    check_plan(ctx, seq, new, 16, 24, spare=-2, head=5, seed=R)
+    new[0] = 300000
+    check_plan(ctx, seq, new, 16, 24, max_tokens=280000, seed=R)
