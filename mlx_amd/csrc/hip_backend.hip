@@ -55,25 +55,21 @@ LuxBackendContext* hip_create_context(int device_index) {
     std::snprintf(ctx->name, sizeof(ctx->name), "%s (%s)", p.name, p.gcnArchName);
     ctx->compute_units = p.multiProcessorCount;
     ctx->max_wg = p.maxThreadsPerBlock;
-    // without a workspace the kernels that need one are skipped
-    if (hipMalloc(&ctx->ws, lxq::kSplitWorkspaceBytes) == hipSuccess) {
-        if (hipMemset(ctx->ws, 0, lxq::kSplitWorkspaceBytes) == hipSuccess) {
-            ctx->ws_bytes = lxq::kSplitWorkspaceBytes;
-        } else {
-            hipFree(ctx->ws);
-            ctx->ws = nullptr;
+    // without a workspace the kernels that need one are skipped.  Zeroed on the
+    // context's stream, which does not wait for the null stream
+    auto zeroed = [&](size_t bytes) -> void* {
+        void* p = nullptr;
+        if (hipMalloc(&p, bytes) != hipSuccess) {
+            (void)hipGetLastError();
+            return nullptr;
         }
-    } else {
-        (void)hipGetLastError();
-        ctx->ws = nullptr;
-    }
-    if (hipMalloc(&ctx->counts, kCountWords * 4) != hipSuccess) {
-        (void)hipGetLastError();
-        ctx->counts = nullptr;
-    } else if (hipMemset(ctx->counts, 0, kCountWords * 4) != hipSuccess) {
-        hipFree(ctx->counts);
-        ctx->counts = nullptr;
-    }
+        if (hipMemsetAsync(p, 0, bytes, ctx->stream) == hipSuccess) return p;
+        hipFree(p);
+        return nullptr;
+    };
+    ctx->ws = zeroed(lxq::kSplitWorkspaceBytes);
+    ctx->ws_bytes = ctx->ws ? lxq::kSplitWorkspaceBytes : 0;
+    ctx->counts = zeroed(kCountWords * 4);
     return reinterpret_cast<LuxBackendContext*>(ctx);
 }
 
