@@ -18,8 +18,9 @@
  *
  * Errors: NULL handle, negative or impossible size, a struct_size that is not
  * the record's, a buffer smaller than the sizes need, a stride below the row
- * length, an output that overlaps an input or another output (but where an op
- * allows it) -> INVALID_ARGUMENT; a dtype, head_dim, dim or pool size outside
+ * length, an output that overlaps an input or another output (from first to last
+ * element, rows between those of the other included; but where an op allows it)
+ * -> INVALID_ARGUMENT; a dtype, head_dim, dim or pool size outside
  * the stated ones -> NOT_SUPPORTED; HIP launch failure -> INTERNAL.  All ops
  * are asynchronous on the context's stream and make no allocation.  Strides
  * and offsets are in elements; a stride of 0 stands for the row length.
@@ -79,7 +80,8 @@ typedef struct lux_paged_plan_args {
 /*
  * k_cache, v_cache at slots[t] = k[t], v[t] (rounded to cache_dtype, RNE), for
  * each t < tokens whose slot is in [0, num_pages * page_size); other tokens
- * are left out.  Two tokens of one call with the same slot: either may stay.
+ * are left out.  Two tokens of one call with the same slot: each value is one
+ * of the two.
  * Row t of k is k_offset + t * k_row_stride elements in, its heads next to
  * each other; so for v.
  */
@@ -153,9 +155,9 @@ typedef enum {
  * x is a block's output, post_norm the norm after it, pre_norm the norm before
  * the next block.  In fp32, h unrounded into pre_norm; each output is rounded
  * once.  A NULL weight is 1, a NULL bias 0.  residual NULL: h = gate *
- * post_norm(x).  Rows of gate are gate_row_stride apart (GATE_ROW: its values).  residual_out or out may be NULL, not both.  residual_out may
- * be residual itself, and out may be x (same place, stride and dtype).  dim:
- * at most 65536.
+ * post_norm(x).  Rows of gate are gate_row_stride apart (GATE_ROW: its values).
+ * residual_out or out may be NULL, not both.  residual_out may be residual
+ * itself, and out may be x (same place, stride and dtype).  dim: at most 65536.
  */
 typedef struct lux_block_norm_args {
     uint32_t struct_size;

@@ -837,6 +837,10 @@ LuxStatus launch_d(Params& p, hipStream_t st) {
     if ((size_t)P * one > p.a.ws_bytes) P = (int)(p.a.ws_bytes / one);
     if (P > p.a.counts / 3) P = p.a.counts / 3;
     const int64_t longest = ((int64_t)p.a.columns * p.a.page + A::kUnit - 1) / A::kUnit + 1;  // units of a pair
+    // Tables of up to two units: a block per pair.  Longer ones may belong to short
+    // or uneven requests, and are cut: 512 requests up to 2000 tokens, 8 heads on 2
+    // of 64, 53.8 us (64.2 whole), 1024 100.3 (102.7); but up to 300 tokens, 8 heads
+    // on one of 128, 1024 take 27.2 (19.7)
     const bool whole = P < 2 || longest <= 2 || longest * pairs >= (1ll << 31);
     if (whole) {
         launch_blocks(pairs, 64 * NW, [&](int first, unsigned n) {
