@@ -195,11 +195,12 @@ typedef struct lux_gpu_serving_vtbl {
      * buffer_free, which leaves the memory alone.  NULL where device_ptr is
      * no memory of the context's device.  Work of other streams on that memory
      * is the caller's to order.  The serving ops read nothing past `bytes`.
-     * The quantized ops, which take operands in vectors, refuse a wrapped one
-     * (INVALID_ARGUMENT) that does not start on 16 bytes, and an input without 256
-     * readable bytes behind what they need of it: in the buffer or in the
-     * rest of the allocation that it lies in.  The base table's ops ask for 4
-     * bytes (matmul: and 12 readable ones behind its inputs). */
+     * The quantized ops read their inputs (but a fused bias) in vectors: they
+     * refuse a wrapped one (INVALID_ARGUMENT) that does not start on 16 bytes or
+     * has not 256 readable bytes behind what they need of it, in the buffer or in
+     * the rest of the allocation that it lies in.  Their outputs start on an
+     * element (op_dequantize's on 16 bytes, codes on 4).  The base table's ops ask for
+     * 4 bytes (matmul: and 12 readable ones behind its inputs). */
     LuxBackendBuffer* (*buffer_wrap)(LuxBackendContext* ctx, void* device_ptr, size_t bytes);
 
     void* _reserved[5];

@@ -331,8 +331,8 @@ LuxBackendError qmm_impl(LuxBackendContext* c, LuxBackendBuffer* x, LuxBackendBu
     if (!read_by(B(x), (size_t)M * K * dtype_size(x_dtype)) || !read_by(B(w_q), (size_t)N * K * bits / 8) ||
         !read_by(B(scales), (size_t)N * G * dtype_size(sb_dtype)) ||
         !read_by(B(biases), (size_t)N * G * dtype_size(sb_dtype)) ||
-        !written_by(B(out), (size_t)M * N * dtype_size(out_dtype)) ||
-        (bias && !read_by(B(bias), (size_t)N * dtype_size(bias_dtype))))
+        !taken_by(B(out), (size_t)M * N * dtype_size(out_dtype), dtype_size(out_dtype)) ||
+        (bias && !taken_by(B(bias), (size_t)N * dtype_size(bias_dtype), dtype_size(bias_dtype))))
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     if (M == 0 || N == 0) return LUX_BACKEND_OK;
 
@@ -399,7 +399,7 @@ LuxBackendError hip_op_dequantize(LuxBackendContext* c, LuxBackendBuffer* w_q,
     const size_t G = (size_t)(K / group_size);
     if (!read_by(B(w_q), (size_t)N * K * bits / 8) || !read_by(B(scales), (size_t)N * G * dtype_size(sb_dtype)) ||
         !read_by(B(biases), (size_t)N * G * dtype_size(sb_dtype)) ||
-        !written_by(B(out), (size_t)N * K * dtype_size(out_dtype)))
+        !taken_by(B(out), (size_t)N * K * dtype_size(out_dtype), 16))
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     if (N == 0) return LUX_BACKEND_OK;
     if (hipSetDevice(ctx->device) != hipSuccess) return LUX_BACKEND_ERROR_DEVICE_LOST;
@@ -418,9 +418,9 @@ LuxBackendError hip_op_quantize(LuxBackendContext* c, LuxBackendBuffer* w, LuxBa
     if (e != LUX_BACKEND_OK) return e;
     if (!dtype_ok(w_dtype) || !dtype_ok(sb_dtype)) return LUX_BACKEND_ERROR_NOT_SUPPORTED;
     const size_t G = (size_t)(K / group_size);
-    if (!read_by(B(w), (size_t)N * K * dtype_size(w_dtype)) || !written_by(B(w_q), (size_t)N * K * bits / 8) ||
-        !written_by(B(scales), (size_t)N * G * dtype_size(sb_dtype)) ||
-        !written_by(B(biases), (size_t)N * G * dtype_size(sb_dtype)))
+    if (!read_by(B(w), (size_t)N * K * dtype_size(w_dtype)) || !taken_by(B(w_q), (size_t)N * K * bits / 8, 4) ||
+        !taken_by(B(scales), (size_t)N * G * dtype_size(sb_dtype), dtype_size(sb_dtype)) ||
+        !taken_by(B(biases), (size_t)N * G * dtype_size(sb_dtype), dtype_size(sb_dtype)))
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     if (N == 0) return LUX_BACKEND_OK;
     if (hipSetDevice(ctx->device) != hipSuccess) return LUX_BACKEND_ERROR_DEVICE_LOST;

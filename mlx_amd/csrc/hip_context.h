@@ -75,9 +75,10 @@ inline bool reaches(HipBuffer* b, size_t need, size_t align, size_t past) {
     return need == 0 || b->owned ||
            (reinterpret_cast<uintptr_t>(b->ptr) % align == 0 && b->size - need + b->tail >= past);
 }
-// operands of the quantized ops
+// operands of the quantized ops: those that they read in vectors, and those that
+// they take element by element or in vectors that may start on any of `align` bytes
 inline bool read_by(HipBuffer* b, size_t need) { return reaches(b, need, 16, lxq::kTailPad); }
-inline bool written_by(HipBuffer* b, size_t need) { return reaches(b, need, 16, 0); }
+inline bool taken_by(HipBuffer* b, size_t need, size_t align) { return reaches(b, need, align, 0); }
 
 }  // namespace lxh
 

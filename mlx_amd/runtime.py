@@ -112,8 +112,8 @@ class Context:
     def wrap(self, address: int, nbytes: int) -> Buffer:
         """A buffer over device memory that the caller owns and keeps; free()
         leaves the memory alone.  Ordering other streams' work on it is the
-        caller's.  The quantized ops refuse it where it does not start on 16
-        bytes or (inputs) has not 256 bytes of its allocation behind it."""
+        caller's.  The quantized ops refuse it as an input where it does not
+        start on 16 bytes or has not 256 bytes of its allocation behind it."""
         h = self._serving().buffer_wrap(self.handle, address, nbytes)
         if not h:
             raise LuxError(abi.ERR_INVALID_ARGUMENT, f"buffer_wrap({address:#x}, {nbytes})")

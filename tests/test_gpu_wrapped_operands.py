@@ -55,12 +55,13 @@ def call(ctx, op, arrays, out_bytes, make, block, wrapped, at):
     return err, got
 
 
-def sweep(ctx, block, op, arrays, out_bytes, make, align, past):
+def sweep(ctx, block, op, arrays, out_bytes, make, needs):
+    """needs: per operand, the output last, the bytes that it starts on and those behind it."""
     err, want = call(ctx, op, arrays, out_bytes, make, block, None, 0)
     assert err == abi.OK
     for i in range(len(arrays) + 1):
         n = arrays[i].nbytes if i < len(arrays) else out_bytes
-        need = past if i < len(arrays) else 0
+        align, need = needs[i]
         end = (SIZE - n) // align * align
         for at, ok in [(0, True), (5 * align, True), ((SIZE - n - need) // align * align, True), (64 + align // 2, False),
                        (end, SIZE - n - end >= need), (end - align, SIZE - n - end + align >= need)]:
@@ -75,15 +76,15 @@ def test_quantized_matmul(ctx, oracle, block, M, K, N, bits):
     x, w, s, b, _ = oracle.make_problem(M, K, N, bits, 64, F16, F16, seed=M)
     bias = np.random.default_rng(1).standard_normal(N).astype(np.float32)
     sweep(ctx, block, ctx.q.op_quantized_matmul, [x, w, s, b], M * N * 2,
-          lambda f, h: f(ctx.handle, *h, M, K, N, 64, bits, F16, F16, F16), 16, 256)
+          lambda f, h: f(ctx.handle, *h, M, K, N, 64, bits, F16, F16, F16), [(16, 256)] * 4 + [(2, 0)])
     sweep(ctx, block, ctx.q.op_quantized_matmul_fused, [x, w, s, b, bias], M * N * 4,
-          lambda f, h: f(ctx.handle, *h, M, K, N, 64, bits, F16, F16, F32, F32, 1), 16, 256)
+          lambda f, h: f(ctx.handle, *h, M, K, N, 64, bits, F16, F16, F32, F32, 1), [(16, 256)] * 4 + [(4, 0)] * 2)
 
 
 def test_dequantize_and_quantize(ctx, oracle, block):
     K, N = 512, 96
     _, w, s, b, _ = oracle.make_problem(1, K, N, 6, 32, F16, F32, seed=2)
-    sweep(ctx, block, ctx.q.op_dequantize, [w, s, b], N * K * 2, lambda f, h: f(ctx.handle, *h, N, K, 32, 6, F32, F16), 16, 256)
+    sweep(ctx, block, ctx.q.op_dequantize, [w, s, b], N * K * 2, lambda f, h: f(ctx.handle, *h, N, K, 32, 6, F32, F16), [(16, 256)] * 3 + [(16, 0)])
     full = np.random.default_rng(3).standard_normal((N, K)).astype(np.float32)
     spare = [ctx.alloc(N * K), ctx.alloc(N * K)]
 
@@ -94,8 +95,8 @@ def test_dequantize_and_quantize(ctx, oracle, block):
             return f(ctx.handle, h[0], *outs, N, K, 32, 4, F32, F32)
         return make
 
-    sweep(ctx, block, ctx.q.op_quantize, [full], N * K // 2, to(0), 16, 256)
-    sweep(ctx, block, ctx.q.op_quantize, [full], N * K // 32 * 4, to(1), 16, 256)
+    sweep(ctx, block, ctx.q.op_quantize, [full], N * K // 2, to(0), [(16, 256), (4, 0)])
+    sweep(ctx, block, ctx.q.op_quantize, [full], N * K // 32 * 4, to(1), [(16, 256), (4, 0)])
     for sp in spare:
         sp.free()
 
@@ -104,9 +105,9 @@ def test_base_ops(ctx, block):
     rng = np.random.default_rng(4)
     a, b = (rng.standard_normal(1003).astype(np.float32) for _ in range(2))
     for name in ("op_add_f32", "op_sub_f32", "op_mul_f32", "op_div_f32"):
-        sweep(ctx, block, getattr(ctx.vt, name), [a, b], a.nbytes, lambda f, h: f(ctx.handle, *h, a.size), 4, 0)
+        sweep(ctx, block, getattr(ctx.vt, name), [a, b], a.nbytes, lambda f, h: f(ctx.handle, *h, a.size), [(4, 0)] * 3)
     for M, K, N in [(5, 7, 9), (70, 33, 65)]:
         x, y = (rng.standard_normal(s).astype(np.float32) for s in ((M, K), (K, N)))
-        sweep(ctx, block, ctx.vt.op_matmul_f32, [x, y], M * N * 4, lambda f, h: f(ctx.handle, *h, M, K, N), 4, 12)  # noqa: B023
+        sweep(ctx, block, ctx.vt.op_matmul_f32, [x, y], M * N * 4, lambda f, h: f(ctx.handle, *h, M, K, N), [(4, 12), (4, 12), (4, 0)])  # noqa: B023
     x = rng.standard_normal((33, 65)).astype(np.float32)
-    sweep(ctx, block, ctx.vt.op_transpose_f32, [x], x.nbytes, lambda f, h: f(ctx.handle, *h, 33, 65), 4, 0)
+    sweep(ctx, block, ctx.vt.op_transpose_f32, [x], x.nbytes, lambda f, h: f(ctx.handle, *h, 33, 65), [(4, 0)] * 2)
