@@ -140,3 +140,24 @@ def test_length_just_below_31_bits(ctx, page, columns):
     want = torch.softmax(s, 0) @ vc[0, 0].double()
     assert ((got[0].double() - want).abs() <= (2.0 ** -5 + ROUND[F16]) * want).all()
     assert abs(float(lse) - float(torch.logsumexp(s, 0) + torch.log(torch.tensor(float(columns), dtype=torch.float64)))) <= 2.0 ** -5
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_nan_and_lowest_scores(ctx, dtype):
+    """NaN in a key that counts makes its heads NaN and no other; a key of score -infinity has no weight."""
+    q, kc, vc, table, n = problem(720 + dtype, dtype, [50, 700], 4, 2, 64, 16, poison=False)
+    kc[int(table[0, 1]), 0, 3] = -INF * torch.sign(q[0, :64])  # head 0 of request 0; head 1 has infinities of both signs: NaN
+    kc[int(table[1, 2]), 1, 5, 0] = float("nan")
+    got, lse = attend(ctx, q, kc, vc, table, n, 4, dtype)
+    got = got.double().view(2, 4, 64)
+    assert torch.isnan(got[1, 2:]).all() and torch.isnan(lse[1, 2:]).all()
+    kc[int(table[1, 2]), 1, 5, 0] = 0
+    kc[int(table[0, 1]), 0, 3] = 0
+    out, _, tol = attention_reference(q, kc, vc, table, n, 4, scale=0.125)
+    keep = torch.tensor([[False, False, True, True], [True, True, False, False]])
+    bound = (tol + {F32: 0, F16: 2.0 ** -21, BF16: 2.0 ** -16}[dtype])[..., None] * float(vc.double().abs().max()) + ROUND[dtype] * out.abs() + 2.0 ** -25
+    assert ((got - out).abs() <= bound)[keep].all()
+    t = torch.tensor([t for t in range(50) if t != 19])
+    k, v = (c[table[0, t // 16].long(), 0, t % 16].double() for c in (kc, vc))
+    want = torch.softmax(k @ q[0, :64].double() / 8, 0) @ v
+    assert ((got[0, 0] - want).abs() <= bound[0, 0] + ROUND[dtype] * want.abs()).all()
