@@ -202,6 +202,9 @@ struct Attn {
     static constexpr size_t lds_bytes(int rows) { return lds_floats(rows) * 4 + 16; }
 
     __device__ __forceinline__ static int dim(const AttnArgs& a) { return FULL ? DP : a.D; }
+    // channel d of a row, in a run of channels that ends at `end`, is one of
+    // head_dim's: below DP - 64 all are, smaller head dims take the next smaller form
+    __device__ __forceinline__ static bool has(const AttnArgs& a, int d, int end) { return FULL || end <= DP - 64 || d < a.D; }
 
     u4 q[NC], k[SUB][NC];
     uv v[4 * SUB][NV];
@@ -270,8 +273,8 @@ struct Attn {
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             const int d = (4 * c + (lane >> 4)) * E;
-            q[c] = *reinterpret_cast<const u4h*>(p + (FULL || d < dim(a) ? d * ES : 0));
-            if (!FULL && d >= dim(a)) q[c] = u4{0, 0, 0, 0};
+            q[c] = *reinterpret_cast<const u4h*>(p + (has(a, d, 4 * (c + 1) * E) ? d * ES : 0));
+            if (!has(a, d, 4 * (c + 1) * E)) q[c] = u4{0, 0, 0, 0};
         }
     }
 
@@ -288,7 +291,7 @@ struct Attn {
             const char* p = at_row(a, a.kc, s, lane & 15) + (lane >> 4) * 16;
 #pragma unroll
             for (int c = 0; c < NC; c++)
-                if (FULL || (4 * c + (lane >> 4)) * E < dim(a)) k[s][c] = load<u4>(p + c * 64);
+                if (has(a, (4 * c + (lane >> 4)) * E, 4 * (c + 1) * E)) k[s][c] = load<u4>(p + c * 64);
         }
     }
     __device__ __forceinline__ void load_v(const AttnArgs& a) {
@@ -299,7 +302,7 @@ struct Attn {
 #pragma unroll
             for (int c = 0; c < NV; c++) {
                 const int d = (16 * c + (lane & 15)) * VE;  // past head_dim: channels that are not stored
-                v[t][c] = load<uv>(p + (FULL || d < dim(a) ? d * ES : 0));
+                v[t][c] = load<uv>(p + (has(a, d, 16 * (c + 1) * VE) ? d * ES : 0));
             }
         }
     }
@@ -889,11 +892,10 @@ LuxStatus launch_t(const AttnArgs& a, hipStream_t st) {
     if (a.D <= 64) return launch_dp<T, 64>(p, st);
     if (a.D <= 128) return launch_dp<T, 128>(p, st);
     // Padded to 192 channels instead of 256: two blocks per CU.  64 requests up to
-    // 4096 tokens, 32 heads on 8, bf16 / f32: 136 channels 121.8 / 226.6 us instead of
-    // 128.1 / 250.7, 160 132.8 / 255.6 (140.0 / 275.3), 184 153.8 / 294.1 (156.5 /
-    // 312.3); 16 of 2048 with a head each f32 160 71.2 (88.6).  Slower where there is
-    // one head of keys: 37 up to 5000, 16 heads on one f32 160 44.3 (42.7), 184 51.3
-    // (45.1; this form's f32 range kernel spills), bf16 184 28.5 (27.2).
+    // 4096 tokens, 32 heads on 8, bf16 / f32: 136 channels 117.1 / 220.0 us instead of
+    // 125.2 / 251.0, 160 135.1 / 244.3 (138.5 / 275.5), 184 150.6 / 285.0 (156.4 /
+    // 310.2); 16 of 2048 with a head each f32 160 67.2 (88.4).  Slower at 184 with
+    // one head of keys (37 up to 5000, 16 heads on it: 28.5 / 47.1, 26.7 / 44.8).
     return a.D <= 192 ? launch_dp<T, 192>(p, st) : launch_dp<T, 256>(p, st);
 }
 
