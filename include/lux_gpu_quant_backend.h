@@ -31,6 +31,7 @@
 #define LUX_GPU_QUANT_BACKEND_H
 
 #include "lux_gpu_backend_abi.h"
+#include "lux_gpu_prompt_backend.h"
 #include "lux_gpu_serving_backend.h"
 
 #ifdef __cplusplus
@@ -168,7 +169,11 @@ typedef struct lux_gpu_quant_vtbl {
      * plugins that predate them */
     const lux_gpu_serving_vtbl* serving;
 
-    void* _reserved[3];
+    /* the operators of prompts and of pages in use (lux_gpu_prompt_backend.h);
+     * NULL in plugins that predate them */
+    const lux_gpu_prompt_vtbl* prompt;
+
+    void* _reserved[2];
 } lux_gpu_quant_vtbl;
 
 /* layout pins: LP64 */

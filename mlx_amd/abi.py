@@ -220,6 +220,65 @@ class ServingVtbl(C.Structure):
     ]
 
 
+# prompts and pages in use (include/lux_gpu_prompt_backend.h)
+PROMPT_EXT_VERSION = 1
+
+
+class PagedChunkArgs(_Args):
+    """lux_paged_chunk_args."""
+    _fields_ = _fields(["requests", "tokens", "heads", "kv_heads", "head_dim", "page_size", "num_pages", "max_pages",
+                        "window", "dtype"], ["scale", "softcap"],
+                       ["q_offset", "q_row_stride", "out_offset", "out_row_stride"],
+                       ["q", "k_cache", "v_cache", "block_table", "token_starts", "seq_lens", "kv_lens", "out", "lse"],
+                       pad=["_pad"])
+
+
+class PagedForkArgs(_Args):
+    """lux_paged_fork_args."""
+    _fields_ = _fields(["forks", "requests", "max_pages", "page_size", "num_pages", "free_count"], [], [],
+                       ["src", "dst", "lens", "block_table", "shares", "free_pages", "free_head", "copy_src", "copy_dst",
+                        "counts"], pad=["_pad"])
+
+
+class PagedReleaseArgs(_Args):
+    """lux_paged_release_args."""
+    _fields_ = _fields(["requests", "max_pages", "page_size", "num_pages", "free_count"], [], [],
+                       ["lens", "keep_lens", "block_table", "shares", "free_pages", "free_head", "kv_lens", "counts"])
+
+
+class PagedCompactArgs(_Args):
+    """lux_paged_compact_args."""
+    _fields_ = _fields(["requests", "max_pages", "page_size", "num_pages", "free_count", "limit", "max_moves"], [], [],
+                       ["lens", "block_table", "shares", "table_out", "shares_out", "free_pages", "copy_src", "copy_dst",
+                        "counts"])
+
+
+class PagedCopyArgs(_Args):
+    """lux_paged_copy_args."""
+    _fields_ = _fields(["pages", "layers", "kv_heads", "head_dim", "page_size", "num_pages", "dtype"], [],
+                       ["layer_stride"], ["copy_src", "copy_dst", "k_cache", "v_cache"])
+
+
+class TokenLogprobsArgs(_Args):
+    """lux_token_logprobs_args."""
+    _fields_ = _fields(["rows", "vocab", "top", "dtype"], ["scale"], ["logits_offset", "row_stride"],
+                       ["logits", "tokens", "logprobs", "entropy", "lse", "top_ids", "top_logprobs"])
+
+
+class PromptVtbl(C.Structure):
+    _fields_ = [
+        ("ext_version", C.c_uint32),
+        ("struct_size", C.c_uint32),
+        ("op_paged_chunk_attention", C.CFUNCTYPE(Err, Ctx, C.POINTER(PagedChunkArgs))),
+        ("op_paged_fork", C.CFUNCTYPE(Err, Ctx, C.POINTER(PagedForkArgs))),
+        ("op_paged_release", C.CFUNCTYPE(Err, Ctx, C.POINTER(PagedReleaseArgs))),
+        ("op_paged_compact", C.CFUNCTYPE(Err, Ctx, C.POINTER(PagedCompactArgs))),
+        ("op_paged_copy", C.CFUNCTYPE(Err, Ctx, C.POINTER(PagedCopyArgs))),
+        ("op_token_logprobs", C.CFUNCTYPE(Err, Ctx, C.POINTER(TokenLogprobsArgs))),
+        ("_reserved", C.c_void_p * 8),
+    ]
+
+
 class QuantVtbl(C.Structure):
     _fields_ = [
         ("ext_version", C.c_uint32),
@@ -235,7 +294,8 @@ class QuantVtbl(C.Structure):
         ("linear_load", LINEAR_LOAD),
         ("linear_free", LINEAR_FREE),
         ("serving", C.POINTER(ServingVtbl)),
-        ("_reserved", C.c_void_p * 3),
+        ("prompt", C.POINTER(PromptVtbl)),
+        ("_reserved", C.c_void_p * 2),
     ]
 
 
@@ -255,6 +315,9 @@ def check_layout() -> None:
     assert QuantVtbl.linear_free.offset == 80 and C.sizeof(LinearInfo) == 96
     assert QuantVtbl.serving.offset == 88 and C.sizeof(ServingVtbl) == 88
     assert [C.sizeof(t) for t in (PagedPlanArgs, PagedAppendArgs, PagedAttentionArgs, BlockNormArgs)] == [120, 104, 136, 160]
+    assert QuantVtbl.prompt.offset == 96 and C.sizeof(PromptVtbl) == 120
+    assert [C.sizeof(t) for t in (PagedChunkArgs, PagedForkArgs, PagedReleaseArgs, PagedCompactArgs, PagedCopyArgs,
+                                  TokenLogprobsArgs)] == [160, 112, 88, 104, 72, 96]
 
 
 check_layout()

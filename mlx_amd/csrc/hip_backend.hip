@@ -70,6 +70,10 @@ LuxBackendContext* hip_create_context(int device_index) {
     ctx->ws = zeroed(lxq::kSplitWorkspaceBytes);
     ctx->ws_bytes = ctx->ws ? lxq::kSplitWorkspaceBytes : 0;
     ctx->counts = zeroed(kCountWords * 4);
+    if (hipMalloc(&ctx->parts, lxq::kChunkPartBytes) != hipSuccess) {
+        (void)hipGetLastError();
+        ctx->parts = nullptr;
+    }
     return reinterpret_cast<LuxBackendContext*>(ctx);
 }
 
@@ -83,6 +87,7 @@ void hip_destroy_context(LuxBackendContext* c) {
     }
     if (ctx->ws) hipFree(ctx->ws);
     if (ctx->counts) hipFree(ctx->counts);
+    if (ctx->parts) hipFree(ctx->parts);
     delete ctx;
 }
 
@@ -585,6 +590,7 @@ lux_gpu_quant_vtbl make_qvtbl() {
     q.linear_load = hip_linear_load;
     q.linear_free = hip_linear_free;
     q.serving = lux_hip_serving_table();
+    q.prompt = lux_hip_prompt_table();
     return q;
 }
 

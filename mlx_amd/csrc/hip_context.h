@@ -4,8 +4,9 @@
 #include <hip/hip_runtime.h>
 
 #include "../../include/lux_gpu_backend_abi.h"
+#include "../../include/lux_gpu_prompt_backend.h"
 #include "../../include/lux_gpu_serving_backend.h"
-#include "kernels.h"
+#include "prompt.h"
 
 namespace lxh {
 
@@ -27,6 +28,9 @@ struct HipContext {
     // arrival counters of the attention's split pairs (three per range), zero
     // between launches; without them the attention is not split
     void* counts = nullptr;
+    // partial results of the chunk attention's split tiles; like ws, used only
+    // by work on `stream`
+    void* parts = nullptr;
 };
 constexpr int kCountWords = 2048;
 
@@ -84,3 +88,5 @@ inline bool taken_by(HipBuffer* b, size_t need, size_t align) { return reaches(b
 
 // the table of include/lux_gpu_serving_backend.h
 const lux_gpu_serving_vtbl* lux_hip_serving_table();
+// and of include/lux_gpu_prompt_backend.h
+const lux_gpu_prompt_vtbl* lux_hip_prompt_table();

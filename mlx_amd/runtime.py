@@ -83,6 +83,8 @@ class Context:
             raise RuntimeError(f"create_context({device_index}) failed")
         serving = getattr(self.q, "serving", None)
         self.s = serving.contents if serving else None
+        prompt = getattr(self.q, "prompt", None)
+        self.p = prompt.contents if prompt else None
 
     def close(self) -> None:
         if self.handle:
@@ -213,6 +215,36 @@ class Context:
     def block_norm(self, args: abi.BlockNormArgs) -> None:
         """h = residual_scale * residual + gate * post_norm(x); out = pre_norm(h)."""
         _check(self._serving().op_block_norm(self.handle, args), "op_block_norm")
+
+    # --- prompts and pages in use (asynchronous on the context stream), records as above ---
+    def _prompt(self) -> abi.PromptVtbl:
+        if self.p is None:
+            raise LuxError(abi.ERR_NOT_SUPPORTED, "prompt operators")
+        return self.p
+
+    def paged_chunk_attention(self, args: abi.PagedChunkArgs) -> None:
+        """Attention of a chunk of new tokens per request over its cached tokens."""
+        _check(self._prompt().op_paged_chunk_attention(self.handle, args), "op_paged_chunk_attention")
+
+    def paged_fork(self, args: abi.PagedForkArgs) -> None:
+        """Requests that begin as copies of others: full pages shared, the rest a page of its own."""
+        _check(self._prompt().op_paged_fork(self.handle, args), "op_paged_fork")
+
+    def paged_release(self, args: abi.PagedReleaseArgs) -> None:
+        """Pages of requests that end or are cut, back to the free list."""
+        _check(self._prompt().op_paged_release(self.handle, args), "op_paged_release")
+
+    def paged_compact(self, args: abi.PagedCompactArgs) -> None:
+        """Live pages from a limit on get places below it; the free list is made anew."""
+        _check(self._prompt().op_paged_compact(self.handle, args), "op_paged_compact")
+
+    def paged_copy(self, args: abi.PagedCopyArgs) -> None:
+        """The contents of pages, in every layer's cache."""
+        _check(self._prompt().op_paged_copy(self.handle, args), "op_paged_copy")
+
+    def token_logprobs(self, args: abi.TokenLogprobsArgs) -> None:
+        """Log probabilities of given tokens, entropy and top alternatives of rows of logits."""
+        _check(self._prompt().op_token_logprobs(self.handle, args), "op_token_logprobs")
 
     # base f32 tensor ops (vtable slots, as the reference core calls them)
     def binary_f32(self, op: str, a: Buffer, b: Buffer, out: Buffer, n: int) -> None:
