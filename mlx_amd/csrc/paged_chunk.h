@@ -70,6 +70,19 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ int scalar_at(const int32_t* p, int64_t i) {
     return ((const __attribute__((address_space(4))) int32_t*)p)[i];
 }
+// The kernel's argument, read again from where it lies: a loop keeps the scalars
+// that it uses, and those of the code around it are no burden to it
+__device__ __forceinline__ const Params& argument() {
+    auto p = (const __attribute__((address_space(4))) Params*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Params*)p;
+}
+// the same value, for code that is to work out again what follows from it instead
+// of keeping it in registers through other loops
+__device__ __forceinline__ int afresh(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 __device__ __forceinline__ int clamp(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
 // rows and tokens of a tile
@@ -221,6 +234,10 @@ struct Chunk {
     // and weights stay below 2^16 in f16
     static constexpr float kBehind = T == DT_F16 ? 1.f : 8.f;
 
+    // where the registers are short, operands of so many steps ahead are loaded and
+    // no more (0: as the compiler likes)
+    static constexpr int kFence = T == DT_F32 && DP >= 128 ? 2 : DP == 256 || (DP == 128 && !WHOLE) ? 4 : 0;
+
     // permutations of a row's chunks
     __device__ __forceinline__ static int k_turn(int row) { return row & KM; }
     __device__ __forceinline__ static int v_turn(int row) {
@@ -228,45 +245,36 @@ struct Chunk {
         else return CPR < 16 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
     }
 
-    const Params& p;
-    const ChunkArgs& a;
     char* lds;
     int lane, w, rg, kg;
-    uint32_t koff[NI], voff[NI];  // the lane's chunk of its wave's runs: bytes from the run's first row
-    bool kon[NI], von[NI];        // is it one of head_dim's
+    uint32_t koff, voff;  // bytes of the lane's chunk in a run at a multiple of 16 tokens
 
     u4 q[NK];
     f16v o[ND];
     float m, l;
     int lo, len;  // the cached tokens that the lane's row sees
-    int page[NI];
 
-    __device__ __forceinline__ Chunk(const Params& params, char* mem) : p(params), a(params.a), lds(mem) {
+    __device__ __forceinline__ explicit Chunk(char* mem) : lds(mem) {
         lane = threadIdx.x & 63;
         w = uniform(threadIdx.x >> 6);
         rg = w % RG;
         kg = w / RG;
-        const int ri = lane / CPR, c = lane % CPR, len16 = a.D / E;
-#pragma unroll
-        for (int j = 0; j < NI; j++) {
-            const int row = (w * NI + j) * TI + ri;
-            const int ck = c ^ k_turn(row), cv = c ^ v_turn(row);
-            kon[j] = ck < len16;
-            von[j] = cv < len16;
-            koff[j] = (uint32_t)(ri * a.D * ES + ck * 16);
-            voff[j] = (uint32_t)(ri * a.D * ES + cv * 16);
-        }
+        const int ri = lane / CPR, c = lane % CPR;
+        koff = (uint32_t)((c ^ k_turn(ri)) * 16);
+        voff = (uint32_t)((c ^ v_turn(ri)) * 16);
     }
 
     // a stage's transfers into LDS stage `buf`: tokens from tb on, those past the
     // tile's last one from its row
-    __device__ __forceinline__ void fill(const Tile& t, int r, int hk, int tb, int buf) {
+    __device__ __forceinline__ void fill(const ChunkArgs& a, const Tile& t, int r, int hk, int tb, int buf) {
         const uint32_t dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + (uint32_t)(buf * kStage);
         const uint32_t row_bytes = (uint32_t)(a.D * ES);
+        const int ri = lane / CPR;
 #pragma unroll
         for (int j = 0; j < NI; j++) {
             const int run = w * NI + j;
             const uint32_t at_lds = dst + (uint32_t)(run * 1024);
+            const uint32_t kc = koff ^ (uint32_t)(k_turn(run * TI) * 16), vc = voff ^ (uint32_t)(v_turn(run * TI) * 16);
             const int t0 = tb + run * TI;
             if constexpr (WHOLE) {
                 const int tr = t0 < t.end ? t0 : (t.end - 1) & ~(TI - 1);
@@ -276,74 +284,69 @@ struct Chunk {
                 const uint64_t row = (uint64_t)(uint32_t)((pg * a.Hk + hk) * a.page + (tr - col * a.page));
                 const char* kp = static_cast<const char*>(a.kc) + row * row_bytes;
                 const char* vp = static_cast<const char*>(a.vc) + row * row_bytes;
-                uint32_t ko = koff[j], vo = voff[j];
-                if (tr + TI > t.end) {  // rows behind the last one: the last one's
-                    const int over = lane / CPR - (t.end - 1 - tr);
-                    const uint32_t back = over > 0 ? (uint32_t)over * row_bytes : 0u;
-                    ko -= back;
-                    vo -= back;
-                }
+                const int last = t.end - 1 - tr;  // rows behind the last one: the last one's
+                const uint32_t at_row = (uint32_t)(ri < last ? ri : last) * row_bytes;
                 if (a.D == RS / ES) {
-                    dma16(at_lds, kp, ko);
-                    dma16(at_lds + kMat, vp, vo);
+                    dma16(at_lds, kp, kc + at_row);
+                    dma16(at_lds + kMat, vp, vc + at_row);
                 } else {
-                    if (kon[j]) dma16(at_lds, kp, ko);
-                    if (von[j]) dma16(at_lds + kMat, vp, vo);
+                    if (kc < row_bytes) dma16(at_lds, kp, kc + at_row);
+                    if (vc < row_bytes) dma16(at_lds + kMat, vp, vc + at_row);
                 }
             } else {
-                const int ri = lane / CPR;
                 int tok = t0 + ri;
                 tok = tok < t.end ? tok : t.end - 1;
                 const int col = div_by(tok, a.div);
                 int pg = a.table[(int64_t)r * a.columns + col];
                 pg = (uint32_t)pg < (uint32_t)a.pool ? pg : 0;
                 const uint64_t row = (uint64_t)(uint32_t)((pg * a.Hk + hk) * a.page + (tok - col * a.page));
-                const uint32_t ri_bytes = (uint32_t)ri * row_bytes;
-                if (kon[j]) dma16a(at_lds, static_cast<const char*>(a.kc) + row * row_bytes + (koff[j] - ri_bytes));
-                if (von[j]) dma16a(at_lds + kMat, static_cast<const char*>(a.vc) + row * row_bytes + (voff[j] - ri_bytes));
+                if (kc < row_bytes) dma16a(at_lds, static_cast<const char*>(a.kc) + row * row_bytes + kc);
+                if (vc < row_bytes) dma16a(at_lds + kMat, static_cast<const char*>(a.vc) + row * row_bytes + vc);
             }
         }
     }
 
     // row of the tile -> token of the tile, head; rows past the tile's take its last
-    __device__ __forceinline__ int token_of(const Tile& t, int row, int qt, int& head) const {
+    __device__ __forceinline__ static int token_of(const Params& p, const Tile& t, int row, int qt, int& head) {
         const int last = t.m * p.GT - 1;
         row = row < last ? row : last < 0 ? 0 : last;
         const int i = div_by(row, p.by_gt);
         head = qt * p.GT + row - i * p.GT;
         return i;
     }
-    __device__ __forceinline__ bool has_row(const Tile& t, int row, int qt) const {
+    __device__ __forceinline__ static bool has_row(const Params& p, const Tile& t, int row, int qt) {
         if (row >= t.m * p.GT) return false;
         const int i = div_by(row, p.by_gt);
-        return qt * p.GT + row - i * p.GT < a.G;
+        return qt * p.GT + row - i * p.GT < p.a.G;
     }
-    __device__ __forceinline__ void sees(const Tile& t, int i, int& from, int& to) const {
+    __device__ __forceinline__ static void sees(const ChunkArgs& a, const Tile& t, int i, int& from, int& to) {
         const int pos = t.pos + i;
         from = a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0;
         to = pos + 1 < t.n ? pos + 1 : t.n;
     }
 
-    __device__ __forceinline__ void load_q(const Tile& t, int hk, int qt) {
+    __device__ __forceinline__ void load_q(const Params& p, const Tile& t, int hk, int qt) {
+        const ChunkArgs& a = p.a;
         int head;
-        const int i = token_of(t, rg * 32 + (lane & 31), qt, head);
+        const int i = token_of(p, t, rg * 32 + (lane & 31), qt, head);
         head = head < a.G ? head : a.G - 1;
         const char* src = static_cast<const char*>(a.q) + ((int64_t)(t.first + i) * a.q_row + (int64_t)(hk * a.G + head) * a.D) * ES;
-        const int h = lane >> 5;
+        const int h = afresh(lane >> 5);
 #pragma unroll
         for (int k = 0; k < NK; k++) {
             const int d = (2 * k + h) * E;
             q[k] = *reinterpret_cast<const u4h*>(src + (d < a.D ? d * ES : 0));
             q[k] = d < a.D ? q[k] ^ p.flip : u4{0, 0, 0, 0};
+            if (k % 16 == 15) __builtin_amdgcn_sched_barrier(0);
         }
         int from, to;
-        sees(t, i, from, to);
+        sees(a, t, i, from, to);
         lo = from;
         len = to > from ? to - from : 0;
     }
 
     // which of the 32 NB tokens from tb on have a page
-    __device__ __forceinline__ uint64_t pages_there(const Tile& t, int r, int tb) const {
+    __device__ __forceinline__ uint64_t pages_there(const ChunkArgs& a, const Tile& t, int r, int tb) const {
         const int tok = tb + lane;
         const bool in = lane < BT && tok < t.end;
         const int pg = in ? a.table[(int64_t)r * a.columns + div_by(tok, a.div)] : -1;
@@ -351,7 +354,8 @@ struct Chunk {
     }
 
     // a group's BT tokens of a stage, from position tb on, into m, l and o
-    __device__ __forceinline__ void take(const Tile& t, int r, int tb, int buf, bool masked, bool holes) {
+    __device__ __forceinline__ void take(const Params& p, const Tile& t, int r, int tb, int buf, bool masked, bool holes) {
+        const ChunkArgs& a = p.a;
         const int h = lane >> 5, l31 = lane & 31;
         lds_ptr kb = (lds_ptr)lds + buf * kStage + kg * BT * RS, vb = kb + kMat;
         f16v s[NB];
@@ -361,12 +365,14 @@ struct Chunk {
             for (int i = 0; i < 16; i++) s[b][i] = 0.f;
         const uint32_t ka = (uint32_t)(l31 * RS) + (uint32_t)((h ^ k_turn(l31)) * 16);
 #pragma unroll
-        for (int k = 0; k < NK; k++)
+        for (int k = 0; k < NK; k++) {
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const u4 x = *reinterpret_cast<const __attribute__((address_space(3))) u4*>(kb + (ka ^ (k * 32)) + b * 32 * RS);
                 s[b] = mfma<T>(x, q[k], s[b]);
             }
+            if (kFence > 0 && k % kFence == kFence - 1) __builtin_amdgcn_sched_barrier(0);
+        }
         if (a.softcap > 0.f) {
 #pragma unroll
             for (int b = 0; b < NB; b++)
@@ -375,15 +381,25 @@ struct Chunk {
         }
         const float c = a.softcap > 0.f ? 1.f : p.c;
         if (masked) {
-            const uint64_t there = holes ? pages_there(t, r, tb) : ~0ull;
+            const int from = lo - tb - 4 * h;  // against the token's number without the lane's 4 h
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int x = 32 * b + (i & 3) + 8 * (i >> 2) + 4 * h;
-                    const bool on = (uint32_t)(tb + x - lo) < (uint32_t)len && ((there >> x) & 1);
-                    s[b][i] = on ? s[b][i] : -INFINITY;
+                    s[b][i] = (uint32_t)(32 * b + (i & 3) + 8 * (i >> 2) - from) < (uint32_t)len ? s[b][i] : -INFINITY;
+                    if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
+            if (holes) {
+                const uint64_t there = pages_there(a, t, r, tb) >> (4 * h);
+                uint32_t bits[2] = {(uint32_t)there, (uint32_t)(there >> 32)};
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        s[b][i] = (bits[b] >> ((i & 3) + 8 * (i >> 2))) & 1 ? s[b][i] : -INFINITY;
+                        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
         }
         float mx = kLowest;
 #pragma unroll
@@ -415,13 +431,15 @@ struct Chunk {
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int i = 0; i < 16; i++)
+                for (int i = 0; i < 16; i++) {
+                    if (kFence > 0 && i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int d = 0; d < ND; d++) {
                         const float x = *reinterpret_cast<const __attribute__((address_space(3))) float*>(
                             vb + (va ^ (d * 128)) + (32 * b + (i & 3) + 8 * (i >> 2)) * RS);
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[b][i], o[d], 0, 0, 0);
                     }
+                }
         } else {
             // One value of the type per weight: off by half a step of it each, in
             // either direction, as the result itself is once
@@ -430,6 +448,7 @@ struct Chunk {
                                 (uint32_t)((((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_turn(4 * h + i4)) * 16) + (lane & 1) * 8);
 #pragma unroll
             for (int kb16 = 0; kb16 < 2 * NB; kb16++) {
+                if (kFence > 0) __builtin_amdgcn_sched_barrier(0);
                 u4 x;
 #pragma unroll
                 for (int j = 0; j < 4; j++) x[j] = pack2<T>(s[kb16 / 2][8 * (kb16 & 1) + 2 * j], s[kb16 / 2][8 * (kb16 & 1) + 2 * j + 1]);
@@ -446,10 +465,10 @@ struct Chunk {
     }
 
     // the maximum by log2 e that goes with l and o
-    __device__ __forceinline__ float top_of(float mm) const { return fmaxf(mm * (a.softcap > 0.f ? 1.f : p.c), -0x1p126f); }
+    __device__ __forceinline__ static float top_of(const Params& p, float mm) { return fmaxf(mm * (p.a.softcap > 0.f ? 1.f : p.c), -0x1p126f); }
 
     // four channels of a row of the tile: into out, or a partial result
-    __device__ __forceinline__ void store4(const Tile& t, int hk, int qt, int to, int row, int d, f4 acc, float top, float sum) const {
+    __device__ __forceinline__ static void store4(const Params& p, const Tile& t, int hk, int qt, int to, int row, int d, f4 acc, float top, float sum) {
         if (to >= 0) {
             const int64_t at = (int64_t)to * (RG * 32) + row;
             *reinterpret_cast<f4*>(p.part_o + at * DP + d) = acc;
@@ -457,8 +476,8 @@ struct Chunk {
             return;
         }
         int head;
-        const int i = token_of(t, row, qt, head);
-        store_out(a, t.first + i, hk * a.G + head, d, acc, top, sum);
+        const int i = token_of(p, t, row, qt, head);
+        store_out(p.a, t.first + i, hk * p.a.G + head, d, acc, top, sum);
     }
     // no position counted: 0 and -infinity
     __device__ __forceinline__ static void store_out(const ChunkArgs& a, int tok, int head, int d, f4 acc, float top, float sum) {
@@ -553,7 +572,8 @@ struct Chunk {
 
     // stages u0 .. u1 - 1 of a tile; to: the slot of a partial result, or -1
     __device__ __forceinline__ void piece(const Tile& t, int r, int hk, int qt, int u0, int u1, int to, uint32_t* bad) {
-        const int h = lane >> 5, l31 = lane & 31;
+        const Params& p = argument();
+        const ChunkArgs& a = p.a;
         const int first_tok = t.base + u0 * ST, last_tok = t.base + u1 * ST < t.end ? t.base + u1 * ST : t.end;
         const bool any = last_tok > first_tok;
         // are there pages that are none
@@ -565,6 +585,19 @@ struct Chunk {
         }
         if (threadIdx.x < RG) bad[threadIdx.x] = 0;
         const bool holes = __syncthreads_or(none);
+        if (any) {
+#pragma unroll
+            for (int s = 0; s < NS - 1; s++)
+                if (u0 + s < u1) fill(a, t, r, hk, first_tok + s * ST, s);
+        }
+        load_q(p, t, hk, qt);
+        // what the compiler knows to be in flight ends here, not at its first use in the loop
+        __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));
+        // the wave's rows: the first one's tokens and the last one's
+        int head, lo0, hi0, lo1, hi1;
+        sees(a, t, token_of(p, t, rg * 32, qt, head), lo0, hi0);
+        sees(a, t, token_of(p, t, rg * 32 + 31, qt, head), lo1, hi1);
+        const bool rows = rg * 32 < t.m * p.GT;
         m = kLowest;
         l = 0.f;
 #pragma unroll
@@ -572,32 +605,20 @@ struct Chunk {
 #pragma unroll
             for (int i = 0; i < 16; i++) o[d][i] = 0.f;
         if (any) {
-#pragma unroll
-            for (int s = 0; s < NS - 1; s++)
-                if (u0 + s < u1) fill(t, r, hk, first_tok + s * ST, s);
-        }
-        load_q(t, hk, qt);
-        // what the compiler knows to be in flight ends here, not at its first use in the loop
-        __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));
-        // the wave's rows: the first one's tokens and the last one's
-        int head, lo0, hi0, lo1, hi1;
-        sees(t, token_of(t, rg * 32, qt, head), lo0, hi0);
-        sees(t, token_of(t, rg * 32 + 31, qt, head), lo1, hi1);
-        const bool rows = rg * 32 < t.m * p.GT;
-        if (any) {
             int buf = 0;
             for (int u = u0; u < u1; u++) {
                 if (NS > 2 && u1 - 1 - u >= NS - 2) wait_vm<WHOLE ? (NS - 2) * 2 * NI : 0>();
                 else wait_vm<0>();
                 barrier();
                 const int ahead = u + NS - 1;
-                if (ahead < u1) fill(t, r, hk, t.base + ahead * ST, buf == 0 ? NS - 1 : buf - 1);
+                if (ahead < u1) fill(a, t, r, hk, t.base + ahead * ST, buf == 0 ? NS - 1 : buf - 1);
                 const int tb = t.base + u * ST + kg * BT;
-                if (rows && tb < hi1 && tb + BT > lo0) take(t, r, tb, buf, holes || tb < lo1 || tb + BT > hi0, holes);
+                if (rows && tb < hi1 && tb + BT > lo0) take(p, t, r, tb, buf, holes || tb < lo1 || tb + BT > hi0, holes);
                 buf = buf == NS - 1 ? 0 : buf + 1;
             }
         }
         l += other_half(l);
+        const int h = afresh(lane >> 5), l31 = afresh(lane & 31);
         // 0 where all sums are finite, else NaN
         float z = 0.f;
 #pragma unroll
@@ -608,15 +629,16 @@ struct Chunk {
         const uint32_t mine = (uint32_t)__ballot(z != z && fabsf(l) < INFINITY);
         if (lane == 0 && rows && mine) atomicOr(&bad[rg], mine);
         __syncthreads();
+        const Params& e = argument();
         if constexpr (KG == 1) {
             const int row = rg * 32 + l31;
-            if (has_row(t, row, qt) && !((bad[rg] >> l31) & 1)) {
-                const float top = top_of(m);
+            if (has_row(e, t, row, qt) && !((bad[rg] >> l31) & 1)) {
+                const float top = top_of(e, m);
 #pragma unroll
                 for (int d = 0; d < ND; d++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        store4(t, hk, qt, to, row, 32 * d + 8 * i + 4 * h, f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}, top, l);
+                        store4(e, t, hk, qt, to, row, 32 * d + 8 * i + 4 * h, f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}, top, l);
             }
         } else {
             float* sums = reinterpret_cast<float*>(lds);
@@ -628,14 +650,14 @@ struct Chunk {
                 for (int i = 0; i < 4; i++)
                     *reinterpret_cast<f4*>(mine_o + 32 * d + 8 * i + 4 * h) = f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
             if (h == 0) {
-                ml[(w * 32 + l31) * 2] = top_of(m);
+                ml[(w * 32 + l31) * 2] = top_of(e, m);
                 ml[(w * 32 + l31) * 2 + 1] = l;
             }
             __syncthreads();
             constexpr int per = DP / 4;
             for (int x = threadIdx.x; x < RG * 32 * per; x += NT) {
                 const int row = x / per, d = (x - row * per) * 4;
-                if (!has_row(t, row, qt) || ((bad[row >> 5] >> (row & 31)) & 1)) continue;
+                if (!has_row(e, t, row, qt) || ((bad[row >> 5] >> (row & 31)) & 1)) continue;
                 float top = -0x1p126f;
 #pragma unroll
                 for (int g = 0; g < KG; g++) top = fmaxf(top, ml[(g * RG * 32 + row) * 2]);
@@ -647,10 +669,10 @@ struct Chunk {
                     sum += ml[(g * RG * 32 + row) * 2 + 1] * f;
                     acc += *reinterpret_cast<const f4*>(sums + (g * RG * 32 + row) * LS + d) * f;
                 }
-                store4(t, hk, qt, to, row, d, acc, top, sum);
+                store4(e, t, hk, qt, to, row, d, acc, top, sum);
             }
         }
-        if (KG > 1 && a.D < RS / ES) {  // the meeting was where no transfer fills
+        if (KG > 1 && e.a.D < RS / ES) {  // the meeting was where no transfer fills
             __syncthreads();
             clear();
         }
@@ -659,11 +681,11 @@ struct Chunk {
             for (int k = 0; rows_left; k++) {
                 const int row = g * 32 + __builtin_ctz(rows_left);
                 rows_left &= rows_left - 1;
-                if (k % NW != w || !has_row(t, row, qt)) continue;
+                if (k % NW != w || !has_row(e, t, row, qt)) continue;
                 int hd;
-                const int i = token_of(t, row, qt, hd);
+                const int i = token_of(e, t, row, qt, hd);
                 const int64_t at = (int64_t)to * (RG * 32) + row;
-                alone(p, t.first, t.pos, t.n, r, hk, hd, i, first_tok, last_tok, to >= 0 ? p.part_o + at * DP : nullptr, p.part_ml + at * 2);
+                alone(e, t.first, t.pos, t.n, r, hk, hd, i, first_tok, last_tok, to >= 0 ? e.part_o + at * DP : nullptr, e.part_ml + at * 2);
             }
         }
     }
@@ -681,7 +703,7 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void chunk_kernel(Params
     const int tid = threadIdx.x, lane = tid & 63;
     // an XCD takes every eighth block
     const int me = p.P % 8 == 0 ? (int)(blockIdx.x & 7) * (p.P / 8) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
-    A x(p, chunk_lds);
+    A x(chunk_lds);
     if (a.D < A::RS / A::ES) x.clear();  // chunks that no transfer fills
     // stages of the thread's places, and of all of them for one head
     const int s0 = tid * p.each, s1 = s0 + p.each < p.slots ? s0 + p.each : p.slots;
