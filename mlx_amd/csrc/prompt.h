@@ -76,8 +76,7 @@ struct LogprobArgs {
     int64_t row;
     char* ws;
     size_t ws_bytes;
-    uint32_t* count;
-    int counts, cus;
+    int cus;
 };
 LuxStatus launch_token_logprobs(const LogprobArgs& a, hipStream_t st);
 

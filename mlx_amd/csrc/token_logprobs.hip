@@ -1,0 +1,437 @@
+// token_logprobs.hip -- log probabilities of given tokens, entropy and the top
+// alternatives of rows of logits, in one pass over them.
+//
+// With y = (x - r) c, c = scale log2 e and r near the row's maximum M:
+//   S = sum exp2(y), E = sum exp2(y) y, moved from r to M at the end
+//   lse = scale M + ln 2 log2 S,  H = ln 2 (log2 S - E / S)
+// A thread keeps its own r, S and E and its largest logit.  Of 64 groups of threads
+// the k-th largest maximum is at most the row's k-th largest logit, so that the top
+// k lie in the few threads with a maximum from there on (24 logits on average for k
+// = 20): these are read again, out of the cache, and ranked by counting.
+//
+// Few rows are cut into parts, a block each, which a second launch joins.
+//
+// Rows in which that goes wrong (more logits from the bound on than are ranked, as
+// where most are -infinity, or NaN) are finished by a search, one largest logit
+// after the other.
+#include "prompt.h"
+#include "serving_device.h"
+
+namespace lxq {
+namespace {
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4h __attribute__((ext_vector_type(4), aligned(2)));
+
+constexpr int NT = 512, NW = NT / 64;
+constexpr int kGroups = 64;     // groups of threads
+constexpr int kRoom = 1024;     // logits that are ranked
+constexpr int kMostParts = 64;
+// r c up to which (x - r) c is taken as x c - r c: the rounding of r c is at most 4
+constexpr float kFar = 0x1p27f;
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
+
+// order of logits: NaN above all, -0 as 0; 0 stands for no logit
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t b = __float_as_uint(x + 0.f);
+    return x != x ? ~0u : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+    return k == ~0u ? __uint_as_float(0x7fc00000u) : __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+// the larger logit first, then the lower place
+__device__ __forceinline__ uint64_t entry_of(uint32_t key, int at) { return (uint64_t)key << 32 | (uint32_t)~at; }
+__device__ __forceinline__ int place_of(uint64_t e) { return (int)~(uint32_t)e; }
+
+// sums of a part of a row, about its largest logit `top` (-infinity: none)
+struct Sums {
+    float top, s, e;  // NaN where there is one; s and e mean nothing where it is not finite
+};
+
+// s and e about r (in units of c) to those about another one
+__device__ __forceinline__ void move(float& s, float& e, float by) {  // by = (r - new r) c
+    by = fmaxf(by, -1e4f);  // where 2^by is 0, its product with e is, too
+    const float f = __builtin_amdgcn_exp2f(by);
+    e = f * fmaf(s, by, e);
+    s *= f;
+}
+
+struct Params {
+    LogprobArgs a;
+    int parts, len;  // of a row, logits of a part (a multiple of 8)
+    float c;
+    Sums* sums;      // [rows, parts]
+    uint64_t* tops;  // [rows, parts, top]
+};
+
+template <int T>
+__device__ __forceinline__ float logit(const void* row, int i) {
+    if constexpr (T == DT_F32) return static_cast<const float*>(row)[i];
+    const uint32_t h = static_cast<const uint16_t*>(row)[i];
+    return T == DT_F16 ? f16_to_f32(h) : bf16_to_f32(h);
+}
+template <int T>
+__device__ __forceinline__ void unpack(const u4& v, float* x) {
+    if constexpr (T == DT_F32) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = __uint_as_float(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[2 * j] = T == DT_F16 ? f16_to_f32(v[j] & 0xffffu) : __uint_as_float(v[j] << 16);
+            x[2 * j + 1] = T == DT_F16 ? f16_to_f32(v[j] >> 16) : __uint_as_float(v[j] & 0xffff0000u);
+        }
+    }
+}
+
+__device__ __forceinline__ uint64_t wave_most(uint64_t v) {
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) {
+        const uint64_t o = __shfl_xor(v, k);
+        v = v > o ? v : o;
+    }
+    return v;
+}
+
+struct Shared {
+    uint64_t list[kRoom];
+    uint64_t most[NW];
+    uint32_t groups[kGroups];
+    float part[NW][3];
+    int count, odd;
+};
+
+// the row's scores, from its sums and its top entries
+__device__ __forceinline__ void write_sums(const LogprobArgs& a, int r, const Sums& t, float x_tok, bool has_tok, float& log_sum) {
+    // NaN in the row, +infinity, nothing but -infinity, or as it should be
+    const bool nan = t.top != t.top, none = t.top == -INFINITY, high = t.top == INFINITY;
+    log_sum = nan ? t.top : none || high ? 0.f : log2f(t.s) * kLn2;
+    const float lse = fmaf(a.scale, t.top, log_sum);
+    if (a.lse) a.lse[r] = lse;
+    if (a.entropy) a.entropy[r] = none ? 0.f : high || nan ? __uint_as_float(0x7fc00000u) : fmaf(-kLn2, t.e / t.s, log_sum);
+    if (a.logprobs) a.logprobs[r] = none || !has_tok ? (nan ? t.top : -INFINITY) : high || nan ? fmaf(a.scale, x_tok, -lse) : (x_tok - t.top) * a.scale - log_sum;
+}
+__device__ __forceinline__ float top_logprob(const LogprobArgs& a, const Sums& t, float x, float log_sum) {
+    if (t.top == -INFINITY) return -INFINITY;
+    if (t.top != t.top || t.top == INFINITY) return a.scale * x - a.scale * t.top;
+    return (x - t.top) * a.scale - log_sum;
+}
+
+// one block: part blockIdx of row; SPLIT: its results go to the workspace
+template <int T, bool SPLIT>
+__global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
+    constexpr int E = T == DT_F32 ? 4 : 8;
+    __shared__ Shared sh;
+    const LogprobArgs& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int block = first + (int)blockIdx.x, r = SPLIT ? block / p.parts : block, part = SPLIT ? block - r * p.parts : 0;
+    const int from = part * p.len, to = SPLIT && from + p.len < a.V ? from + p.len : a.V, n = to > from ? to - from : 0;
+    const char* base = static_cast<const char*>(a.logits) + ((int64_t)r * a.row + from) * (T == DT_F32 ? 4 : 2);
+    const int vectors = n >= NT * E ? n / E : 0;  // fewer logits: one by one, so that all threads have some
+    const bool want = !SPLIT && a.tokens && a.logprobs;
+    const int token = want ? a.tokens[r] : -1;
+    const bool has = (uint32_t)token < (uint32_t)a.V;
+    const float x_tok = has ? logit<T>(base, token) : 0.f;
+    if (tid == 0) sh.count = sh.odd = 0;
+
+    // the thread's vectors tid, tid + NT, ..., and logits behind the vectors likewise
+    float top = -INFINITY, ref = 0.f, s = 0.f, e = 0.f;  // ref: r c, as the loop subtracts it
+    bool fresh = true;
+    auto take = [&](const float* x, int m) {
+        float mx = x[0];
+#pragma unroll
+        for (int j = 1; j < m; j++) mx = fmaxf(mx, x[j]);
+        top = fmaxf(top, mx);
+        // a new r only where exp2 could pass 2^60
+        if (__any(fresh || fmaf(mx, p.c, -ref) > 60.f)) {
+            const float to = mx * p.c;
+            if ((fresh || to - ref > 60.f) && fabsf(to) < kFar) {
+                if (!fresh) move(s, e, ref - to);
+                ref = to;
+                fresh = false;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < m; j++) {
+            const float y = fmaf(x[j], p.c, -ref), q = __builtin_amdgcn_exp2f(y);
+            s += q;
+            e = fmaf(q, fmaxf(y, -1000.f), e);  // not 0 times -infinity
+        }
+    };
+    constexpr int kU = 4;
+    int v = tid;
+    for (; v + (kU - 1) * NT < vectors; v += kU * NT) {
+        u4 d[kU];
+#pragma unroll
+        for (int k = 0; k < kU; k++) d[k] = *reinterpret_cast<const u4h*>(base + (int64_t)(v + k * NT) * 16);
+#pragma unroll
+        for (int k = 0; k < kU; k++) {
+            float x[E];
+            unpack<T>(d[k], x);
+            take(x, E);
+        }
+    }
+    for (; v < vectors; v += NT) {
+        float x[E];
+        unpack<T>(*reinterpret_cast<const u4h*>(base + (int64_t)v * 16), x);
+        take(x, E);
+    }
+    const int behind = vectors * E;
+    for (int i = behind + tid; i < n; i += NT) {
+        float x[1] = {logit<T>(base, i)};
+        take(x, 1);
+    }
+
+    // the block's sums, about its largest logit
+    const bool odd = !(s < INFINITY);
+    float wtop = top;
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) wtop = fmaxf(wtop, __shfl_xor(wtop, k));
+    // groups of 8 threads
+    float gtop = top;
+#pragma unroll
+    for (int k = 1; k < 8; k *= 2) gtop = fmaxf(gtop, __shfl_xor(gtop, k));
+    const bool any = tid < vectors || behind + tid < n;
+    uint32_t gkey = any ? key_of(gtop) : 0u;
+#pragma unroll
+    for (int k = 1; k < 8; k *= 2) {
+        const uint32_t o = (uint32_t)__shfl_xor((int)gkey, k);
+        gkey = gkey > o ? gkey : o;
+    }
+    if ((lane & 7) == 0) sh.groups[tid >> 3] = gkey;
+    if (lane == 0) sh.part[w][0] = wtop;
+    __syncthreads();
+    if (odd) sh.odd = 1;
+    float all = sh.part[0][0];
+#pragma unroll
+    for (int i = 1; i < NW; i++) all = fmaxf(all, sh.part[i][0]);
+    if (fresh || all == -INFINITY) s = e = 0.f;
+    else move(s, e, fmaf(-all, p.c, ref));
+    s = wave_sum(s);
+    e = wave_sum(e);
+    if (lane == 0) {
+        sh.part[w][1] = s;
+        sh.part[w][2] = e;
+    }
+    // the bound: the k-th largest of the groups' maxima, each wave for itself
+    uint32_t bound = 0;
+    if (a.top > 0) {
+        const uint32_t mine = sh.groups[lane];
+        int rank = 0;
+#pragma unroll
+        for (int i = 0; i < kGroups; i++) {
+            const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
+            rank += o > mine || (o == mine && i < lane);
+        }
+        bound = (uint32_t)__builtin_amdgcn_readlane((int)mine, __builtin_ctzll(__ballot(rank == a.top - 1)));
+    }
+    __syncthreads();
+    Sums t = {all, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+        t.s += sh.part[i][1];
+        t.e += sh.part[i][2];
+    }
+    // NaN, infinite and far logits, and rows of nothing else than far ones below 0:
+    // the sums once more
+    bool nan = false;
+    if (sh.odd || (all > -INFINITY && all * p.c <= -kFar)) {
+        s = e = 0.f;
+        for (int i = tid; i < n; i += NT) {
+            const float x = logit<T>(base, i), y = fmaxf((x - all) * p.c, -1000.f), q = __builtin_amdgcn_exp2f(y);
+            nan |= x != x;
+            s += q;
+            e = fmaf(q, y, e);
+        }
+        nan = __syncthreads_or(nan);
+        s = wave_sum(s);
+        e = wave_sum(e);
+        if (lane == 0) {
+            sh.part[w][1] = s;
+            sh.part[w][2] = e;
+        }
+        __syncthreads();
+        t.s = t.e = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            t.s += sh.part[i][1];
+            t.e += sh.part[i][2];
+        }
+        if (nan) t.top = __uint_as_float(0x7fc00000u);
+    }
+
+    int found = 0;
+    if (a.top > 0 && !nan) {
+        // logits from the bound on
+        uint64_t flagged = __ballot(any && key_of(top) >= bound);
+        while (flagged) {
+            const int t0 = __builtin_ctzll(flagged), who = (w << 6) + t0;
+            flagged &= flagged - 1;
+            for (int i = who + lane * NT; i < vectors; i += 64 * NT) {
+                float x[E];
+                unpack<T>(*reinterpret_cast<const u4h*>(base + (int64_t)i * 16), x);
+#pragma unroll
+                for (int j = 0; j < E; j++) {
+                    const uint32_t k = key_of(x[j]);
+                    if (k >= bound) {
+                        const int at = atomicAdd(&sh.count, 1);
+                        if (at < kRoom) sh.list[at] = entry_of(k, from + i * E + j);
+                    }
+                }
+            }
+            for (int i = behind + who + lane * NT; i < n; i += 64 * NT) {
+                const uint32_t k = key_of(logit<T>(base, i));
+                if (k >= bound) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < kRoom) sh.list[at] = entry_of(k, from + i);
+                }
+            }
+        }
+        __syncthreads();
+        found = sh.count;
+    }
+    float log_sum = 0.f;
+    if (!SPLIT) {
+        if (tid == 0) write_sums(a, r, t, x_tok, has && want, log_sum);
+        else log_sum = t.top == -INFINITY || t.top == INFINITY ? 0.f : log2f(t.s) * kLn2;
+    } else if (tid == 0) {
+        p.sums[(int64_t)r * p.parts + part] = t;
+    }
+    auto put = [&](int rank, uint64_t entry) {
+        if (SPLIT) {
+            p.tops[((int64_t)r * p.parts + part) * a.top + rank] = entry;
+        } else {
+            if (a.top_ids) a.top_ids[(int64_t)r * a.top + rank] = place_of(entry);
+            if (a.top_lp) a.top_lp[(int64_t)r * a.top + rank] = top_logprob(a, t, value_of((uint32_t)(entry >> 32)), log_sum);
+        }
+    };
+    if (a.top == 0) return;
+    if (!nan && found <= kRoom) {
+        for (int i = tid; i < found; i += NT) {
+            const uint64_t mine = sh.list[i];
+            int rank = 0;
+            for (int j = 0; j < found; j++) rank += sh.list[j] > mine;
+            if (rank < a.top) put(rank, mine);
+        }
+        // a part with fewer logits than that
+        if (SPLIT && tid >= found && tid < a.top) put(tid, 0);
+        return;
+    }
+    // one after the other: the largest entry below the last one
+    uint64_t last = ~0ull;
+    for (int k = 0; k < a.top; k++) {
+        uint64_t best = 0;
+        for (int i = tid; i < n; i += NT) {
+            const uint64_t x = entry_of(key_of(logit<T>(base, i)), from + i);
+            if (x < last && x > best) best = x;
+        }
+        best = wave_most(best);
+        if (lane == 0) sh.most[w] = best;
+        __syncthreads();
+        last = sh.most[0];
+#pragma unroll
+        for (int i = 1; i < NW; i++) last = sh.most[i] > last ? sh.most[i] : last;
+        if (tid == 0) put(k, last);
+        __syncthreads();
+    }
+}
+
+// a block per row: its parts' sums and entries
+template <int T>
+__global__ __launch_bounds__(NT) void logprobs_join_kernel(Params p, int first) {
+    __shared__ uint64_t list[kRoom];
+    __shared__ int count;
+    const LogprobArgs& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 63, r = first + (int)blockIdx.x;
+    const int token = a.tokens && a.logprobs ? a.tokens[r] : -1;
+    const bool has = (uint32_t)token < (uint32_t)a.V;
+    const float x_tok = has ? logit<T>(static_cast<const char*>(a.logits) + (int64_t)r * a.row * (T == DT_F32 ? 4 : 2), token) : 0.f;
+    const uint64_t* tops = p.tops + (int64_t)r * p.parts * a.top;
+    if (tid == 0) count = 0;
+    // each wave for itself
+    const Sums mine = lane < p.parts ? p.sums[(int64_t)r * p.parts + lane] : Sums{-INFINITY, 0.f, 0.f};
+    uint32_t k = lane < p.parts ? key_of(mine.top) : 0u;
+    uint32_t most = k;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+        const uint32_t o = (uint32_t)__shfl_xor((int)most, i);
+        most = most > o ? most : o;
+    }
+    Sums t = {value_of(most), 0.f, 0.f};
+    float s = mine.s, e = mine.e;
+    if (!(fabsf(mine.top) < INFINITY) || !(fabsf(t.top) < INFINITY)) s = e = 0.f;
+    else move(s, e, (mine.top - t.top) * p.c);
+    t.s = wave_sum(s);
+    t.e = wave_sum(e);
+    float log_sum;
+    if (tid == 0) write_sums(a, r, t, x_tok, has, log_sum);
+    else log_sum = t.top == -INFINITY || t.top == INFINITY ? 0.f : log2f(t.s) * kLn2;
+    if (a.top == 0) return;
+    // a bound: each part's entries down to the k-th over the parts, rounded up, are
+    // at least k
+    const int down = (a.top + p.parts - 1) / p.parts - 1;
+    uint64_t low = lane < p.parts ? tops[lane * a.top + down] : ~0ull;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+        const uint64_t o = __shfl_xor(low, i);
+        low = low < o ? low : o;
+    }
+    __syncthreads();
+    for (int i = tid; i < p.parts * a.top; i += NT) {
+        const uint64_t x = tops[i];
+        if (x >= low && x != 0) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kRoom) list[at] = x;
+        }
+    }
+    __syncthreads();
+    const int found = count;
+    const uint64_t* from = found <= kRoom ? list : tops;
+    const int n = found <= kRoom ? found : p.parts * a.top;
+    for (int i = tid; i < n; i += NT) {
+        const uint64_t x = from[i];
+        int rank = 0;
+        for (int j = 0; j < n; j++) rank += from[j] > x;
+        if (rank < a.top && x != 0) {
+            if (a.top_ids) a.top_ids[(int64_t)r * a.top + rank] = place_of(x);
+            if (a.top_lp) a.top_lp[(int64_t)r * a.top + rank] = top_logprob(a, t, value_of((uint32_t)(x >> 32)), log_sum);
+        }
+    }
+}
+
+template <int T>
+LuxStatus launch_t(const LogprobArgs& a, hipStream_t st) {
+    Params p = {};
+    p.a = a;
+    p.c = a.scale * kLog2e;
+    // two blocks per CU; parts of at least 4096 logits
+    int parts = a.T > 0 ? 2 * a.cus / a.T : 1;
+    if (parts > a.V / 4096) parts = a.V / 4096;
+    if (parts > kMostParts) parts = kMostParts;
+    const size_t one = sizeof(Sums) + (size_t)a.top * 8;
+    if (parts > 1 && (!a.ws || (size_t)a.T * parts * one > a.ws_bytes)) parts = 1;
+    if (parts <= 1) {
+        p.parts = 1;
+        p.len = a.V;
+        launch_blocks(a.T, NT, [&](int first, unsigned n) {
+            hipLaunchKernelGGL((logprobs_kernel<T, false>), dim3(n), dim3(NT), 0, st, p, first);
+        });
+    } else {
+        p.len = ((a.V + parts - 1) / parts + 7) & ~7;
+        p.parts = (a.V + p.len - 1) / p.len;
+        p.tops = reinterpret_cast<uint64_t*>(a.ws);
+        p.sums = reinterpret_cast<Sums*>(a.ws + (size_t)a.T * p.parts * a.top * 8);
+        hipLaunchKernelGGL((logprobs_kernel<T, true>), dim3(a.T * p.parts), dim3(NT), 0, st, p, 0);
+        hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3(a.T), dim3(NT), 0, st, p, 0);
+    }
+    return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
+}
+
+}  // namespace
+
+LuxStatus launch_token_logprobs(const LogprobArgs& a, hipStream_t st) {
+    if (a.dtype == DT_F32) return launch_t<DT_F32>(a, st);
+    return a.dtype == DT_F16 ? launch_t<DT_F16>(a, st) : launch_t<DT_BF16>(a, st);
+}
+
+}  // namespace lxq

@@ -131,3 +131,148 @@ def run_chunk(ctx, dtype, q, kc, vc, table, starts, seq, lens, H, /, window=0, s
             return None
         assert rc == 0, rc
         return get(), get_lse()
+
+
+# --- pages in use -------------------------------------------------------------------------
+
+
+def cut(n, cols, page):
+    return min(max(int(n), 0), cols * page)
+
+
+def up(n, page):
+    return -(-n // page)
+
+
+def ints(v, *shape):
+    t = torch.tensor(v, dtype=torch.int32)
+    return t.reshape(*shape) if shape else t
+
+
+def fork_reference(src, dst, lens, table, shares, free, head, page):
+    src, dst, lens, shares, free = (list(map(int, x)) for x in (src, dst, lens, shares, free))
+    table = [list(map(int, row)) for row in table]
+    R, cols, pool, F = len(lens), len(table[0]), len(shares), len(free)
+    before, made = list(lens), set()
+    head = at = min(max(int(head), 0), F)
+    copy_src, copy_dst, taken, shared, missing, out = [], [], 0, 0, 0, 0
+    for s, d in zip(src, dst):
+        copy_src.append(-1)
+        copy_dst.append(-1)
+        if not (0 <= s < R and 0 <= d < R and s != d and before[d] <= 0) or d in made:
+            out += 1
+            continue
+        made.add(d)
+        n = cut(before[s], cols, page)
+        full = n // page
+        for c in range(full):
+            table[d][c] = table[s][c]
+            if 0 <= table[s][c] < pool:
+                shares[table[s][c]] += 1
+        shared += full
+        if n % page:
+            last = table[s][full]
+            table[d][full] = last
+            if 0 <= last < pool:
+                if at < F:
+                    table[d][full], copy_src[-1], copy_dst[-1] = free[at], last, free[at]
+                    taken += 1
+                else:
+                    table[d][full], n = -1, full * page
+                    missing += 1
+                at += 1
+        lens[d] = n
+    return {"lens": ints(lens), "block_table": ints(table), "shares": ints(shares), "copy_src": ints(copy_src), "copy_dst": ints(copy_dst),
+            "counts": ints([head + taken, shared, missing, out])}
+
+
+def release_reference(lens, keep, table, shares, free, head, page):
+    shares, free = list(map(int, shares)), list(map(int, free))
+    pool, cols = len(shares), table.shape[1]
+    head = min(max(int(head), 0), len(free))
+    kv, back, entries = [], set(), 0
+    for r in range(len(lens)):
+        n = cut(lens[r], cols, page)
+        kept = min(n, max(0, int(keep[r])))
+        kv.append(kept)
+        for c in range(up(kept, page), up(n, page)):
+            p = int(table[r, c])
+            if 0 <= p < pool:
+                entries += 1
+                if shares[p] == 0:
+                    back.add(p)
+                else:
+                    shares[p] -= 1
+    back = sorted(back)
+    lost = max(0, len(back) - head)
+    free[head - (len(back) - lost):head] = back[lost:]
+    return {"kv_lens": ints(kv), "shares": ints(shares), "free_pages": ints(free),
+            "counts": ints([max(0, head - len(back)), len(back), entries - len(back), lost])}
+
+
+def compact_reference(lens, table, shares, free, limit, max_moves, page):
+    pool, cols = len(shares), table.shape[1]
+    held = [up(cut(n, cols, page), page) for n in lens]
+    live = {int(table[r, c]) for r in range(len(lens)) for c in range(held[r]) if 0 <= int(table[r, c]) < pool}
+    high, room = sorted(p for p in live if p >= limit), [p for p in range(limit) if p not in live]
+    moves = min(len(high), len(room), max_moves)
+    name = dict(zip(high[:moves], room))
+    new_table, new_shares = table.clone(), list(map(int, shares))
+    for r in range(len(lens)):
+        for c in range(held[r]):
+            new_table[r, c] = name.get(int(table[r, c]), int(table[r, c]))
+    for a, b in name.items():
+        new_shares[b], new_shares[a] = int(shares[a]), 0
+    left, free = room[moves:], list(map(int, free))
+    first = max(0, len(free) - len(left))
+    free[first:] = left[len(left) - (len(free) - first):]
+    fill = lambda v: ints(v + [-1] * (max_moves - moves))  # noqa: E731
+    return {"table_out": new_table, "shares_out": ints(new_shares), "free_pages": ints(free), "copy_src": fill(high[:moves]),
+            "copy_dst": fill(room[:moves]), "counts": ints([first, moves, len(high) - moves, len(live)])}
+
+
+# --- log probabilities --------------------------------------------------------------------
+
+
+def logprobs_reference(logits, tokens, top, scale):
+    """Scores in 64 bits of rows without NaN and +infinity, and the absolute tolerance of each kind.  A row of
+    n logits: each exp is off by 2^-24 (4 + 2 y) of itself, y its distance to the largest one by log2 e (the
+    factor's rounding and that of y), its share of the sum at most 2^-y, so 8 2^-24 in all; a thread adds
+    n / 512 and then 70 of them one by one; log and the products round 4 times at the result's size.
+    The entropy's second sum weighs each error by y, at most log2 n + 1 on average."""
+    x = logits.double() * scale
+    T, V = x.shape
+    lse = torch.logsumexp(x, -1)
+    every = x - lse[:, None]
+    p = torch.exp(every)
+    p = torch.where(torch.isneginf(x), 0.0, p)
+    entropy = torch.where(torch.isneginf(lse), 0.0, -torch.where(p > 0, p * every, 0.0).sum(-1))
+    every = torch.where(torch.isneginf(lse)[:, None], -math.inf, every)
+    log_p = torch.tensor([float(every[t, i]) if 0 <= i < V else -math.inf for t, i in enumerate(map(int, tokens))], dtype=torch.float64)
+    # -0 is 0, ties go to the lowest place
+    order = torch.argsort(logits.double() + 0.0, dim=-1, descending=True, stable=True)[:, :top]
+    unit = 2.0 ** -24
+    base = unit * (12 + V / 512 + 70 + math.log2(V) * 4)
+    size = 4 * unit * (scale * logits.double()).masked_fill(torch.isinf(logits.double()), 0).abs().amax(-1)
+    return {"lse": lse, "logprobs": log_p, "entropy": entropy, "top_ids": order.to(torch.int32), "top_logprobs": every.gather(1, order)}, \
+        {"lse": base + size, "logprobs": base + size, "top_logprobs": (base + size)[:, None], "entropy": (base + size) * (math.log2(V) + 2)}
+
+
+def run_logprobs(ctx, dtype, logits, tokens, top, /, scale=1.0, offset=0, pad=0, expect=None, **over):
+    T, V = logits.shape
+    wide = torch.full((T * (V + pad) + offset,), math.nan, dtype=logits.dtype)
+    wide[offset:].view(T, V + pad)[:, :V] = logits
+    with Device(ctx) as d:
+        outs = {k: d.new(*s, dtype=t, fill=9) for k, s, t in [
+            ("logprobs", (T,), torch.float32), ("entropy", (T,), torch.float32), ("lse", (T,), torch.float32),
+            ("top_ids", (T, top), torch.int32), ("top_logprobs", (T, top), torch.float32)]}
+        a = abi.TokenLogprobsArgs(rows=T, vocab=V, top=top, dtype=dtype, scale=scale, logits_offset=offset, row_stride=V + pad,
+                                  logits=d.up(wide), tokens=d.up(tokens), **{k: v[0] for k, v in outs.items()})
+        for k, v in over.items():
+            setattr(a, k, v)
+        rc = ctx.p.op_token_logprobs(ctx.handle, a)
+        if expect is not None:
+            assert rc == expect, rc
+            return None
+        assert rc == 0, rc
+        return {k: v[1]() for k, v in outs.items()}
