@@ -26,6 +26,8 @@
 // launch joins.  Ranges follow each other head by head, and an XCD takes a run
 // of ranges, so that its L2 holds the keys that its blocks share.
 #pragma once
+#include <type_traits>
+
 #include "prompt.h"
 #include "serving_device.h"
 
@@ -44,10 +46,11 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 constexpr float kLowest = -0x1.fffffep127f;  // the maximum of no score: no finite score is below
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 constexpr float kLeast = 0x1p-126f;
+constexpr int kLeastPiece = 2;
 
-// a tile that starts in a range and ends behind it: its parts, where it is
+// a tile that starts in a range and ends behind it: its parts, tokens and heads
 struct Cut {
-    int32_t parts, r, tile, hq;
+    int32_t parts, first, m, hq;
 };
 
 struct Params {
@@ -56,7 +59,7 @@ struct Params {
     int TB;           // tokens of a tile
     int slots, each;  // places of tiles (some may be empty); places per thread
     DivBy by_tb, by_gt;
-    int P;
+    int P, log;       // ranges: 2^log
     float c;          // scores by log2 e are s * c (or, capped, cap tanh(y) with 2 y log2 e = s * c)
     float cap;        // softcap log2 e
     uint32_t flip;    // sign bits of q: c is not negative
@@ -91,6 +94,11 @@ struct Tile {
     int pos, n;      // position of the first one; tokens held
     int base, end;   // cached tokens that the tile sees lie in [base, end)
     int units;       // stages; a tile that sees nothing has one, which writes its zeros
+};
+// a tile, where it is, and a unit in it
+struct Found {
+    Tile t;
+    int r, tile, at;
 };
 template <int ST>
 __device__ __forceinline__ Tile tile_of(const Params& p, int r, int tile) {
@@ -131,16 +139,27 @@ __device__ __forceinline__ int request_of_token(const ChunkArgs& a, int t) {
     return lo;
 }
 
-// of `units` units, range w of P starts at first(w): the first units % P ranges
-// are one unit longer
+// The units of all tiles in 2^log equal ranges, none of them empty.  A piece of a tile costs as
+// much beyond its units as a few of them: a cut less than `least` units from a
+// tile's end is moved there.  Ranges are at least four times as long, so that
+// at most one cut moves to each end.
 struct Ranges {
-    uint64_t base, rem;
-    __device__ Ranges(uint64_t units, int P) : base(units / (uint32_t)P), rem(units - base * (uint32_t)P) {}
-    __device__ uint64_t first(int w) const { return (uint64_t)w * base + ((uint64_t)w < rem ? (uint64_t)w : rem); }
-    __device__ int of(uint64_t u) const {
-        const uint64_t long_ones = rem * (base + 1);
-        return (int)(u < long_ones ? u / (base + 1) : rem + (u - long_ones) / base);
+    uint64_t units;
+    int log, least;
+    __device__ Ranges(uint64_t n, int l) : units(n), log(l) {
+        while (n >> log == 0) log--;
+        const uint64_t quarter = n >> (log + 2);
+        least = quarter < kLeastPiece ? (int)quarter : kLeastPiece;
     }
+    __device__ uint64_t first(int w) const { return (units * (uint32_t)w) >> log; }
+    __device__ int of(uint64_t u) const {
+        int w = (int)((double)(u + 1) * (double)(1 << log) / (double)units);  // or one beside it
+        while (first(w) > u) w--;
+        while (first(w + 1) <= u) w++;
+        return w;
+    }
+    // where a cut `at` units into a tile of n goes
+    __device__ int cut(int at, int n) const { return at < least ? 0 : n - at < least ? n : at; }
 };
 
 // slot of the s-th part of a tile that starts in range w0: a range keeps the part
@@ -161,12 +180,15 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
-// global -> LDS: lane l copies 16 bytes to LDS m0 + 16 l
+// global -> LDS: lane l copies 16 bytes to LDS m0 + 16 l (a transfer reads m0 one
+// wait state after it was written at the earliest)
 __device__ __forceinline__ void dma16(uint32_t m0v, const void* sbase, uint32_t voff) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(m0v), "v"(voff), "s"(sbase) : "memory", "m0");
+    const uint64_t b = reinterpret_cast<uint64_t>(sbase);
+    const uint64_t s = (uint64_t)(uint32_t)uniform((int)(b >> 32)) << 32 | (uint32_t)uniform((int)b);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(uniform((int)m0v)), "v"(voff), "s"(s) : "memory", "m0");
 }
 __device__ __forceinline__ void dma16a(uint32_t m0v, const void* addr) {
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0v), "v"(addr) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(uniform((int)m0v)), "v"(addr) : "memory", "m0");
 }
 
 __device__ __forceinline__ float other_half(float v) {
@@ -211,32 +233,31 @@ typedef const __attribute__((address_space(3))) char* lds_ptr;
 
 // T: type of q, cache and out; DP: head_dim rounded up to 64, 128, 192 or 256; RG
 // row groups times KG groups of tokens = waves; BT: tokens of a group's part of a
-// stage; NS: stages in LDS; WHOLE: pages hold whole runs of the tokens that one
-// transfer takes, so that a run has one scalar address (else each lane finds its
-// token's)
-template <int T, int DP, int RG, int KG, int BT, int NS, bool WHOLE>
+// stage; NS: stages in LDS; EASY: head_dim is DP, a power of two, scores are not capped, and
+// pages hold whole runs of the tokens that a wave finds with one entry of the
+// table, so that a run has one scalar address (else each lane finds its token's)
+template <int T, int DP, int RG, int KG, int BT, int NS, bool EASY>
 struct Chunk {
     static constexpr int ES = T == DT_F32 ? 4 : 2, E = 16 / ES;  // bytes; elements per 16 bytes
     static constexpr int RS = (DP == 192 ? 256 : DP) * ES;       // LDS row of a token
     static constexpr int CPR = RS / 16, TI = 64 / CPR;           // its 16-byte chunks; tokens per transfer
     static constexpr int NW = RG * KG, NT = 64 * NW, ST = BT * KG, NI = ST / TI / NW;
     static_assert(NI * TI * NW == ST && TI <= 16, "every wave moves whole runs");
-    static constexpr int kMat = ST * RS, kStage = 2 * kMat;
+    // tokens that a wave finds with one entry of the table, and how often per stage
+    static constexpr int LT = TI * NI < 8 ? TI * NI : 8, NL = TI * NI / LT;
+    static constexpr int ROWS = RG * 32;
+    static constexpr int kMat = ST * RS, kRings = 2 * NS * kMat;  // LDS: NS slots of keys, then of values
     static constexpr int NK = DP / (2 * E), ND = DP / 32, NB = BT / 32;
     static constexpr int KM = CPR < 16 ? 7 : 15;
     static constexpr int LS = DP + 4;  // row of the groups' meeting, in floats
-    static constexpr int kMeet = KG > 1 ? NW * 32 * (LS + 2) * 4 : 0;
-    static constexpr int kLds = NS * kStage > kMeet ? NS * kStage : kMeet;
+    static constexpr int kMeet = KG > 1 ? NW * 32 * (LS + 2) * 4 + ROWS * (KG + 2) * 4 : 0;
+    static constexpr int kLds = kRings > kMeet ? kRings : kMeet;
     // the weights are 2^kLift exp2(s - m): f16 ends at 2^-24, and many weights
     // below 2^-25 beside a large one may together be most of the result
     static constexpr float kLift = T == DT_F16 ? 14.f : 0.f, kDown = T == DT_F16 ? 0x1p-14f : 1.f;
     // m may stay behind the maximum by this much (log2): O is rescaled less often,
     // and weights stay below 2^16 in f16
     static constexpr float kBehind = T == DT_F16 ? 1.f : 8.f;
-
-    // where the registers are short, operands of so many steps ahead are loaded and
-    // no more (0: as the compiler likes)
-    static constexpr int kFence = T == DT_F32 && DP >= 128 ? 2 : DP == 256 || (DP == 128 && !WHOLE) ? 4 : 0;
 
     // permutations of a row's chunks
     __device__ __forceinline__ static int k_turn(int row) { return row & KM; }
@@ -253,6 +274,7 @@ struct Chunk {
     f16v o[ND];
     float m, l;
     int lo, len;  // the cached tokens that the lane's row sees
+    int found[NL], row_at[NL];  // see find()
 
     __device__ __forceinline__ explicit Chunk(char* mem) : lds(mem) {
         lane = threadIdx.x & 63;
@@ -264,45 +286,75 @@ struct Chunk {
         voff = (uint32_t)((c ^ v_turn(ri)) * 16);
     }
 
-    // a stage's transfers into LDS stage `buf`: tokens from tb on, those past the
-    // tile's last one from its row
-    __device__ __forceinline__ void fill(const ChunkArgs& a, const Tile& t, int r, int hk, int tb, int buf) {
-        const uint32_t dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + (uint32_t)(buf * kStage);
+    // The cache rows where the wave's parts of stages s0 + lane begin, tokens behind
+    // the tile's last one taken as its run: 64 stages with one trip to the table
+    __device__ __forceinline__ void find(const ChunkArgs& a, const Tile& t, int r, int hk, int first_tok, int s0) {
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int t0 = first_tok + (s0 + lane) * ST + w * NI * TI + i * LT;
+            const int tr = (uint32_t)t0 < (uint32_t)t.end ? t0 : (t.end - 1) & ~(LT - 1);
+            const int col = div_by(tr, a.div);
+            int pg = a.table[(int64_t)r * a.columns + col];
+            pg = (uint32_t)pg < (uint32_t)a.pool ? pg : 0;
+            found[i] = (pg * a.Hk + hk) * a.page + (tr - col * a.page);
+        }
+    }
+    // what the compiler knows to be in flight ends here, not at its first use in a loop
+    __device__ __forceinline__ static void settle() { __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8)); }
+    __device__ __forceinline__ uint32_t lds_at() const { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + (uint32_t)(w * NI * 1024); }
+    // A stage's rows of keys (V: of values) into the slot at `slot` of their ring:
+    // tokens from tb on, those past the tile's last one from its row
+    template <bool V>
+    __device__ __forceinline__ void fill(const ChunkArgs& a, const Tile& t, int r, int hk, int tb, uint32_t slot) {
+        const uint32_t dst = lds_at() + (V ? NS * kMat : 0) + slot;
         const uint32_t row_bytes = (uint32_t)(a.D * ES);
+        const char* cache = static_cast<const char*>(V ? a.vc : a.kc);
         const int ri = lane / CPR;
 #pragma unroll
         for (int j = 0; j < NI; j++) {
-            const int run = w * NI + j;
-            const uint32_t at_lds = dst + (uint32_t)(run * 1024);
-            const uint32_t kc = koff ^ (uint32_t)(k_turn(run * TI) * 16), vc = voff ^ (uint32_t)(v_turn(run * TI) * 16);
-            const int t0 = tb + run * TI;
-            if constexpr (WHOLE) {
-                const int tr = t0 < t.end ? t0 : (t.end - 1) & ~(TI - 1);
-                const int col = div_by(tr, a.div);
-                int pg = scalar_at(a.table, (int64_t)r * a.columns + col);
-                pg = (uint32_t)pg < (uint32_t)a.pool ? pg : 0;
-                const uint64_t row = (uint64_t)(uint32_t)((pg * a.Hk + hk) * a.page + (tr - col * a.page));
-                const char* kp = static_cast<const char*>(a.kc) + row * row_bytes;
-                const char* vp = static_cast<const char*>(a.vc) + row * row_bytes;
-                const int last = t.end - 1 - tr;  // rows behind the last one: the last one's
-                const uint32_t at_row = (uint32_t)(ri < last ? ri : last) * row_bytes;
-                if (a.D == RS / ES) {
-                    dma16(at_lds, kp, kc + at_row);
-                    dma16(at_lds + kMat, vp, vc + at_row);
-                } else {
-                    if (kc < row_bytes) dma16(at_lds, kp, kc + at_row);
-                    if (vc < row_bytes) dma16(at_lds + kMat, vp, vc + at_row);
+            const int run = w * NI + j, in = j * TI % LT;  // the run's first token, from where the entry was found
+            const uint32_t c = V ? voff ^ (uint32_t)(v_turn(run * TI) * 16) : koff ^ (uint32_t)(k_turn(run * TI) * 16);
+            if constexpr (EASY) {
+                const int i = j * TI / LT;
+                const char* from = cache + (uint64_t)(uint32_t)row_at[i] * row_bytes;
+                uint32_t at = c + (uint32_t)(ri + in) * row_bytes;
+                if (tb + ST > t.end) {
+                    const int t0 = tb + w * NI * TI + i * LT, tr = t0 < t.end ? t0 : (t.end - 1) & ~(LT - 1), last = t.end - 1 - tr;
+                    at = c + (uint32_t)(ri + in < last ? ri + in : last) * row_bytes;
                 }
+                dma16(dst + j * 1024, from, at);
             } else {
-                int tok = t0 + ri;
+                int tok = tb + run * TI + ri;
                 tok = tok < t.end ? tok : t.end - 1;
                 const int col = div_by(tok, a.div);
                 int pg = a.table[(int64_t)r * a.columns + col];
                 pg = (uint32_t)pg < (uint32_t)a.pool ? pg : 0;
                 const uint64_t row = (uint64_t)(uint32_t)((pg * a.Hk + hk) * a.page + (tok - col * a.page));
-                if (kc < row_bytes) dma16a(at_lds, static_cast<const char*>(a.kc) + row * row_bytes + kc);
-                if (vc < row_bytes) dma16a(at_lds + kMat, static_cast<const char*>(a.vc) + row * row_bytes + vc);
+                if (c < row_bytes) dma16a(dst + j * 1024, cache + row * row_bytes + c);
             }
+        }
+    }
+    // the same of a stage that is all there, in an EASY form
+    template <bool V>
+    __device__ __forceinline__ void fill_whole(const ChunkArgs& a, uint32_t slot) const {
+        const uint32_t dst = lds_at() + (V ? NS * kMat : 0) + slot;
+#pragma unroll
+        for (int j = 0; j < NI; j++) {
+            const uint32_t c = V ? voff ^ (uint32_t)(v_turn((w * NI + j) * TI) * 16) : koff ^ (uint32_t)(k_turn((w * NI + j) * TI) * 16);
+            const int i = j * TI / LT;
+            const char* from = static_cast<const char*>(V ? a.vc : a.kc) + (uint64_t)(uint32_t)row_at[i] * (uint32_t)(DP * ES);
+            dma16(dst + j * 1024, from, c + (uint32_t)(lane / CPR + j * TI % LT) * (uint32_t)(DP * ES));
+        }
+    }
+    // the rows of stage s
+    __device__ __forceinline__ void next_rows(const ChunkArgs& a, const Tile& t, int r, int hk, int first_tok, int s) {
+        if constexpr (EASY) {
+            if ((s & 63) == 0 && s > 0) {
+                find(a, t, r, hk, first_tok, s);
+                settle();
+            }
+#pragma unroll
+            for (int i = 0; i < NL; i++) row_at[i] = __builtin_amdgcn_readlane(found[i], s & 63);
         }
     }
 
@@ -353,59 +405,119 @@ struct Chunk {
         return __ballot((uint32_t)pg < (uint32_t)a.pool);
     }
 
-    // a group's BT tokens of a stage, from position tb on, into m, l and o
-    __device__ __forceinline__ void take(const Params& p, const Tile& t, int r, int tb, int buf, bool masked, bool holes) {
-        const ChunkArgs& a = p.a;
-        const int h = lane >> 5, l31 = lane & 31;
-        lds_ptr kb = (lds_ptr)lds + buf * kStage + kg * BT * RS, vb = kb + kMat;
+    struct Scores {
         f16v s[NB];
+    };
+    struct Weights {
+        u4 w[T == DT_F32 ? 1 : 2 * NB];
+    };
+
+    // Operands of the products that are on their way from LDS: those of AK steps of
+    // the first product (a step: 16 bytes of each key row) and AV of the second
+    // (a step: 16 tokens, 32 channels; f32: 2 tokens).  The steps are fenced: left to
+    // itself the compiler reads each operand right before its product and waits
+    static constexpr int AK = T == DT_F32 && DP >= 128 ? 1 : DP == 256 ? 2 : 3, AV = 4;
+    static constexpr int NVS = T == DT_F32 ? 16 * NB * ND : 2 * NB * ND;  // steps of the second product
+    struct Ahead {
+        u4 k[AK][NB];
+        u4 v[AV];
+    };
+    // offsets into the rings of the lane's part of a step
+    __device__ __forceinline__ uint32_t key_at(uint32_t slot) const {
+        return slot + (uint32_t)((kg * BT + (lane & 31)) * RS) + (uint32_t)(((lane >> 5) ^ k_turn(lane & 31)) * 16);
+    }
+    __device__ __forceinline__ uint32_t value_at(uint32_t slot) const {
+        const int h = lane >> 5, row = NS * ST + kg * BT + 4 * h;
+        if constexpr (T == DT_F32) {
+            return slot + (uint32_t)(row * RS) + (uint32_t)((((lane & 31) >> 2) ^ v_turn(4 * h)) * 16 + (lane & 3) * 4);
+        } else {
+            const int i4 = (lane & 15) >> 2;
+            return slot + (uint32_t)((row + i4) * RS) + (uint32_t)(((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_turn(4 * h + i4)) * 16 + (lane & 1) * 8);
+        }
+    }
+    __device__ __forceinline__ void read_k(u4* x, uint32_t at, int k) const {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+            x[b] = *reinterpret_cast<const __attribute__((address_space(3))) u4*>((lds_ptr)lds + (at ^ (uint32_t)(k * 32)) + b * 32 * RS);
+    }
+    __device__ __forceinline__ u4 read_v(uint32_t at, int s) const {
+        const int d = s % ND;
+        if constexpr (T == DT_F32) {
+            const int i = s / ND;  // token pair of all blocks
+            return u4{*reinterpret_cast<const __attribute__((address_space(3))) uint32_t*>(
+                          (lds_ptr)lds + (at ^ (uint32_t)(d * 128)) + (32 * (i / 16) + (i & 3) + 8 * (i % 16 >> 2)) * RS), 0, 0, 0};
+        } else {
+            typedef __attribute__((address_space(3))) s4* tr_ptr;
+            const lds_ptr from = (lds_ptr)lds + (at ^ (uint32_t)(d * 64)) + 16 * (s / ND) * RS;
+            const u2 x = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)from));
+            const u2 y = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(from + 8 * RS)));
+            return u4{x[0], x[1], y[0], y[1]};
+        }
+    }
+    __device__ __forceinline__ static void clear(Scores& x) {
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[b][i] = 0.f;
-        const uint32_t ka = (uint32_t)(l31 * RS) + (uint32_t)((h ^ k_turn(l31)) * 16);
+            for (int i = 0; i < 16; i++) x.s[b][i] = 0.f;
+    }
+    // the first steps' keys, to be read before other work
+    __device__ __forceinline__ void begin(Ahead& f, uint32_t at) const {
+#pragma unroll
+        for (int k = 0; k < AK; k++) read_k(f.k[k], at, k);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __device__ __forceinline__ void score(Scores& x, Ahead& f, uint32_t at, int k) const {
+#pragma unroll
+        for (int b = 0; b < NB; b++) x.s[b] = mfma<T>(f.k[k % AK][b], q[k], x.s[b]);
+        if (k + AK < NK) read_k(f.k[k % AK], at, k + AK);
+    }
+    __device__ __forceinline__ void scores(Scores& x, Ahead& f, uint32_t at) const {
+        clear(x);
 #pragma unroll
         for (int k = 0; k < NK; k++) {
+            score(x, f, at, k);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+
+    // the cap, and -infinity for tokens that the row does not see: those of a group's
+    // part of a stage, from position tb on
+    __device__ __forceinline__ void mask(const ChunkArgs& a, Scores& x, const Tile& t, int r, int tb, bool holes) const {
+        const int h = lane >> 5;
+        const int from = lo - tb - 4 * h;  // against the token's number without the lane's 4 h
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const u4 x = *reinterpret_cast<const __attribute__((address_space(3))) u4*>(kb + (ka ^ (k * 32)) + b * 32 * RS);
-                s[b] = mfma<T>(x, q[k], s[b]);
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                x.s[b][i] = (uint32_t)(32 * b + (i & 3) + 8 * (i >> 2) - from) < (uint32_t)len ? x.s[b][i] : -INFINITY;
+                if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
-            if (kFence > 0 && k % kFence == kFence - 1) __builtin_amdgcn_sched_barrier(0);
-        }
-        if (a.softcap > 0.f) {
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) s[b][i] = p.cap * tanh_of(s[b][i] * p.c);
-        }
-        const float c = a.softcap > 0.f ? 1.f : p.c;
-        if (masked) {
-            const int from = lo - tb - 4 * h;  // against the token's number without the lane's 4 h
+        if (holes) {
+            const uint64_t there = pages_there(a, t, r, tb) >> (4 * h);
+            const uint32_t bits[2] = {(uint32_t)there, (uint32_t)(there >> 32)};
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    s[b][i] = (uint32_t)(32 * b + (i & 3) + 8 * (i >> 2) - from) < (uint32_t)len ? s[b][i] : -INFINITY;
+                    x.s[b][i] = (bits[b] >> ((i & 3) + 8 * (i >> 2))) & 1 ? x.s[b][i] : -INFINITY;
                     if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
-            if (holes) {
-                const uint64_t there = pages_there(a, t, r, tb) >> (4 * h);
-                uint32_t bits[2] = {(uint32_t)there, (uint32_t)(there >> 32)};
-#pragma unroll
-                for (int b = 0; b < NB; b++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        s[b][i] = (bits[b] >> ((i & 3) + 8 * (i >> 2))) & 1 ? s[b][i] : -INFINITY;
-                        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                    }
-            }
         }
+    }
+    __device__ __forceinline__ static void limit(const Params& p, Scores& x) {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) x.s[b][i] = p.cap * tanh_of(x.s[b][i] * p.c);
+    }
+
+    // the running maximum, and o and l by it
+    __device__ __forceinline__ void follow(const Scores& x, float c) {
         float mx = kLowest;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[b][i]);
+            for (int i = 0; i < 16; i++) mx = fmaxf(mx, x.s[b][i]);
         mx = half_max(mx);
         if (__any((mx - m) * c > kBehind)) {
             const float to = fmaxf(m, mx), f = __builtin_amdgcn_exp2f((m - to) * c);
@@ -416,51 +528,41 @@ struct Chunk {
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] *= f;
         }
+    }
+
+    // the weights of x (exp2 of the distance to m, lifted), packed in w where the type
+    // has 16 bits
+    __device__ __forceinline__ void weigh(Scores& x, float c, Weights& w) {
         // below every product of a maximum: a masked score's weight is 0 then, and
         // so is that of a row with no score yet
         const float from = fmaxf(m * c, -0x1p126f) - kLift;
 #pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], c, -from));
-                l += s[b][i];
-            }
-        if constexpr (T == DT_F32) {
-            const uint32_t va = (uint32_t)(4 * h * RS) + (uint32_t)(((l31 >> 2) ^ v_turn(4 * h)) * 16 + (lane & 3) * 4);
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    if (kFence > 0 && i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        const float x = *reinterpret_cast<const __attribute__((address_space(3))) float*>(
-                            vb + (va ^ (d * 128)) + (32 * b + (i & 3) + 8 * (i >> 2)) * RS);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[b][i], o[d], 0, 0, 0);
-                    }
-                }
-        } else {
+        for (int e = 0; e < NB * 16; e += 2) {
+            const int b = e / 16, i = e % 16;
+            x.s[b][i] = __builtin_amdgcn_exp2f(fmaf(x.s[b][i], c, -from));
+            x.s[b][i + 1] = __builtin_amdgcn_exp2f(fmaf(x.s[b][i + 1], c, -from));
+            l += x.s[b][i] + x.s[b][i + 1];
             // One value of the type per weight: off by half a step of it each, in
             // either direction, as the result itself is once
-            const int i4 = (lane & 15) >> 2;
-            const uint32_t va = (uint32_t)((4 * h + i4) * RS) +
-                                (uint32_t)((((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_turn(4 * h + i4)) * 16) + (lane & 1) * 8);
+            if constexpr (T != DT_F32) w.w[e / 8][e % 8 / 2] = pack2<T>(x.s[b][i], x.s[b][i + 1]);
+        }
+    }
+
+    // o += V^T . weights, of the values at `at`
+    __device__ __forceinline__ void begin_values(Ahead& f, uint32_t at) const {
 #pragma unroll
-            for (int kb16 = 0; kb16 < 2 * NB; kb16++) {
-                if (kFence > 0) __builtin_amdgcn_sched_barrier(0);
-                u4 x;
+        for (int s = 0; s < AV; s++) f.v[s] = read_v(at, s);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __device__ __forceinline__ void gather(const Scores& x, const Weights& w, Ahead& f, uint32_t at) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[j] = pack2<T>(s[kb16 / 2][8 * (kb16 & 1) + 2 * j], s[kb16 / 2][8 * (kb16 & 1) + 2 * j + 1]);
-#pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    typedef __attribute__((address_space(3))) s4* tr_ptr;
-                    const s4 y0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(vb + (va ^ (d * 64)) + 16 * kb16 * RS));
-                    const s4 y1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(vb + (va ^ (d * 64)) + (16 * kb16 + 8) * RS));
-                    const u2 z0 = __builtin_bit_cast(u2, y0), z1 = __builtin_bit_cast(u2, y1);
-                    o[d] = mfma<T>(u4{z0[0], z0[1], z1[0], z1[1]}, x, o[d]);
-                }
-            }
+        for (int s = 0; s < NVS; s++) {
+            const int d = s % ND, i = s / ND;
+            if constexpr (T == DT_F32)
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f.v[s % AV][0]), x.s[i / 16][i % 16], o[d], 0, 0, 0);
+            else o[d] = mfma<T>(f.v[s % AV], w.w[i], o[d]);
+            if (s + AV < NVS) f.v[s % AV] = read_v(at, s + AV);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
@@ -470,7 +572,7 @@ struct Chunk {
     // four channels of a row of the tile: into out, or a partial result
     __device__ __forceinline__ static void store4(const Params& p, const Tile& t, int hk, int qt, int to, int row, int d, f4 acc, float top, float sum) {
         if (to >= 0) {
-            const int64_t at = (int64_t)to * (RG * 32) + row;
+            const int64_t at = (int64_t)to * ROWS + row;
             *reinterpret_cast<f4*>(p.part_o + at * DP + d) = acc;
             if (d == 0) *reinterpret_cast<u2*>(p.part_ml + at * 2) = u2{__float_as_uint(top), __float_as_uint(sum)};
             return;
@@ -567,7 +669,7 @@ struct Chunk {
     }
 
     __device__ __forceinline__ void clear() {
-        for (int i = threadIdx.x * 16; i < NS * kStage; i += NT * 16) *reinterpret_cast<u4*>(lds + i) = u4{0, 0, 0, 0};
+        for (int i = threadIdx.x * 16; i < kRings; i += NT * 16) *reinterpret_cast<u4*>(lds + i) = u4{0, 0, 0, 0};
     }
 
     // stages u0 .. u1 - 1 of a tile; to: the slot of a partial result, or -1
@@ -576,23 +678,31 @@ struct Chunk {
         const ChunkArgs& a = p.a;
         const int first_tok = t.base + u0 * ST, last_tok = t.base + u1 * ST < t.end ? t.base + u1 * ST : t.end;
         const bool any = last_tok > first_tok;
-        // are there pages that are none
+        // the table's entries, for the places of the stages and for pages that are none,
+        // and the queries in one trip
         bool none = false;
         if (any) {
             const int c0 = div_by(first_tok, a.div), c1 = div_by(last_tok - 1, a.div);
             for (int c = c0 + (int)threadIdx.x; c <= c1; c += NT)
                 none |= (uint32_t)a.table[(int64_t)r * a.columns + c] >= (uint32_t)a.pool;
-        }
-        if (threadIdx.x < RG) bad[threadIdx.x] = 0;
-        const bool holes = __syncthreads_or(none);
-        if (any) {
-#pragma unroll
-            for (int s = 0; s < NS - 1; s++)
-                if (u0 + s < u1) fill(a, t, r, hk, first_tok + s * ST, s);
+            if constexpr (EASY) find(a, t, r, hk, first_tok, 0);
         }
         load_q(p, t, hk, qt);
-        // what the compiler knows to be in flight ends here, not at its first use in the loop
-        __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0xF << 8));
+        if (threadIdx.x < RG) bad[threadIdx.x] = 0;
+        settle();
+        // step j takes stage j, which has arrived then, and fills stage j + L where stage
+        // j - 1 was
+        constexpr int L = NS - 1;
+        const int nu = any ? u1 - u0 : 0;
+        auto fill_both = [&](int s, uint32_t slot) {
+            next_rows(a, t, r, hk, first_tok, s);
+            fill<false>(a, t, r, hk, first_tok + s * ST, slot);
+            fill<true>(a, t, r, hk, first_tok + s * ST, slot);
+        };
+#pragma unroll
+        for (int s = 0; s < L; s++)
+            if (s < nu) fill_both(s, s * kMat);
+        const bool holes = __syncthreads_or(none);
         // the wave's rows: the first one's tokens and the last one's
         int head, lo0, hi0, lo1, hi1;
         sees(a, t, token_of(p, t, rg * 32, qt, head), lo0, hi0);
@@ -605,16 +715,61 @@ struct Chunk {
 #pragma unroll
             for (int i = 0; i < 16; i++) o[d][i] = 0.f;
         if (any) {
-            int buf = 0;
-            for (int u = u0; u < u1; u++) {
-                if (NS > 2 && u1 - 1 - u >= NS - 2) wait_vm<WHOLE ? (NS - 2) * 2 * NI : 0>();
+            const float c = !EASY && a.softcap > 0.f ? 1.f : p.c;
+            Scores x;
+            Weights wt;
+            uint32_t here = 0, behind = L * kMat;  // slots of stages j and j - 1
+            auto turn = [&] {
+                behind = here;
+                here = here == (NS - 1) * kMat ? 0 : here + kMat;
+            };
+            constexpr int kOut = 2 * (L - 1) * NI;  // transfers behind the stage's
+            auto step = [&](int j) {
+                if (EASY && j + L <= nu) wait_vm<kOut>();
                 else wait_vm<0>();
                 barrier();
-                const int ahead = u + NS - 1;
-                if (ahead < u1) fill(a, t, r, hk, t.base + ahead * ST, buf == 0 ? NS - 1 : buf - 1);
-                const int tb = t.base + u * ST + kg * BT;
-                if (rows && tb < hi1 && tb + BT > lo0) take(p, t, r, tb, buf, holes || tb < lo1 || tb + BT > hi0, holes);
-                buf = buf == NS - 1 ? 0 : buf + 1;
+                if (j + L < nu) fill_both(j + L, behind);
+                const int tb = first_tok + j * ST + kg * BT;
+                if (rows && tb < hi1 && tb + BT > lo0) {
+                    Ahead f;
+                    const uint32_t kat = key_at(here), vat = value_at(here);
+                    begin(f, kat);
+                    scores(x, f, kat);
+                    if (!EASY && a.softcap > 0.f) limit(p, x);
+                    if (holes || tb < lo1 || tb + BT > hi0) mask(a, x, t, r, tb, holes);
+                    follow(x, c);
+                    begin_values(f, vat);
+                    weigh(x, c, wt);
+                    gather(x, wt, f, vat);
+                }
+                turn();
+            };
+            // steps in which the wave's rows see all of a stage and whole stages are filled
+            int ja = 0, jb = 0;
+            if (EASY && rows && !holes) {
+                const int t0 = first_tok + kg * BT;
+                ja = lo1 > t0 ? (lo1 - t0 + ST - 1) / ST : 0;
+                jb = hi0 >= t0 + BT ? (hi0 - BT - t0) / ST + 1 : 0;
+                jb = jb < nu - 1 - L ? jb : nu - 1 - L;
+            }
+            for (int j = 0; j < nu; j++) {
+                for (; EASY && j >= ja && j < jb; j++) {
+                    Ahead f;
+                    wait_vm<kOut>();
+                    barrier();
+                    const uint32_t kat = key_at(here), vat = value_at(here);
+                    begin(f, kat);
+                    next_rows(a, t, r, hk, first_tok, j + L);
+                    fill_whole<false>(a, behind);
+                    fill_whole<true>(a, behind);
+                    scores(x, f, kat);
+                    follow(x, c);
+                    begin_values(f, vat);
+                    weigh(x, c, wt);
+                    gather(x, wt, f, vat);
+                    turn();
+                }
+                step(j);
             }
         }
         l += other_half(l);
@@ -654,22 +809,32 @@ struct Chunk {
                 ml[(w * 32 + l31) * 2 + 1] = l;
             }
             __syncthreads();
-            constexpr int per = DP / 4;
-            for (int x = threadIdx.x; x < RG * 32 * per; x += NT) {
-                const int row = x / per, d = (x - row * per) * 4;
-                if (!has_row(e, t, row, qt) || ((bad[row >> 5] >> (row & 31)) & 1)) continue;
-                float top = -0x1p126f;
+            // a row's groups' weights, its maximum and sum
+            float* weight = ml + NW * 32 * 2;  // [ROWS][KG + 2]
+            for (int row = threadIdx.x; row < ROWS; row += NT) {
+                float top = -0x1p126f, sum = 0.f;
 #pragma unroll
-                for (int g = 0; g < KG; g++) top = fmaxf(top, ml[(g * RG * 32 + row) * 2]);
-                float sum = 0.f;
-                f4 acc = {0.f, 0.f, 0.f, 0.f};
+                for (int g = 0; g < KG; g++) top = fmaxf(top, ml[(g * ROWS + row) * 2]);
+                float* mine_w = weight + row * (KG + 2);
 #pragma unroll
                 for (int g = 0; g < KG; g++) {
-                    const float f = __builtin_amdgcn_exp2f(ml[(g * RG * 32 + row) * 2] - top);
-                    sum += ml[(g * RG * 32 + row) * 2 + 1] * f;
-                    acc += *reinterpret_cast<const f4*>(sums + (g * RG * 32 + row) * LS + d) * f;
+                    mine_w[g] = __builtin_amdgcn_exp2f(ml[(g * ROWS + row) * 2] - top);
+                    sum += ml[(g * ROWS + row) * 2 + 1] * mine_w[g];
                 }
-                store4(e, t, hk, qt, to, row, d, acc, top, sum);
+                mine_w[KG] = top;
+                mine_w[KG + 1] = sum;
+            }
+            __syncthreads();
+            constexpr int per = DP / 4, kTurns = ROWS * per / NT;
+            static_assert(kTurns * NT == ROWS * per, "whole turns");
+#pragma unroll
+            for (int k = 0; k < kTurns; k++) {
+                const int x = (int)threadIdx.x + k * NT, row = x / per, d = (x - row * per) * 4;
+                const float* its = weight + row * (KG + 2);
+                f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int g = 0; g < KG; g++) acc += *reinterpret_cast<const f4*>(sums + (g * ROWS + row) * LS + d) * its[g];
+                if (has_row(e, t, row, qt) && !((bad[row >> 5] >> (row & 31)) & 1)) store4(e, t, hk, qt, to, row, d, acc, its[KG], its[KG + 1]);
             }
         }
         if (KG > 1 && e.a.D < RS / ES) {  // the meeting was where no transfer fills
@@ -684,7 +849,7 @@ struct Chunk {
                 if (k % NW != w || !has_row(e, t, row, qt)) continue;
                 int hd;
                 const int i = token_of(e, t, row, qt, hd);
-                const int64_t at = (int64_t)to * (RG * 32) + row;
+                const int64_t at = (int64_t)to * ROWS + row;
                 alone(e, t.first, t.pos, t.n, r, hk, hd, i, first_tok, last_tok, to >= 0 ? e.part_o + at * DP : nullptr, e.part_ml + at * 2);
             }
         }
@@ -693,24 +858,27 @@ struct Chunk {
 
 extern __shared__ __attribute__((aligned(16))) char chunk_lds[];
 
-template <int T, int DP, int RG, int KG, int BT, int NS, bool WHOLE>
+template <int T, int DP, int RG, int KG, int BT, int NS, bool EASY>
 __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void chunk_kernel(Params p) {
-    using A = Chunk<T, DP, RG, KG, BT, NS, WHOLE>;
+    using A = Chunk<T, DP, RG, KG, BT, NS, EASY>;
     constexpr int NW = A::NW, ST = A::ST;
-    __shared__ int part[NW], own[3];
+    __shared__ int part[NW];
+    __shared__ Found own;
     __shared__ uint32_t bad[RG];
     const ChunkArgs& a = p.a;
     const int tid = threadIdx.x, lane = tid & 63;
-    // an XCD takes every eighth block
-    const int me = p.P % 8 == 0 ? (int)(blockIdx.x & 7) * (p.P / 8) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
     A x(chunk_lds);
     if (a.D < A::RS / A::ES) x.clear();  // chunks that no transfer fills
     // stages of the thread's places, and of all of them for one head
     const int s0 = tid * p.each, s1 = s0 + p.each < p.slots ? s0 + p.each : p.slots;
     int mine = 0;
+    Tile t = {0, 0, 0, 0, 0, 0, 0};
+    int r = 0, tile = 0;
+    // goes through the thread's places until f() is true of one
     auto walk = [&](auto f) {
         if (s0 >= s1) return;
-        int r = request_of_place(p, s0), from = place_of(p, r);
+        r = request_of_place(p, s0);
+        int from = place_of(p, r);
         for (int s = s0; s < s1; s++) {
             if (r + 1 < a.R) {
                 const int next = place_of(p, r + 1);
@@ -719,12 +887,13 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void chunk_kernel(Params
                     from = next;
                 }
             }
-            const Tile t = tile_of<ST>(p, r, s - from);
-            if (t.m > 0 && f(r, s - from, t.units)) return;
+            tile = s - from;
+            t = tile_of<ST>(p, r, tile);
+            if (t.m > 0 && f()) return;
         }
     };
-    walk([&](int, int, int units) {
-        mine += units;
+    walk([&] {
+        mine += t.units;
         return false;
     });
     int through = wave_scan(mine);
@@ -737,41 +906,50 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void chunk_kernel(Params
         all += part[i];
     }
     all = uniform(all);
-    const Ranges ranges((uint64_t)(uint32_t)all * (uint32_t)p.HQ, p.P);
-    uint64_t pos = ranges.first(me);
-    int64_t left = (int64_t)(ranges.first(me + 1) - pos);
-    Cut cut = {0, 0, 0, 0};
-    if (left > 0) {
-        int hq = (int)(pos / (uint32_t)all);
-        const int at = (int)(pos - (uint64_t)hq * (uint32_t)all);
+    const Ranges ranges((uint64_t)(uint32_t)(all > 0 ? all : 1) * (uint32_t)p.HQ, p.log);
+    // an XCD takes every eighth block: a run of ranges
+    const int per = 1 << ranges.log >> 3, b = (int)blockIdx.x;
+    const int me = per == 0 ? b : (b >> 3) < per ? (b & 7) * per + (b >> 3) : b;
+    Cut out = {0, 0, 0, 0};
+    if (all > 0 && me < 1 << ranges.log) {
+        const uint64_t lo = ranges.first(me), hi = ranges.first(me + 1);
+        int hq = (int)((double)lo / (double)(uint32_t)all);
+        if ((uint64_t)hq * (uint32_t)all > lo) hq--;
+        if ((uint64_t)(hq + 1) * (uint32_t)all <= lo) hq++;
+        const int at = (int)(lo - (uint64_t)hq * (uint32_t)all);
         if (at >= through - mine && at < through) {
             int before = through - mine;
-            walk([&](int r, int tile, int units) {
-                if (at >= before + units) {
-                    before += units;
+            if (p.each > 1)  // else the thread's one place is still at hand
+                walk([&] {
+                    if (at < before + t.units) return true;
+                    before += t.units;
                     return false;
-                }
-                own[0] = r;
-                own[1] = tile;
-                own[2] = at - before;
-                return true;
-            });
+                });
+            own = Found{t, r, tile, at - before};
         }
         __syncthreads();
-        int r = uniform(own[0]), tile = uniform(own[1]), u = uniform(own[2]);
+        auto share = [](const Tile& x) {
+            return Tile{uniform(x.first), uniform(x.m), uniform(x.pos), uniform(x.n), uniform(x.base), uniform(x.end), uniform(x.units)};
+        };
+        t = share(own.t);
+        r = uniform(own.r);
+        tile = uniform(own.tile);
+        uint64_t start = lo - (uint32_t)uniform(own.at);  // of the tile
+        int u = ranges.cut(uniform(own.at), t.units);
         while (true) {
-            Tile t = tile_of<ST>(p, r, tile);
-            t = Tile{uniform(t.first), uniform(t.m), uniform(t.pos), uniform(t.n), uniform(t.base), uniform(t.end), uniform(t.units)};
-            const int64_t can = (int64_t)u + left;
-            const int u1 = can < t.units ? (int)can : t.units;
+            const int u1 = hi >= start + t.units ? t.units : ranges.cut((int)(hi - start), t.units);
             const int hk = p.QT == 1 ? hq : hq / p.QT, qt = hq - hk * p.QT;
-            const bool whole = u == 0 && u1 == t.units;
-            if (!whole && u == 0) cut = Cut{ranges.of(pos + t.units - 1) - me + 1, r, tile, hq};
-            if (t.m > 0 && hq < p.HQ) x.piece(t, r, hk, qt, u, u1, whole ? -1 : 2 * me + (u == 0), bad);
-            left -= u1 - u;
-            pos += u1 - u;
-            if (left <= 0) break;
+            if (u < u1 && t.m > 0 && hq < p.HQ) {
+                const bool whole = u == 0 && u1 == t.units;
+                if (!whole && u == 0) {
+                    const int last = ranges.of(start + t.units - 1);
+                    out = Cut{last - (ranges.cut((int)(ranges.first(last) - start), t.units) == t.units) - me + 1, t.first, t.m, hq};
+                }
+                x.piece(t, r, hk, qt, u, u1, whole ? -1 : 2 * me + (u == 0), bad);
+            }
+            if (hi <= start + t.units) break;
             // the next tile: of the request, of the next one with new tokens, of the next head
+            start += t.units;
             u = 0;
             tile++;
             int next = t.first + t.m;
@@ -786,25 +964,51 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void chunk_kernel(Params
                 r++;
                 if (r >= a.R || clamp(scalar_at(a.starts, r + 1), 0, a.T) <= next) r = request_of_token(a, next);
             }
+            t = share(tile_of<ST>(p, r, tile));
             __syncthreads();  // the piece's last readers of LDS
         }
     }
-    if (tid == 0 && p.cuts) p.cuts[me] = cut;
+    if (tid == 0) p.cuts[me] = out;
 }
 
-// The parts of the tile that range blockIdx.x started and others ended: a wave takes
-// a row, a lane DP / 64 of its channels.
-template <int T, int DP, int RG, int KG, int BT, int NS, bool WHOLE>
-__global__ __launch_bounds__(256) void join_kernel(Params p) {
-    using A = Chunk<T, DP, RG, KG, BT, NS, WHOLE>;
+// The parts of the tiles that were cut: a wave takes a row, a lane DP / 64 of its
+// channels.  The rows of all cut tiles are dealt out to all waves.
+template <int T, int DP, int RG, int KG, int BT, int NS, bool EASY>
+__global__ __launch_bounds__(512) void join_kernel(Params p) {
+    using A = Chunk<T, DP, RG, KG, BT, NS, EASY>;
     constexpr int NV = DP / 64;
     const ChunkArgs& a = p.a;
-    const Cut cut = p.cuts[blockIdx.x];
-    if (cut.parts == 0) return;
-    const int w0 = blockIdx.x, lane = threadIdx.x & 63;
-    const Tile t = tile_of<A::ST>(p, cut.r, cut.tile);
-    const int hk = cut.hq / p.QT, qt = cut.hq - hk * p.QT, rows = t.m * p.GT;
-    for (int row = blockIdx.y * 4 + uniform(threadIdx.x >> 6); row < rows; row += gridDim.y * 4) {
+    __shared__ Cut cuts[kChunkRanges];
+    __shared__ int through[kChunkRanges], part[8];
+    const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
+    static_assert(kChunkRanges <= 512, "a thread per range");
+    int rows = 0;
+    if (tid < p.P) {
+        const Cut c = p.cuts[tid];
+        cuts[tid] = c;
+        rows = c.parts > 0 ? c.m * p.GT : 0;
+    }
+    int sum_rows = wave_scan(rows);
+    if (lane == 63) part[w] = sum_rows;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if (i < w) sum_rows += part[i];
+        all += part[i];
+    }
+    if (tid < p.P) through[tid] = sum_rows;
+    __syncthreads();
+    for (int g = (int)blockIdx.x * 8 + w; g < all; g += (int)gridDim.x * 8) {
+        int w0 = 0, end = p.P - 1;  // the first range with more rows through it than g
+        while (w0 < end) {
+            const int mid = (w0 + end) >> 1;
+            if (through[mid] > g) end = mid;
+            else w0 = mid + 1;
+        }
+        w0 = uniform(w0);
+        const Cut cut = Cut{uniform(cuts[w0].parts), uniform(cuts[w0].first), uniform(cuts[w0].m), uniform(cuts[w0].hq)};
+        const int row = g - uniform(through[w0]) + cut.m * p.GT, hk = cut.hq / p.QT, qt = cut.hq - hk * p.QT;
         const int i = div_by(row, p.by_gt), head = qt * p.GT + row - i * p.GT;
         if (head >= a.G) continue;
         float top = -0x1p126f, sum = 0.f, acc[NV];
@@ -812,8 +1016,20 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
         for (int j = 0; j < NV; j++) acc[j] = 0.f;
         for (int s0 = 0; s0 < cut.parts; s0 += 64) {
             const int n = cut.parts - s0 < 64 ? cut.parts - s0 : 64;
-            const u2 ml = lane < n ? *reinterpret_cast<const u2*>(p.part_ml + ((int64_t)slot(w0, s0 + lane) * (RG * 32) + row) * 2) : u2{0, 0};
-            float tm = lane < n ? __uint_as_float(ml[0]) : -0x1p126f;
+            constexpr int kB = 8;
+            float v[kB][NV];
+            auto load = [&](int s) {
+#pragma unroll
+                for (int b = 0; b < kB; b++) {
+                    const int at = s + b < n ? s + b : n - 1;
+                    const float* src = p.part_o + ((int64_t)slot(w0, s0 + at) * A::ROWS + row) * DP + lane;
+#pragma unroll
+                    for (int j = 0; j < NV; j++) v[b][j] = src[64 * j];
+                }
+            };
+            const u2 ml = lane < n ? *reinterpret_cast<const u2*>(p.part_ml + ((int64_t)slot(w0, s0 + lane) * A::ROWS + row) * 2) : u2{0, 0};
+            load(0);
+            const float tm = lane < n ? __uint_as_float(ml[0]) : -0x1p126f;
             float mx = tm;
 #pragma unroll
             for (int k = 1; k < 64; k *= 2) mx = fmaxf(mx, __shfl_xor(mx, k));
@@ -824,16 +1040,8 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
             sum = sum * f0 + wave_sum(lane < n ? wgt * __uint_as_float(ml[1]) : 0.f);
 #pragma unroll
             for (int j = 0; j < NV; j++) acc[j] *= fmaxf(f0, kLeast);
-            constexpr int kB = 8;
             for (int s = 0; s < n; s += kB) {
-                float v[kB][NV];
-#pragma unroll
-                for (int b = 0; b < kB; b++) {
-                    const int at = s + b < n ? s + b : n - 1;
-                    const float* src = p.part_o + ((int64_t)slot(w0, s0 + at) * (RG * 32) + row) * DP + lane;
-#pragma unroll
-                    for (int j = 0; j < NV; j++) v[b][j] = src[64 * j];
-                }
+                if (s > 0) load(s);
 #pragma unroll
                 for (int b = 0; b < kB; b++) {
                     const float f = lane_f(wgt, s + b < n ? s + b : n - 1);
@@ -842,7 +1050,7 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
                 }
             }
         }
-        const int tok = t.first + i, hd = hk * a.G + head;
+        const int tok = cut.first + i, hd = hk * a.G + head;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const int d = lane + 64 * j;
@@ -852,11 +1060,11 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
     }
 }
 
-template <int T, int DP, int RG, int KG, int BT, int NS, bool WHOLE>
+template <int T, int DP, int RG, int KG, int BT, int NS, bool EASY>
 LuxStatus launch_as(Params& p, hipStream_t st) {
-    using A = Chunk<T, DP, RG, KG, BT, NS, WHOLE>;
+    using A = Chunk<T, DP, RG, KG, BT, NS, EASY>;
     const ChunkArgs& a = p.a;
-    constexpr int rows = RG * 32;
+    constexpr int rows = A::ROWS;
     p.GT = a.G < rows ? a.G : rows;
     p.QT = (a.G + p.GT - 1) / p.GT;
     p.HQ = a.Hk * p.QT;
@@ -865,19 +1073,30 @@ LuxStatus launch_as(Params& p, hipStream_t st) {
     p.by_gt = DivBy(p.GT);
     p.slots = a.T / p.TB + a.R;
     p.each = (p.slots + A::NT - 1) / A::NT;
-    auto main = chunk_kernel<T, DP, RG, KG, BT, NS, WHOLE>;
-    auto join = join_kernel<T, DP, RG, KG, BT, NS, WHOLE>;
+    auto main = chunk_kernel<T, DP, RG, KG, BT, NS, EASY>;
+    auto join = join_kernel<T, DP, RG, KG, BT, NS, EASY>;
     static const bool attr = hipFuncSetAttribute((const void*)main, hipFuncAttributeMaxDynamicSharedMemorySize, A::kLds) == hipSuccess;
     if (!attr) return LuxStatus::Internal;
-    p.P = a.cus < kChunkRanges ? a.cus : kChunkRanges;
+    // a block per CU, and as many as a power of two has
+    p.log = 0;
+    while ((2 << p.log) <= (a.cus < kChunkRanges ? a.cus : kChunkRanges)) p.log++;
+    p.P = 1 << p.log;
     const size_t one = (size_t)rows * (DP + 2) * 2 * 4 + sizeof(Cut);
     if (!a.ws || (size_t)p.P * one > kChunkPartBytes) return LuxStatus::NotSupported;
     p.part_o = reinterpret_cast<float*>(a.ws);
     p.part_ml = p.part_o + (size_t)2 * p.P * rows * DP;
     p.cuts = reinterpret_cast<Cut*>(p.part_ml + (size_t)2 * p.P * rows * 2);
     hipLaunchKernelGGL(main, dim3(p.P), dim3(A::NT), A::kLds, st, p);
-    hipLaunchKernelGGL(join, dim3(p.P, 8), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(join, dim3(p.P), dim3(512), 0, st, p);
     return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
+}
+
+template <int T, int DP, int RG, int KG, int BT, int NS>
+LuxStatus launch_page(Params& p, hipStream_t st) {
+    using A = Chunk<T, DP, RG, KG, BT, NS, true>;
+    if constexpr (A::RS == DP * A::ES)
+        if (p.a.D == DP && p.a.softcap == 0.f && p.a.page % A::LT == 0) return launch_as<T, DP, RG, KG, BT, NS, true>(p, st);
+    return launch_as<T, DP, RG, KG, BT, NS, false>(p, st);
 }
 
 template <int T>
@@ -889,17 +1108,24 @@ LuxStatus launch_t(const ChunkArgs& a, hipStream_t st) {
     p.c = s < 0.f ? -s : s > 0.f ? s : 0x1p-149f;
     p.flip = s < 0.f ? (T == DT_F32 ? 0x80000000u : 0x80008000u) : 0u;
     p.cap = a.softcap * kLog2e;
-    // tokens per transfer: 1024 bytes of rows
+    // Tiles of 64 rows (f32 of 128 channels: 128), whose stages are shared out among
+    // four (two) groups of waves, where there are few rows, or where the requests'
+    // fill less than three quarters of a wide tile on average: a wave of a wide tile
+    // that waits for its few stages' loads, or has only padding, costs more there than
+    // the narrow tiles' further reads of K and V.  32 heads on 8, bf16, one request's
+    // new tokens on 4096 held: 64 tokens 25.7 us against 32.4, 256 tokens 54.4 against
+    // 56.7, 512 tokens 86.5 against 80.0, 1536 tokens 215 against 191; 4 chunks of up
+    // to 512 among 64 requests 287 against 313.
+    const bool narrow = (int64_t)a.T * a.H < 48 * (int64_t)a.cus || (int64_t)a.T * a.G < 192 * (int64_t)a.R;
     if constexpr (T == DT_F32) {
-        if (a.D <= 64) return a.page % 4 ? launch_as<T, 64, 8, 1, 32, 3, false>(p, st) : launch_as<T, 64, 8, 1, 32, 3, true>(p, st);
-        if (a.D <= 128) return a.page % 2 ? launch_as<T, 128, 8, 1, 32, 3, false>(p, st) : launch_as<T, 128, 8, 1, 32, 3, true>(p, st);
-        if (a.D <= 192) return launch_as<T, 192, 4, 1, 32, 2, true>(p, st);
-        return launch_as<T, 256, 4, 1, 32, 2, true>(p, st);
+        if (a.D <= 64) return narrow ? launch_page<T, 64, 2, 4, 32, 2>(p, st) : launch_page<T, 64, 8, 1, 32, 3>(p, st);
+        if (a.D <= 128) return narrow ? launch_page<T, 128, 4, 2, 32, 2>(p, st) : launch_page<T, 128, 8, 1, 32, 3>(p, st);
+        return a.D <= 192 ? launch_page<T, 192, 4, 1, 32, 2>(p, st) : launch_page<T, 256, 4, 1, 32, 2>(p, st);
     } else {
-        if (a.D <= 64) return a.page % 8 ? launch_as<T, 64, 8, 1, 64, 3, false>(p, st) : launch_as<T, 64, 8, 1, 64, 3, true>(p, st);
-        if (a.D <= 128) return a.page % 4 ? launch_as<T, 128, 8, 1, 64, 3, false>(p, st) : launch_as<T, 128, 8, 1, 64, 3, true>(p, st);
-        if (a.D <= 192) return a.page % 2 ? launch_as<T, 192, 4, 1, 64, 2, false>(p, st) : launch_as<T, 192, 4, 1, 64, 2, true>(p, st);
-        return a.page % 2 ? launch_as<T, 256, 4, 1, 64, 2, false>(p, st) : launch_as<T, 256, 4, 1, 64, 2, true>(p, st);
+        if (a.D <= 64) return narrow ? launch_page<T, 64, 2, 4, 32, 2>(p, st) : launch_page<T, 64, 8, 1, 64, 3>(p, st);
+        if (a.D <= 128) return narrow ? launch_page<T, 128, 2, 4, 32, 2>(p, st) : launch_page<T, 128, 8, 1, 64, 3>(p, st);
+        if (a.D <= 192) return narrow ? launch_page<T, 192, 2, 2, 32, 2>(p, st) : launch_page<T, 192, 4, 1, 64, 2>(p, st);
+        return narrow ? launch_page<T, 256, 2, 2, 32, 2>(p, st) : launch_page<T, 256, 4, 1, 64, 2>(p, st);
     }
 }
 
