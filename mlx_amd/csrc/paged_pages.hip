@@ -41,30 +41,122 @@ __device__ __forceinline__ int block_sum(int v, int& all, int* part) {
     return before;
 }
 
-// --- fork -----------------------------------------------------------------------------
-
-// the table's entries of fork f: ws[f] full pages from src's row, then ws[F + f]
-// where it is not kNoEntry
-constexpr int kNoEntry = -0x7fffffff - 1;
-__device__ __forceinline__ void fork_columns(const ForkArgs& a, int f, int first, int step) {
-    const int full = a.ws[f];
-    if (full < 0) return;
-    const int32_t* from = a.table + (int64_t)a.src[f] * a.columns;
-    int32_t* to = a.table + (int64_t)a.dst[f] * a.columns;
-    for (int c = first; c < full; c += step) {
-        const int id = from[c];
-        to[c] = id;
-        if ((uint32_t)id < (uint32_t)a.pool) add_now(a.shares + id, 1);
+// the same of N values at once: v becomes the sums before
+template <int NW, int N>
+__device__ __forceinline__ void block_sums(int (&v)[N], int (&all)[N], int (*part)[N]) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int through = wave_scan(v[k]);
+        if (lane == 63) part[w][k] = through;
+        v[k] = through - v[k];
+        all[k] = 0;
     }
-    if (first == 0 && a.ws[a.F + f] != kNoEntry) to[full] = a.ws[a.F + f];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; i++)
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int x = part[i][k];
+            if (i < w) v[k] += x;
+            all[k] += x;
+        }
 }
 
-// One block: which forks are made, and the pages they take.  A fork is made if it is
-// the first one of its dst: each writes its number, below 0, as dst's length, and
-// the lowest stays.  ALL: the table too, in the same launch.
+// --- fork -----------------------------------------------------------------------------
+
+constexpr int kNoEntry = -0x7fffffff - 1;
+
+// A wave: the table's entries of a fork that shares `full` pages of row s, four
+// columns a lane at a time
+__device__ __forceinline__ void fork_columns(const ForkArgs& a, int s, int d, int full) {
+    const int32_t* from = a.table + (int64_t)s * a.columns;
+    int32_t* to = a.table + (int64_t)d * a.columns;
+    const int lane = threadIdx.x & 63;
+    for (int c = lane; c < full; c += 256) {
+        int id[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) id[i] = c + 64 * i < full ? from[c + 64 * i] : -1;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (c + 64 * i < full) to[c + 64 * i] = id[i];
+            if ((uint32_t)id[i] < (uint32_t)a.pool) add_now(a.shares + id[i], 1);
+        }
+    }
+}
+
+// a fork of n tokens (below 0: not made) of which the last are not a whole page: the
+// page for them, of which the forks before took those up to `at`.  `last`: the
+// source's entry
+struct Taken {
+    int entry;   // after the full pages' ones, or kNoEntry
+    int n;       // tokens that it holds
+    bool there;  // a page was needed and there
+};
+__device__ __forceinline__ Taken take_page(const ForkArgs& a, int f, int n, int full, int last, int at, int& all, int* part) {
+    const bool rest = n > full * a.page;
+    const bool take = rest && (uint32_t)last < (uint32_t)a.pool;
+    at += block_sum<16>(take ? 1 : 0, all, part);
+    const bool there = take && at < a.free_count;
+    const int page = there ? a.free_pages[at] : -1;
+    if (f < a.F) {
+        a.copy_src[f] = there ? last : -1;
+        a.copy_dst[f] = page;
+    }
+    return Taken{rest ? (take ? page : last) : kNoEntry, take && !there ? full * a.page : n, there};
+}
+__device__ __forceinline__ void fork_counts(const ForkArgs& a, int head, int taken, int shared, int out, int needed) {
+    a.counts[0] = head + taken;
+    a.counts[1] = shared;
+    a.counts[2] = needed - taken;
+    a.counts[3] = out;
+}
+
+// One block, a thread per fork: which forks are made (the first one of its dst is),
+// and the pages they take.  ALL: the table too, in the same launch.
 template <bool ALL>
+__global__ __launch_bounds__(1024) void fork_few_kernel(ForkArgs a) {
+    __shared__ __attribute__((aligned(16))) int dsts[1024];
+    __shared__ int part[16], parts[16][3], rows[ALL ? 1024 : 1][3];
+    const int cap = a.columns * a.page, f = threadIdx.x, head = cut(a.head[0], a.free_count);
+    const int s = f < a.F ? a.src[f] : -1, d = f < a.F ? a.dst[f] : -1;
+    bool made = (uint32_t)s < (uint32_t)a.R && (uint32_t)d < (uint32_t)a.R && s != d;
+    const int held = made ? a.lens[s] : 0, has = made ? a.lens[d] : 0;
+    made = made && has <= 0;
+    dsts[f] = made ? d : -1;
+    __syncthreads();
+    for (int g = 0; g < a.F; g += 4) {
+        const int4 x = *reinterpret_cast<const int4*>(dsts + g);
+        if ((g < f && x.x == d) || (g + 1 < f && x.y == d) || (g + 2 < f && x.z == d) || (g + 3 < f && x.w == d)) made = false;
+    }
+    const int n = made ? cut(held, cap) : -1, full = made ? div_by(n, a.div) : 0;
+    const int last = n > full * a.page ? a.table[(int64_t)s * a.columns + full] : -1;
+    if constexpr (ALL) {
+        rows[f][0] = s;
+        rows[f][1] = d;
+        rows[f][2] = full;
+        __syncthreads();
+        for (int g = f >> 6; g < a.F; g += 16) fork_columns(a, rows[g][0], rows[g][1], rows[g][2]);
+    }
+    int needed;
+    const Taken t = take_page(a, f, n, full, last, head, needed, part);
+    int v[3] = {t.there, full, f < a.F && !made}, all[3];
+    block_sums<16, 3>(v, all, parts);
+    if (made) a.lens[d] = t.n;
+    if (f == 0) fork_counts(a, head, all[0], all[1], all[2], needed);
+    if constexpr (ALL) {
+        if (t.entry != kNoEntry) a.table[(int64_t)d * a.columns + full] = t.entry;
+    } else if (f < a.F) {
+        a.ws[f] = full;
+        a.ws[a.F + f] = t.entry;
+    }
+}
+
+// One block, for more forks than threads: each writes its number, below 0, as its
+// dst's length, and the lowest stays.
 __global__ __launch_bounds__(1024) void fork_kernel(ForkArgs a) {
-    __shared__ int part[16];
+    __shared__ int part[16], parts[16][3];
     const int cap = a.columns * a.page, tid = threadIdx.x, head = cut(a.head[0], a.free_count);
     for (int f = tid; f < a.F; f += 1024) {
         const int s = a.src[f], d = a.dst[f];
@@ -78,72 +170,64 @@ __global__ __launch_bounds__(1024) void fork_kernel(ForkArgs a) {
     for (int f = tid; f < a.F; f += 1024)
         if (a.ws[f] >= 0) __hip_atomic_fetch_min(a.lens + a.dst[f], f - a.F, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    int taken = 0, shared = 0, out = 0;
-    int needed = 0;
+    int v[3] = {0, 0, 0}, all[3], needed = 0;
     for (int f0 = 0; f0 < a.F; f0 += 1024) {
         const int f = f0 + tid;
         const int n = f < a.F ? a.ws[f] : -1;
         const int d = n >= 0 ? a.dst[f] : 0;
         const bool made = n >= 0 && load_now(a.lens + d) == f - a.F;
+        int round;
         const int full = made ? div_by(n, a.div) : 0;
-        int last = -1;
-        const bool rest = made && n > full * a.page;
-        if (rest) last = a.table[(int64_t)a.src[f] * a.columns + full];
-        const bool take = rest && (uint32_t)last < (uint32_t)a.pool;
-        int all;
-        const int at = head + needed + block_sum<16>(take ? 1 : 0, all, part);
-        needed += all;
+        const int last = made && n > full * a.page ? a.table[(int64_t)a.src[f] * a.columns + full] : -1;
+        const Taken t = take_page(a, f, made ? n : -1, full, last, head + needed, round, part);
+        needed += round;
         if (f < a.F) {
-            const bool there = take && at < a.free_count;
-            const int page = there ? a.free_pages[at] : -1;
-            a.copy_src[f] = there ? last : -1;
-            a.copy_dst[f] = page;
-            a.ws[f] = made ? full : -1;
-            a.ws[a.F + f] = rest ? (take ? page : last) : kNoEntry;
-            if (made) store_now(a.lens + d, take && !there ? full * a.page : n);
-            taken += there;
-            shared += full;
-            out += !made;
+            a.ws[f] = full;
+            a.ws[a.F + f] = t.entry;
         }
+        if (made) store_now(a.lens + d, t.n);
+        v[0] += t.there;
+        v[1] += full;
+        v[2] += f < a.F && !made;
     }
-    int all_taken, all_shared, all_out;
-    block_sum<16>(taken, all_taken, part);
-    block_sum<16>(shared, all_shared, part);
-    block_sum<16>(out, all_out, part);
-    if (tid == 0) {
-        a.counts[0] = head + all_taken;
-        a.counts[1] = all_shared;
-        a.counts[2] = needed - all_taken;
-        a.counts[3] = all_out;
-    }
-    if constexpr (ALL) {
-        __syncthreads();
-        for (int f = tid >> 6; f < a.F; f += 16) fork_columns(a, f, tid & 63, 64);
-    }
+    block_sums<16, 3>(v, all, parts);
+    if (tid == 0) fork_counts(a, head, all[0], all[1], all[2], needed);
 }
 
 // a wave per fork
 __global__ __launch_bounds__(256) void fork_table_kernel(ForkArgs a) {
-    for (int64_t f = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); f < a.F; f += (int64_t)gridDim.x * 4)
-        fork_columns(a, (int)f, threadIdx.x & 63, 64);
+    for (int64_t f = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); f < a.F; f += (int64_t)gridDim.x * 4) {
+        const int full = a.ws[f], entry = a.ws[a.F + f];
+        if (full > 0) fork_columns(a, a.src[f], a.dst[f], full);
+        if (entry != kNoEntry && (threadIdx.x & 63) == 0) a.table[(int64_t)a.dst[f] * a.columns + full] = entry;
+    }
 }
 
 // --- release --------------------------------------------------------------------------
 
 constexpr int kDropBlocks = 512, kRun = 4096;  // blocks that drop entries; pages of a run
 
-// request r's pages behind what it keeps lose a holder; a page that had one alone
-// counts -1 until the list has it.  `back`: pages that go back; returns the entries
-__device__ __forceinline__ int drop(const ReleaseArgs& a, int r, int first, int step, int& back) {
+// A wave: request r's pages behind what it keeps lose a holder, and a page that had
+// one alone counts -1 until the list has it.  Four columns a lane, so that a trip to
+// the table and one to the counts serve 256.  `back`: pages that go back; returns
+// the entries
+__device__ __forceinline__ int drop(const ReleaseArgs& a, int r, int& back) {
     const int n = cut(a.lens[r], a.columns * a.page), k = a.keep[r];
     const int kept = k < 0 ? 0 : k < n ? k : n;
     const int c1 = pages_of(n, a.div);
+    const int32_t* row = a.table + (int64_t)r * a.columns;
     int entries = 0;
-    for (int c = pages_of(kept, a.div) + first; c < c1; c += step) {
-        const int id = a.table[(int64_t)r * a.columns + c];
-        if ((uint32_t)id >= (uint32_t)a.pool) continue;
-        entries++;
-        back += add_now(a.shares + id, -1) == 0;
+    for (int c = pages_of(kept, a.div) + ((int)threadIdx.x & 63); c < c1; c += 256) {
+        int id[4], had[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) id[i] = c + 64 * i < c1 ? row[c + 64 * i] : -1;
+#pragma unroll
+        for (int i = 0; i < 4; i++) had[i] = (uint32_t)id[i] < (uint32_t)a.pool ? add_now(a.shares + id[i], -1) : 1;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            entries += (uint32_t)id[i] < (uint32_t)a.pool;
+            back += had[i] == 0;
+        }
     }
     return entries;
 }
@@ -152,27 +236,25 @@ __device__ __forceinline__ void write_kept(const ReleaseArgs& a, int r) {
     a.kv[r] = k < 0 ? 0 : k < n ? k : n;
 }
 
-// the pages from p0 on, four to a thread: those that go back take the list's entries
-// from `at` on (below 0: lost)
-template <int NT>
-__device__ __forceinline__ int give_back(const ReleaseArgs& a, int p0, int at, int* part) {
-    const int p = p0 + 4 * (int)threadIdx.x;
-    int v[4], mine = 0, all;
+// four pages of a thread: their counts, how many of them go back (a count below 0),
+// and their entries of the list from `to` on (below 0: lost)
+struct Four {
+    int p, v[4];
+    __device__ __forceinline__ Four(const ReleaseArgs& a, int run) : p(run * kRun + 4 * (int)threadIdx.x) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        v[i] = p + i < a.pool ? load_now(a.shares + p + i) : 0;
-        mine += v[i] < 0;
+        for (int i = 0; i < 4; i++) v[i] = p + i < a.pool ? load_now(a.shares + p + i) : 0;
     }
-    int to = at + block_sum<NT / 64>(mine, all, part);
+    __device__ __forceinline__ int back() const { return (v[0] < 0) + (v[1] < 0) + (v[2] < 0) + (v[3] < 0); }
+    __device__ __forceinline__ void give(const ReleaseArgs& a, int to) const {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (v[i] < 0) {
-            if (to >= 0) a.free_pages[to] = p + i;
-            to++;
-            a.shares[p + i] = 0;
-        }
-    return all;
-}
+        for (int i = 0; i < 4; i++)
+            if (v[i] < 0) {
+                if (to >= 0) a.free_pages[to] = p + i;
+                to++;
+                a.shares[p + i] = 0;
+            }
+    }
+};
 __device__ __forceinline__ void release_counts(const ReleaseArgs& a, int head, int back, int entries) {
     a.counts[0] = head > back ? head - back : 0;
     a.counts[1] = back;
@@ -182,16 +264,21 @@ __device__ __forceinline__ void release_counts(const ReleaseArgs& a, int head, i
 
 // one block for small pools
 __global__ __launch_bounds__(1024) void release_kernel(ReleaseArgs a) {
-    __shared__ int part[16];
+    __shared__ int part[16], parts[16][2];
     const int tid = threadIdx.x, head = cut(a.head[0], a.free_count);
-    int back = 0, entries = 0, all_back, all_entries;
-    for (int r = tid >> 6; r < a.R; r += 16) entries += drop(a, r, tid & 63, 64, back);
-    block_sum<16>(back, all_back, part);
-    block_sum<16>(entries, all_entries, part);
+    int v[2] = {0, 0}, all[2];
+    for (int r = tid >> 6; r < a.R; r += 16) v[1] += drop(a, r, v[0]);
+    block_sums<16, 2>(v, all, parts);
     for (int r = tid; r < a.R; r += 1024) write_kept(a, r);  // kv may be lens: all have read them
-    int at = head - all_back;
-    for (int p0 = 0; p0 < a.pool; p0 += kRun) at += give_back<1024>(a, p0, at, part);
-    if (tid == 0) release_counts(a, head, all_back, all_entries);
+    int at = head - all[0];
+    for (int run = 0; run * kRun < a.pool; run++) {
+        const Four pages(a, run);
+        int back;
+        const int to = at + block_sum<16>(pages.back(), back, part);
+        pages.give(a, to);
+        at += back;
+    }
+    if (tid == 0) release_counts(a, head, all[0], all[1]);
 }
 
 // three launches: entries per block into ws, pages that go back per run into ws
@@ -199,8 +286,8 @@ __global__ __launch_bounds__(1024) void release_kernel(ReleaseArgs a) {
 __global__ __launch_bounds__(256) void release_drop_kernel(ReleaseArgs a) {
     __shared__ int part[4];
     int back = 0, entries = 0, all;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.R; r += kDropBlocks * 4) {
-        entries += drop(a, (int)r, threadIdx.x & 63, 64, back);
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.R; r += (int64_t)gridDim.x * 4) {
+        entries += drop(a, (int)r, back);
         if ((threadIdx.x & 63) == 0) write_kept(a, (int)r);
     }
     block_sum<4>(entries, all, part);
@@ -208,30 +295,24 @@ __global__ __launch_bounds__(256) void release_drop_kernel(ReleaseArgs a) {
 }
 __global__ __launch_bounds__(1024) void release_count_kernel(ReleaseArgs a) {
     __shared__ int part[16];
-    const int p = blockIdx.x * kRun + 4 * (int)threadIdx.x;
-    int mine = 0, all;
-#pragma unroll
-    for (int i = 0; i < 4; i++) mine += p + i < a.pool && a.shares[p + i] < 0;
-    block_sum<16>(mine, all, part);
+    int all;
+    block_sum<16>(Four(a, blockIdx.x).back(), all, part);
     if (threadIdx.x == 0) a.ws[kDropBlocks + blockIdx.x] = all;
 }
-__global__ __launch_bounds__(1024) void release_list_kernel(ReleaseArgs a, int runs) {
-    __shared__ int part[16];
+__global__ __launch_bounds__(1024) void release_list_kernel(ReleaseArgs a, int drops, int runs) {
+    __shared__ int parts[16][4];
     const int tid = threadIdx.x, head = cut(a.head[0], a.free_count);
-    int mine = 0, before = 0, back, first;
+    const Four pages(a, blockIdx.x);
+    // pages that go back in this run; in all, and before this run; entries
+    int v[4] = {pages.back(), 0, 0, tid < drops ? a.ws[tid] : 0}, all[4];
     for (int i = tid; i < runs; i += 1024) {
         const int n = a.ws[kDropBlocks + i];
-        mine += n;
-        before += i < (int)blockIdx.x ? n : 0;
+        v[1] += n;
+        v[2] += i < (int)blockIdx.x ? n : 0;
     }
-    block_sum<16>(mine, back, part);
-    block_sum<16>(before, first, part);
-    give_back<1024>(a, blockIdx.x * kRun, head - back + first, part);
-    if (blockIdx.x == 0) {
-        int entries;
-        block_sum<16>(tid < kDropBlocks ? a.ws[tid] : 0, entries, part);
-        if (tid == 0) release_counts(a, head, back, entries);
-    }
+    block_sums<16, 4>(v, all, parts);
+    pages.give(a, head - all[1] + all[2] + v[0]);
+    if (blockIdx.x == 0 && tid == 0) release_counts(a, head, all[1], all[3]);
 }
 
 // --- compaction -----------------------------------------------------------------------
@@ -321,15 +402,108 @@ __global__ __launch_bounds__(256) void compact_table_kernel(CompactArgs a) {
     }
 }
 
+// The same in one block, for pools of up to kFewPages and tables of up to kFewEntries:
+// the bits, the ranks before each word and the new names stay in LDS, the table's
+// entries in registers.
+constexpr int kFewPages = 8192, kFewEntries = 16384;
+__global__ __launch_bounds__(1024) void compact_few_kernel(CompactArgs a) {
+    constexpr int W = kFewPages / 32, EACH = kFewEntries / 1024;
+    __shared__ uint32_t bits[W];
+    __shared__ int before[W][2], to[kFewPages], parts[16][3];
+    const int tid = threadIdx.x, entries = a.R * a.columns, cap = a.columns * a.page;
+    if (tid < W) bits[tid] = 0;
+    if (a.shares_out != a.shares)
+        for (int p = tid; p < a.pool; p += 1024) a.shares_out[p] = a.shares[p];
+    __syncthreads();
+    int id[EACH];
+    uint32_t held = 0;
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+        const int x = tid + 1024 * k;
+        id[k] = x < entries ? a.table[x] : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+        const int x = tid + 1024 * k;
+        if (x >= entries) break;
+        const int r = div_by(x, a.by_columns), c = x - r * a.columns;
+        const bool in = c < pages_of(cut(a.lens[r], cap), a.div);
+        held |= (uint32_t)in << k;
+        if (in && (uint32_t)id[k] < (uint32_t)a.pool) atomicOr(bits + (id[k] >> 5), 1u << (id[k] & 31));
+    }
+    __syncthreads();
+    // of word w: live pages from the limit on, and places below it
+    auto low = [&](int w) { return 32 * w + 32 <= a.limit ? ~0u : 32 * w >= a.limit ? 0u : (1u << (a.limit & 31)) - 1u; };
+    int v[3] = {0, 0, 0}, all[3];
+    if (tid < W) {
+        const uint32_t b = bits[tid], l = low(tid);
+        v[0] = __popc(b & ~l);
+        v[1] = __popc(~b & l);
+        v[2] = __popc(b);
+    }
+    block_sums<16, 3>(v, all, parts);
+    if (tid < W) {
+        before[tid][0] = v[0];
+        before[tid][1] = v[1];
+    }
+    const int high = all[0], room = all[1];
+    int moves = high < room ? high : room;
+    moves = moves < a.max_moves ? moves : a.max_moves;
+    const int first = a.free_count - (room - moves);
+    __syncthreads();
+    auto rank_high = [&](int p) { return before[p >> 5][0] + __popc(bits[p >> 5] & ~low(p >> 5) & ((1u << (p & 31)) - 1u)); };
+    for (int p = tid; p < a.limit; p += 1024) {
+        const uint32_t b = bits[p >> 5];
+        if ((b >> (p & 31)) & 1) continue;
+        const int at = before[p >> 5][1] + __popc(~b & ((1u << (p & 31)) - 1u));
+        if (at < moves) {
+            a.copy_dst[at] = p;
+            to[at] = p;
+        } else if (first + at - moves >= 0) {
+            a.free_pages[first + at - moves] = p;
+        }
+    }
+    for (int i = moves + tid; i < a.max_moves; i += 1024) a.copy_src[i] = a.copy_dst[i] = -1;
+    __syncthreads();
+    for (int p = a.limit + tid; p < a.pool; p += 1024) {
+        if (!((bits[p >> 5] >> (p & 31)) & 1)) continue;
+        const int at = rank_high(p);
+        if (at >= moves) continue;
+        a.copy_src[at] = p;
+        a.shares_out[to[at]] = a.shares[p];
+        a.shares_out[p] = 0;
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; k++) {
+        const int x = tid + 1024 * k;
+        if (x >= entries) break;
+        const bool in = (held >> k) & 1;
+        int now = id[k];
+        if (in && now >= a.limit && now < a.pool) {
+            const int at = rank_high(now);
+            if (at < moves) now = to[at];
+        }
+        if (now != id[k] || a.table_out != a.table) a.table_out[x] = now;
+    }
+    if (tid == 0) {
+        a.counts[0] = first > 0 ? first : 0;
+        a.counts[1] = moves;
+        a.counts[2] = high - moves;
+        a.counts[3] = all[2];
+    }
+}
+
 // --- copy -----------------------------------------------------------------------------
 
 constexpr int kPiece = 16384;  // bytes of a block
 
-// pieces of `pieces` per page of a matrix; matrices: keys and values of each layer
+// Pieces of a page, pages, then matrices (keys and values of each layer): blocks that
+// run together stay within a matrix, whose pages lie close (4096 pages' contents in
+// 16 layers: 342 us against 369 with the matrices of a page one after the other)
 template <class V>
 __global__ __launch_bounds__(256) void copy_kernel(CopyArgs a, int first, int pieces) {
     const uint32_t b = (uint32_t)first + blockIdx.x, pair = b / (uint32_t)pieces, piece = b - pair * (uint32_t)pieces;
-    const uint32_t i = pair / (uint32_t)(2 * a.layers), m = pair - i * (uint32_t)(2 * a.layers);
+    const uint32_t m = pair / (uint32_t)a.n, i = pair - m * (uint32_t)a.n;
     const int from = a.src[i], to = a.dst[i];
     if ((uint32_t)from >= (uint32_t)a.pool || (uint32_t)to >= (uint32_t)a.pool || from == to) return;
     char* base = static_cast<char*>(m & 1 ? a.vc : a.kc) + (int64_t)(m >> 1) * a.layer_bytes;
@@ -363,29 +537,40 @@ unsigned blocks_of(int64_t items, int per, int most) {
 
 LuxStatus launch_paged_fork(const ForkArgs& a, hipStream_t st) {
     if (!a.ws || (size_t)a.F * 2 > a.ws_words) return LuxStatus::NotSupported;
-    if ((int64_t)a.F * a.columns <= 16384) {
-        hipLaunchKernelGGL(fork_kernel<true>, dim3(1), dim3(1024), 0, st, a);
-    } else {
-        hipLaunchKernelGGL(fork_kernel<false>, dim3(1), dim3(1024), 0, st, a);
-        hipLaunchKernelGGL(fork_table_kernel, dim3(blocks_of(a.F, 4, 4096)), dim3(256), 0, st, a);
+    // A wave of the one block takes its forks one after the other, 2 us each; a second
+    // launch costs 3 us and has a wave for each: 24 forks (with 24 KB pages copied and
+    // given back again) take 18.8 us against 21.5, 224 forks 177 against 172.
+    if (a.F <= 64 && (int64_t)a.F * a.columns <= 16384) {
+        hipLaunchKernelGGL(fork_few_kernel<true>, dim3(1), dim3(1024), 0, st, a);
+        return status();
     }
+    if (a.F <= 1024) hipLaunchKernelGGL(fork_few_kernel<false>, dim3(1), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL(fork_kernel, dim3(1), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL(fork_table_kernel, dim3(blocks_of(a.F, 4, 4096)), dim3(256), 0, st, a);
     return status();
 }
 
 LuxStatus launch_paged_release(const ReleaseArgs& a, hipStream_t st) {
-    const int runs = (a.pool + kRun - 1) / kRun;
-    if (a.pool <= 8 * kRun && (int64_t)a.R * a.columns <= 65536) {
+    const int runs = a.pool > 0 ? (a.pool + kRun - 1) / kRun : 1;
+    // A round of the one block's sixteen waves over requests, or over a run of pages,
+    // takes about as long as another launch.
+    if (a.pool <= kRun && a.R <= 16) {
         hipLaunchKernelGGL(release_kernel, dim3(1), dim3(1024), 0, st, a);
         return status();
     }
     if (!a.ws || (size_t)runs + kDropBlocks > a.ws_words) return LuxStatus::NotSupported;
-    hipLaunchKernelGGL(release_drop_kernel, dim3(kDropBlocks), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(release_count_kernel, dim3(runs < 1 ? 1 : runs), dim3(1024), 0, st, a);
-    hipLaunchKernelGGL(release_list_kernel, dim3(runs < 1 ? 1 : runs), dim3(1024), 0, st, a, runs);
+    const unsigned drops = blocks_of(a.R, 4, kDropBlocks);
+    hipLaunchKernelGGL(release_drop_kernel, dim3(drops), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(release_count_kernel, dim3(runs), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL(release_list_kernel, dim3(runs), dim3(1024), 0, st, a, (int)drops, runs);
     return status();
 }
 
 LuxStatus launch_paged_compact(const CompactArgs& a, hipStream_t st) {
+    if (a.pool <= kFewPages && (int64_t)a.R * a.columns <= kFewEntries) {
+        hipLaunchKernelGGL(compact_few_kernel, dim3(1), dim3(1024), 0, st, a);
+        return status();
+    }
     if (!a.ws || (size_t)a.pool + (size_t)(a.pool + 31) / 32 > a.ws_words) return LuxStatus::NotSupported;
     hipLaunchKernelGGL(compact_clear_kernel, dim3(blocks_of(a.pool, 256, 1024)), dim3(256), 0, st, a);
     hipLaunchKernelGGL(compact_mark_kernel, dim3(blocks_of(a.R, 4, 4096)), dim3(256), 0, st, a);

@@ -51,7 +51,7 @@ struct CompactArgs {
     const int32_t *lens, *table, *shares;
     int32_t *table_out, *shares_out, *free_pages, *copy_src, *copy_dst, *counts;
     int R, columns, page, pool, free_count, limit, max_moves;
-    DivBy div;
+    DivBy div, by_columns;
     int32_t* ws;
     size_t ws_words;
 };

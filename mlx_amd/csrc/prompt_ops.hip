@@ -155,7 +155,7 @@ LuxBackendError op_paged_compact(LuxBackendContext* c, const lux_paged_compact_a
     if (!s.apart()) return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     a.R = p->requests; a.columns = p->max_pages; a.page = p->page_size; a.pool = p->num_pages; a.free_count = p->free_count;
     a.limit = p->limit; a.max_moves = p->max_moves;
-    a.div = lxq::DivBy(p->page_size);
+    a.div = lxq::DivBy(p->page_size); a.by_columns = lxq::DivBy(p->max_pages > 0 ? p->max_pages : 1);
     a.ws = words(ctx, a.ws_words);
     if (hipSetDevice(ctx->device) != hipSuccess) return LUX_BACKEND_ERROR_DEVICE_LOST;
     return map_status(lxq::launch_paged_compact(a, ctx->stream));

@@ -98,7 +98,8 @@ struct Shared {
     uint64_t most[NW];
     uint32_t groups[kGroups];
     float part[NW][3];
-    int count, odd;
+    int count, odd, threads;
+    uint16_t who[NT];
 };
 
 // the row's scores, from its sums and its top entries
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
     const int token = want ? a.tokens[r] : -1;
     const bool has = (uint32_t)token < (uint32_t)a.V;
     const float x_tok = has ? logit<T>(base, token) : 0.f;
-    if (tid == 0) sh.count = sh.odd = 0;
+    if (tid == 0) sh.count = sh.odd = sh.threads = 0;
 
     // the thread's vectors tid, tid + NT, ..., and logits behind the vectors likewise
     float top = -INFINITY, ref = 0.f, s = 0.f, e = 0.f;  // ref: r c, as the loop subtracts it
@@ -171,10 +172,18 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
             take(x, E);
         }
     }
-    for (; v < vectors; v += NT) {
-        float x[E];
-        unpack<T>(*reinterpret_cast<const u4h*>(base + (int64_t)v * 16), x);
-        take(x, E);
+    {
+        u4 d[kU - 1];
+#pragma unroll
+        for (int k = 0; k < kU - 1; k++)
+            if (v + k * NT < vectors) d[k] = *reinterpret_cast<const u4h*>(base + (int64_t)(v + k * NT) * 16);
+#pragma unroll
+        for (int k = 0; k < kU - 1; k++) {
+            if (v + k * NT >= vectors) break;
+            float x[E];
+            unpack<T>(d[k], x);
+            take(x, E);
+        }
     }
     const int behind = vectors * E;
     for (int i = behind + tid; i < n; i += NT) {
@@ -262,29 +271,33 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
 
     int found = 0;
     if (a.top > 0 && !nan) {
-        // logits from the bound on
-        uint64_t flagged = __ballot(any && key_of(top) >= bound);
-        while (flagged) {
-            const int t0 = __builtin_ctzll(flagged), who = (w << 6) + t0;
-            flagged &= flagged - 1;
-            for (int i = who + lane * NT; i < vectors; i += 64 * NT) {
-                float x[E];
-                unpack<T>(*reinterpret_cast<const u4h*>(base + (int64_t)i * 16), x);
+        // the threads that have logits from the bound on, then those logits: a thread
+        // reads one vector of one of them
+        if (any && key_of(top) >= bound) {
+            const int at = atomicAdd(&sh.threads, 1);
+            sh.who[at] = (uint16_t)tid;
+        }
+        __syncthreads();
+        const int each = (vectors + NT - 1) / NT, items = sh.threads * each;
+        for (int x0 = tid; x0 < items; x0 += NT) {
+            const int which = (int)((uint32_t)x0 / (uint32_t)each), i = sh.who[which] + (x0 - which * each) * NT;
+            if (i >= vectors) continue;
+            float x[E];
+            unpack<T>(*reinterpret_cast<const u4h*>(base + (int64_t)i * 16), x);
 #pragma unroll
-                for (int j = 0; j < E; j++) {
-                    const uint32_t k = key_of(x[j]);
-                    if (k >= bound) {
-                        const int at = atomicAdd(&sh.count, 1);
-                        if (at < kRoom) sh.list[at] = entry_of(k, from + i * E + j);
-                    }
-                }
-            }
-            for (int i = behind + who + lane * NT; i < n; i += 64 * NT) {
-                const uint32_t k = key_of(logit<T>(base, i));
+            for (int j = 0; j < E; j++) {
+                const uint32_t k = key_of(x[j]);
                 if (k >= bound) {
                     const int at = atomicAdd(&sh.count, 1);
-                    if (at < kRoom) sh.list[at] = entry_of(k, from + i);
+                    if (at < kRoom) sh.list[at] = entry_of(k, from + i * E + j);
                 }
+            }
+        }
+        for (int i = behind + tid; i < n; i += NT) {
+            const uint32_t k = key_of(logit<T>(base, i));
+            if (k >= bound) {
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < kRoom) sh.list[at] = entry_of(k, from + i);
             }
         }
         __syncthreads();
@@ -348,6 +361,8 @@ __global__ __launch_bounds__(NT) void logprobs_join_kernel(Params p, int first) 
     const float x_tok = has ? logit<T>(static_cast<const char*>(a.logits) + (int64_t)r * a.row * (T == DT_F32 ? 4 : 2), token) : 0.f;
     const uint64_t* tops = p.tops + (int64_t)r * p.parts * a.top;
     if (tid == 0) count = 0;
+    const int entries = p.parts * a.top;
+    const uint64_t first_entry = tid < entries ? tops[tid] : 0, second_entry = tid + NT < entries ? tops[tid + NT] : 0;
     // each wave for itself
     const Sums mine = lane < p.parts ? p.sums[(int64_t)r * p.parts + lane] : Sums{-INFINITY, 0.f, 0.f};
     uint32_t k = lane < p.parts ? key_of(mine.top) : 0u;
@@ -367,18 +382,19 @@ __global__ __launch_bounds__(NT) void logprobs_join_kernel(Params p, int first) 
     if (tid == 0) write_sums(a, r, t, x_tok, has, log_sum);
     else log_sum = t.top == -INFINITY || t.top == INFINITY ? 0.f : log2f(t.s) * kLn2;
     if (a.top == 0) return;
-    // a bound: each part's entries down to the k-th over the parts, rounded up, are
-    // at least k
-    const int down = (a.top + p.parts - 1) / p.parts - 1;
-    uint64_t low = lane < p.parts ? tops[lane * a.top + down] : ~0ull;
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) {
-        const uint64_t o = __shfl_xor(low, i);
-        low = low < o ? low : o;
+    // a bound: the m-th largest of the parts' d-th entries, where m d is top or more
+    const int d = (a.top + p.parts - 1) / p.parts, m = (a.top + d - 1) / d;
+    const uint64_t low_mine = lane < p.parts ? tops[lane * a.top + d - 1] : 0;
+    int rank_low = 0;
+    for (int i = 0; i < p.parts; i++) {
+        const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(low_mine >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)low_mine, i);
+        rank_low += o > low_mine || (o == low_mine && i < lane);
     }
+    const int holder = __builtin_ctzll(__ballot(lane < p.parts && rank_low == m - 1));
+    const uint64_t low = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(low_mine >> 32), holder) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)low_mine, holder);
     __syncthreads();
-    for (int i = tid; i < p.parts * a.top; i += NT) {
-        const uint64_t x = tops[i];
+    for (int i = tid; i < entries; i += NT) {
+        const uint64_t x = i == tid ? first_entry : i == tid + NT ? second_entry : tops[i];
         if (x >= low && x != 0) {
             const int at = atomicAdd(&count, 1);
             if (at < kRoom) list[at] = x;
@@ -387,7 +403,7 @@ __global__ __launch_bounds__(NT) void logprobs_join_kernel(Params p, int first) 
     __syncthreads();
     const int found = count;
     const uint64_t* from = found <= kRoom ? list : tops;
-    const int n = found <= kRoom ? found : p.parts * a.top;
+    const int n = found <= kRoom ? found : entries;
     for (int i = tid; i < n; i += NT) {
         const uint64_t x = from[i];
         int rank = 0;
