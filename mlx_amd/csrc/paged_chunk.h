@@ -1109,23 +1109,31 @@ LuxStatus launch_t(const ChunkArgs& a, hipStream_t st) {
     p.flip = s < 0.f ? (T == DT_F32 ? 0x80000000u : 0x80008000u) : 0u;
     p.cap = a.softcap * kLog2e;
     // Tiles of 64 rows (f32 of 128 channels: 128), whose stages are shared out among
-    // four (two) groups of waves, where there are few rows, or where the requests'
-    // fill less than three quarters of a wide tile on average: a wave of a wide tile
-    // that waits for its few stages' loads, or has only padding, costs more there than
-    // the narrow tiles' further reads of K and V.  32 heads on 8, bf16, one request's
-    // new tokens on 4096 held: 64 tokens 25.7 us against 32.4, 256 tokens 54.4 against
-    // 56.7, 512 tokens 86.5 against 80.0, 1536 tokens 215 against 191; 4 chunks of up
-    // to 512 among 64 requests 287 against 313.
-    const bool narrow = (int64_t)a.T * a.H < 48 * (int64_t)a.cus || (int64_t)a.T * a.G < 192 * (int64_t)a.R;
+    // four (two) groups of waves, where there are few rows: a wave of a wide tile waits
+    // longer for its few stages than the narrow tiles' further reads of K and V cost.
+    // 32 heads on 8, bf16, one request's new tokens on 4096 held: 64 tokens 25.8 us
+    // against 32.5, 256 tokens 54.6 against 56.9, but 512 tokens 86.8 against 80.0 and
+    // 4096 tokens 628 against 509.
+    const bool few = (int64_t)a.T * a.H < 48 * (int64_t)a.cus;
+    // Tiles of 128 rows and two groups, where the requests' rows fill less than three
+    // quarters of a wide tile on average, whose waves have only padding then: 4 chunks
+    // of up to 512 among 64 requests 260 us, against 313 with wide tiles and 288 with
+    // narrow ones; 16384 tokens of one request 3.1 ms against 2.5.
+    const bool padded = (int64_t)a.T * a.G < 192 * (int64_t)a.R;
     if constexpr (T == DT_F32) {
-        if (a.D <= 64) return narrow ? launch_page<T, 64, 2, 4, 32, 2>(p, st) : launch_page<T, 64, 8, 1, 32, 3>(p, st);
-        if (a.D <= 128) return narrow ? launch_page<T, 128, 4, 2, 32, 2>(p, st) : launch_page<T, 128, 8, 1, 32, 3>(p, st);
+        if (a.D <= 64) return few || padded ? launch_page<T, 64, 2, 4, 32, 2>(p, st) : launch_page<T, 64, 8, 1, 32, 3>(p, st);
+        if (a.D <= 128) return few || padded ? launch_page<T, 128, 4, 2, 32, 2>(p, st) : launch_page<T, 128, 8, 1, 32, 3>(p, st);
         return a.D <= 192 ? launch_page<T, 192, 4, 1, 32, 2>(p, st) : launch_page<T, 256, 4, 1, 32, 2>(p, st);
+    } else if (a.D <= 64) {
+        if (few) return launch_page<T, 64, 2, 4, 32, 2>(p, st);
+        return padded ? launch_page<T, 64, 4, 2, 64, 2>(p, st) : launch_page<T, 64, 8, 1, 64, 3>(p, st);
+    } else if (a.D <= 128) {
+        if (few) return launch_page<T, 128, 2, 4, 32, 2>(p, st);
+        return padded ? launch_page<T, 128, 4, 2, 64, 2>(p, st) : launch_page<T, 128, 8, 1, 64, 3>(p, st);
+    } else if (a.D <= 192) {
+        return few || padded ? launch_page<T, 192, 2, 2, 32, 2>(p, st) : launch_page<T, 192, 4, 1, 64, 2>(p, st);
     } else {
-        if (a.D <= 64) return narrow ? launch_page<T, 64, 2, 4, 32, 2>(p, st) : launch_page<T, 64, 8, 1, 64, 3>(p, st);
-        if (a.D <= 128) return narrow ? launch_page<T, 128, 2, 4, 32, 2>(p, st) : launch_page<T, 128, 8, 1, 64, 3>(p, st);
-        if (a.D <= 192) return narrow ? launch_page<T, 192, 2, 2, 32, 2>(p, st) : launch_page<T, 192, 4, 1, 64, 2>(p, st);
-        return narrow ? launch_page<T, 256, 2, 2, 32, 2>(p, st) : launch_page<T, 256, 4, 1, 64, 2>(p, st);
+        return few || padded ? launch_page<T, 256, 2, 2, 32, 2>(p, st) : launch_page<T, 256, 4, 1, 64, 2>(p, st);
     }
 }
 
