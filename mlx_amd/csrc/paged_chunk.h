@@ -231,15 +231,22 @@ __device__ __forceinline__ f16v mfma(const u4& x, const u4& y, f16v c) {
 
 typedef const __attribute__((address_space(3))) char* lds_ptr;
 
-// T: type of q, cache and out; DP: head_dim rounded up to 64, 128, 192 or 256; RG
+// How a wave finds its tokens' rows of the cache.  kLanes: each lane its own, with a
+// load of the table per transfer.  kRuns: pages hold whole runs of the tokens that a
+// wave finds with one entry of the table, so that a run has one scalar address,
+// looked up for 64 stages at a time.  kPlain: as kRuns, and head_dim is DP, a power
+// of two, and scores are not capped, so that the steps of most stages hold nothing
+// but the products and the softmax.
+enum { kLanes, kRuns, kPlain };
+
+// T: type of q, cache and out; DP: head_dim rounded up to 64, 96, 128, 192 or 256; RG
 // row groups times KG groups of tokens = waves; BT: tokens of a group's part of a
-// stage; NS: stages in LDS; EASY: head_dim is DP, a power of two, scores are not capped, and
-// pages hold whole runs of the tokens that a wave finds with one entry of the
-// table, so that a run has one scalar address (else each lane finds its token's)
-template <int T, int DP, int RG, int KG, int BT, int NS, bool EASY>
+// stage; NS: stages in LDS
+template <int T, int DP, int RG, int KG, int BT, int NS, int FORM>
 struct Chunk {
     static constexpr int ES = T == DT_F32 ? 4 : 2, E = 16 / ES;  // bytes; elements per 16 bytes
-    static constexpr int RS = (DP == 192 ? 256 : DP) * ES;       // LDS row of a token
+    static constexpr bool EASY = FORM == kPlain;
+    static constexpr int RS = (DP == 192 ? 256 : DP == 96 ? 128 : DP) * ES;  // LDS row of a token
     static constexpr int CPR = RS / 16, TI = 64 / CPR;           // its 16-byte chunks; tokens per transfer
     static constexpr int NW = RG * KG, NT = 64 * NW, ST = BT * KG, NI = ST / TI / NW;
     static_assert(NI * TI * NW == ST && TI <= 16, "every wave moves whole runs");
@@ -314,7 +321,7 @@ struct Chunk {
         for (int j = 0; j < NI; j++) {
             const int run = w * NI + j, in = j * TI % LT;  // the run's first token, from where the entry was found
             const uint32_t c = V ? voff ^ (uint32_t)(v_turn(run * TI) * 16) : koff ^ (uint32_t)(k_turn(run * TI) * 16);
-            if constexpr (EASY) {
+            if constexpr (FORM != kLanes) {
                 const int i = j * TI / LT;
                 const char* from = cache + (uint64_t)(uint32_t)row_at[i] * row_bytes;
                 uint32_t at = c + (uint32_t)(ri + in) * row_bytes;
@@ -322,7 +329,7 @@ struct Chunk {
                     const int t0 = tb + w * NI * TI + i * LT, tr = t0 < t.end ? t0 : (t.end - 1) & ~(LT - 1), last = t.end - 1 - tr;
                     at = c + (uint32_t)(ri + in < last ? ri + in : last) * row_bytes;
                 }
-                dma16(dst + j * 1024, from, at);
+                if (EASY || c < row_bytes) dma16(dst + j * 1024, from, at);
             } else {
                 int tok = tb + run * TI + ri;
                 tok = tok < t.end ? tok : t.end - 1;
@@ -334,21 +341,23 @@ struct Chunk {
             }
         }
     }
-    // the same of a stage that is all there, in an EASY form
+    // the same of a stage that is all there
     template <bool V>
     __device__ __forceinline__ void fill_whole(const ChunkArgs& a, uint32_t slot) const {
         const uint32_t dst = lds_at() + (V ? NS * kMat : 0) + slot;
+        const uint32_t row_bytes = (uint32_t)((EASY ? DP : a.D) * ES);
 #pragma unroll
         for (int j = 0; j < NI; j++) {
             const uint32_t c = V ? voff ^ (uint32_t)(v_turn((w * NI + j) * TI) * 16) : koff ^ (uint32_t)(k_turn((w * NI + j) * TI) * 16);
             const int i = j * TI / LT;
-            const char* from = static_cast<const char*>(V ? a.vc : a.kc) + (uint64_t)(uint32_t)row_at[i] * (uint32_t)(DP * ES);
-            dma16(dst + j * 1024, from, c + (uint32_t)(lane / CPR + j * TI % LT) * (uint32_t)(DP * ES));
+            const char* from = static_cast<const char*>(V ? a.vc : a.kc) + (uint64_t)(uint32_t)row_at[i] * row_bytes;
+            const uint32_t at = c + (uint32_t)(lane / CPR + j * TI % LT) * row_bytes;
+            if (EASY || c < row_bytes) dma16(dst + j * 1024, from, at);
         }
     }
     // the rows of stage s
     __device__ __forceinline__ void next_rows(const ChunkArgs& a, const Tile& t, int r, int hk, int first_tok, int s) {
-        if constexpr (EASY) {
+        if constexpr (FORM != kLanes) {
             if ((s & 63) == 0 && s > 0) {
                 find(a, t, r, hk, first_tok, s);
                 settle();
@@ -611,7 +620,7 @@ struct Chunk {
     __device__ __forceinline__ static void alone(const Params& p, int first, int pos, int n, int r, int hk, int head, int i, int from, int to,
                                               float* part_o, float* part_ml) {
         const ChunkArgs& a = p.a;
-        constexpr int NV = DP / 64;
+        constexpr int NV = (DP + 63) / 64;
         const int lane = threadIdx.x & 63, at = pos + i;
         const int lo = a.window > 0 && at + 1 > a.window ? at + 1 - a.window : 0, hi = at + 1 < n ? at + 1 : n;
         const float c = a.softcap > 0.f ? 1.f : p.c;
@@ -652,7 +661,7 @@ struct Chunk {
         for (int j = 0; j < NV; j++) {
             const int d = lane + 64 * j;
             if (part_o) {
-                part_o[d] = acc[j] * up;
+                if (d < DP) part_o[d] = acc[j] * up;
             } else if (d < a.D) {
                 const float y = l == 0.f ? 0.f : acc[j] / l;
                 store_f(a.out, (size_t)((int64_t)tok * a.out_row + (int64_t)hd * a.D + d), T, y);
@@ -685,7 +694,7 @@ struct Chunk {
             const int c0 = div_by(first_tok, a.div), c1 = div_by(last_tok - 1, a.div);
             for (int c = c0 + (int)threadIdx.x; c <= c1; c += NT)
                 none |= (uint32_t)a.table[(int64_t)r * a.columns + c] >= (uint32_t)a.pool;
-            if constexpr (EASY) find(a, t, r, hk, first_tok, 0);
+            if constexpr (FORM != kLanes) find(a, t, r, hk, first_tok, 0);
         }
         load_q(p, t, hk, qt);
         if (threadIdx.x < RG) bad[threadIdx.x] = 0;
@@ -725,7 +734,7 @@ struct Chunk {
             };
             constexpr int kOut = 2 * (L - 1) * NI;  // transfers behind the stage's
             auto step = [&](int j) {
-                if (EASY && j + L <= nu) wait_vm<kOut>();
+                if (FORM != kLanes && j + L <= nu) wait_vm<kOut>();
                 else wait_vm<0>();
                 barrier();
                 if (j + L < nu) fill_both(j + L, behind);
@@ -746,14 +755,14 @@ struct Chunk {
             };
             // steps in which the wave's rows see all of a stage and whole stages are filled
             int ja = 0, jb = 0;
-            if (EASY && rows && !holes) {
+            if (FORM != kLanes && rows && !holes) {
                 const int t0 = first_tok + kg * BT;
                 ja = lo1 > t0 ? (lo1 - t0 + ST - 1) / ST : 0;
                 jb = hi0 >= t0 + BT ? (hi0 - BT - t0) / ST + 1 : 0;
                 jb = jb < nu - 1 - L ? jb : nu - 1 - L;
             }
             for (int j = 0; j < nu; j++) {
-                for (; EASY && j >= ja && j < jb; j++) {
+                for (; FORM != kLanes && j >= ja && j < jb; j++) {
                     Ahead f;
                     wait_vm<kOut>();
                     barrier();
@@ -763,6 +772,7 @@ struct Chunk {
                     fill_whole<false>(a, behind);
                     fill_whole<true>(a, behind);
                     scores(x, f, kat);
+                    if (!EASY && a.softcap > 0.f) limit(p, x);
                     follow(x, c);
                     begin_values(f, vat);
                     weigh(x, c, wt);
@@ -858,9 +868,9 @@ struct Chunk {
 
 extern __shared__ __attribute__((aligned(16))) char chunk_lds[];
 
-template <int T, int DP, int RG, int KG, int BT, int NS, bool EASY>
+template <int T, int DP, int RG, int KG, int BT, int NS, int FORM>
 __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void chunk_kernel(Params p) {
-    using A = Chunk<T, DP, RG, KG, BT, NS, EASY>;
+    using A = Chunk<T, DP, RG, KG, BT, NS, FORM>;
     constexpr int NW = A::NW, ST = A::ST;
     __shared__ int part[NW];
     __shared__ Found own;
@@ -972,11 +982,11 @@ __global__ __launch_bounds__(64 * RG * KG, RG * KG / 4) void chunk_kernel(Params
 }
 
 // The parts of the tiles that were cut: a wave takes a row, a lane DP / 64 of its
-// channels.  The rows of all cut tiles are dealt out to all waves.
-template <int T, int DP, int RG, int KG, int BT, int NS, bool EASY>
+// channels, rounded up (those past DP are another row's and are not stored).  The rows of all cut tiles are dealt out to all waves.
+template <int T, int DP, int RG, int KG, int BT, int NS, int FORM>
 __global__ __launch_bounds__(512) void join_kernel(Params p) {
-    using A = Chunk<T, DP, RG, KG, BT, NS, EASY>;
-    constexpr int NV = DP / 64;
+    using A = Chunk<T, DP, RG, KG, BT, NS, FORM>;
+    constexpr int NV = (DP + 63) / 64;
     const ChunkArgs& a = p.a;
     __shared__ Cut cuts[kChunkRanges];
     __shared__ int through[kChunkRanges], part[8];
@@ -1060,9 +1070,9 @@ __global__ __launch_bounds__(512) void join_kernel(Params p) {
     }
 }
 
-template <int T, int DP, int RG, int KG, int BT, int NS, bool EASY>
+template <int T, int DP, int RG, int KG, int BT, int NS, int FORM>
 LuxStatus launch_as(Params& p, hipStream_t st) {
-    using A = Chunk<T, DP, RG, KG, BT, NS, EASY>;
+    using A = Chunk<T, DP, RG, KG, BT, NS, FORM>;
     const ChunkArgs& a = p.a;
     constexpr int rows = A::ROWS;
     p.GT = a.G < rows ? a.G : rows;
@@ -1073,8 +1083,8 @@ LuxStatus launch_as(Params& p, hipStream_t st) {
     p.by_gt = DivBy(p.GT);
     p.slots = a.T / p.TB + a.R;
     p.each = (p.slots + A::NT - 1) / A::NT;
-    auto main = chunk_kernel<T, DP, RG, KG, BT, NS, EASY>;
-    auto join = join_kernel<T, DP, RG, KG, BT, NS, EASY>;
+    auto main = chunk_kernel<T, DP, RG, KG, BT, NS, FORM>;
+    auto join = join_kernel<T, DP, RG, KG, BT, NS, FORM>;
     static const bool attr = hipFuncSetAttribute((const void*)main, hipFuncAttributeMaxDynamicSharedMemorySize, A::kLds) == hipSuccess;
     if (!attr) return LuxStatus::Internal;
     // a block per CU, and as many as a power of two has
@@ -1093,10 +1103,11 @@ LuxStatus launch_as(Params& p, hipStream_t st) {
 
 template <int T, int DP, int RG, int KG, int BT, int NS>
 LuxStatus launch_page(Params& p, hipStream_t st) {
-    using A = Chunk<T, DP, RG, KG, BT, NS, true>;
+    using A = Chunk<T, DP, RG, KG, BT, NS, kPlain>;
+    if (p.a.page % A::LT != 0) return launch_as<T, DP, RG, KG, BT, NS, kLanes>(p, st);
     if constexpr (A::RS == DP * A::ES)
-        if (p.a.D == DP && p.a.softcap == 0.f && p.a.page % A::LT == 0) return launch_as<T, DP, RG, KG, BT, NS, true>(p, st);
-    return launch_as<T, DP, RG, KG, BT, NS, false>(p, st);
+        if (p.a.D == DP && p.a.softcap == 0.f) return launch_as<T, DP, RG, KG, BT, NS, kPlain>(p, st);
+    return launch_as<T, DP, RG, KG, BT, NS, kRuns>(p, st);
 }
 
 template <int T>
@@ -1122,11 +1133,15 @@ LuxStatus launch_t(const ChunkArgs& a, hipStream_t st) {
     const bool padded = (int64_t)a.T * a.G < 192 * (int64_t)a.R;
     if constexpr (T == DT_F32) {
         if (a.D <= 64) return few || padded ? launch_page<T, 64, 2, 4, 32, 2>(p, st) : launch_page<T, 64, 8, 1, 32, 3>(p, st);
+        if (a.D <= 96) return few || padded ? launch_page<T, 96, 4, 2, 32, 2>(p, st) : launch_page<T, 96, 8, 1, 32, 3>(p, st);
         if (a.D <= 128) return few || padded ? launch_page<T, 128, 4, 2, 32, 2>(p, st) : launch_page<T, 128, 8, 1, 32, 3>(p, st);
         return a.D <= 192 ? launch_page<T, 192, 4, 1, 32, 2>(p, st) : launch_page<T, 256, 4, 1, 32, 2>(p, st);
     } else if (a.D <= 64) {
         if (few) return launch_page<T, 64, 2, 4, 32, 2>(p, st);
         return padded ? launch_page<T, 64, 4, 2, 64, 2>(p, st) : launch_page<T, 64, 8, 1, 64, 3>(p, st);
+    } else if (a.D <= 96) {
+        if (few) return launch_page<T, 96, 2, 4, 32, 2>(p, st);
+        return padded ? launch_page<T, 96, 4, 2, 64, 2>(p, st) : launch_page<T, 96, 8, 1, 64, 3>(p, st);
     } else if (a.D <= 128) {
         if (few) return launch_page<T, 128, 2, 4, 32, 2>(p, st);
         return padded ? launch_page<T, 128, 4, 2, 64, 2>(p, st) : launch_page<T, 128, 8, 1, 64, 3>(p, st);
