@@ -58,9 +58,9 @@ extern "C" {
  * and the running statistics are fp32; with 16-bit types exp(s - max), rounded to
  * the type, enters the product with v.
  * head_dim: a multiple of 8, at most 256; heads a multiple of kv_heads;
- * num_pages * kv_heads * page_size, max_pages * page_size + tokens and the
- * tiles' work (tokens + 256 requests, times max_pages * page_size / 64) below
- * 2^31, 2^31 and 2^39; the caches start on 16 bytes.
+ * num_pages * kv_heads * page_size and max_pages * page_size + tokens below 2^31,
+ * and so is (tokens / n + requests) * (max_pages * page_size / 32 + 1), where n is
+ * 64 / (heads / kv_heads), at least 1; the caches start on 16 bytes.
  */
 typedef struct lux_paged_chunk_args {
     uint32_t struct_size;
@@ -92,8 +92,9 @@ typedef struct lux_paged_chunk_args {
  *             taken (for op_paged_copy, on every layer's cache); -1 otherwise
  * Where the list has no page left, dst keeps the full pages alone.  Where src's
  * page is none, so is dst's, and nothing is taken.  Other forks are left out.
- *   counts = {entry of free_pages after the last one taken, full pages shared,
- *             pages needed and not there, forks left out}
+ *   counts = {entry of free_pages after the last one taken, columns of full pages
+ *             that dsts got (of a page that is none, too), pages needed and not
+ *             there, forks left out}
  */
 typedef struct lux_paged_fork_args {
     uint32_t struct_size;
@@ -193,7 +194,8 @@ typedef struct lux_paged_copy_args {
 } lux_paged_copy_args;
 
 /*
- * Scores of a row of logits, x = scale * logits (scale > 0 and finite):
+ * Scores of a row of logits, x = scale * logits (scale > 0 and finite; x log2(e)
+ * of finite logits is finite in fp32):
  *   lse = log(sum_v exp(x_v));  logprobs = x[token] - lse, -infinity for a token
  *   outside [0, vocab);  entropy = lse - sum_v exp(x_v - lse) x_v, terms of
  *   probability 0 left out

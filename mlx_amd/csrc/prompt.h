@@ -22,7 +22,7 @@ struct ChunkArgs {
     float scale, softcap;
     int64_t q_row, out_row;
     DivBy div;
-    char* ws;  // kChunkPartBytes, or nullptr: no tile is split
+    char* ws;  // kChunkPartBytes
     int cus;
 };
 LuxStatus launch_paged_chunk(const ChunkArgs& a, hipStream_t st);

@@ -20,8 +20,11 @@ LuxBackendError op_paged_chunk_attention(LuxBackendContext* c, const lux_paged_c
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     const int64_t reach = (int64_t)p->max_pages * p->page_size;
     if (!dtype_ok(p->dtype) || p->head_dim % 8 || p->head_dim > 256 || row >= (1ll << 31) ||
-        !rows_ok(p->kv_heads, p->page_size, p->num_pages) || reach + p->tokens >= (1ll << 31) ||
-        ((int64_t)p->tokens + 256ll * p->requests) * (reach / 64 + 1) >= (1ll << 39))
+        !rows_ok(p->kv_heads, p->page_size, p->num_pages) || reach + p->tokens >= (1ll << 31))
+        return LUX_BACKEND_ERROR_NOT_SUPPORTED;
+    // the stages of all tiles for one head, of the smallest tiles and shortest stages
+    const int group = p->heads / p->kv_heads;
+    if ((p->tokens / (group < 64 ? 64 / group : 1) + (int64_t)p->requests) * (reach / 32 + 1) >= (1ll << 31))
         return LUX_BACKEND_ERROR_NOT_SUPPORTED;
     lxq::ChunkArgs a;
     Spans s;
