@@ -3,7 +3,8 @@
 //
 // With y = (x - r) c, c = scale log2 e and r near the row's maximum M:
 //   S = sum exp2(y), E = sum exp2(y) y, moved from r to M at the end
-//   lse = scale M + ln 2 log2 S,  H = ln 2 (log2 S - E / S)
+//   lse = scale M + ln 2 (log2 S + d E / S),  H = ln 2 (log2 S - E / S)
+// where c is d of itself below scale log2 e, by its rounding: a mean of y times d.
 // A thread keeps its own r, S and E and its largest logit.  Of 64 groups of threads
 // the k-th largest maximum is at most the row's k-th largest logit, so that the top
 // k lie in the few threads with a maximum from there on (24 logits on average for k
@@ -29,7 +30,7 @@ constexpr int kRoom = 1024;     // logits that are ranked
 constexpr int kMostParts = 64;
 // r c up to which (x - r) c is taken as x c - r c: the rounding of r c is at most 4
 constexpr float kFar = 0x1p27f;
-constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
+constexpr float kLn2 = 0.69314718055994531f;
 
 // order of logits: NaN above all, -0 as 0; 0 stands for no logit
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -59,7 +60,7 @@ __device__ __forceinline__ void move(float& s, float& e, float by) {  // by = (r
 struct Params {
     LogprobArgs a;
     int parts, len;  // of a row, logits of a part (a multiple of 8)
-    float c;
+    float c, d;
     Sums* sums;      // [rows, parts]
     uint64_t* tops;  // [rows, parts, top]
 };
@@ -102,11 +103,17 @@ struct Shared {
     uint16_t who[NT];
 };
 
+// lse - scale M
+__device__ __forceinline__ float log_of(const Params& p, const Sums& t) {
+    if (t.top == -INFINITY || t.top == INFINITY) return 0.f;
+    return fmaf(p.d, t.e / t.s, log2f(t.s)) * kLn2;
+}
 // the row's scores, from its sums and its top entries
-__device__ __forceinline__ void write_sums(const LogprobArgs& a, int r, const Sums& t, float x_tok, bool has_tok, float& log_sum) {
+__device__ __forceinline__ void write_sums(const Params& p, int r, const Sums& t, float x_tok, bool has_tok, float log_sum) {
+    const LogprobArgs& a = p.a;
     // NaN in the row, +infinity, nothing but -infinity, or as it should be
     const bool nan = t.top != t.top, none = t.top == -INFINITY, high = t.top == INFINITY;
-    log_sum = nan ? t.top : none || high ? 0.f : log2f(t.s) * kLn2;
+    if (nan) log_sum = t.top;
     const float lse = fmaf(a.scale, t.top, log_sum);
     if (a.lse) a.lse[r] = lse;
     if (a.entropy) a.entropy[r] = none ? 0.f : high || nan ? __uint_as_float(0x7fc00000u) : fmaf(-kLn2, t.e / t.s, log_sum);
@@ -303,10 +310,9 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
         __syncthreads();
         found = sh.count;
     }
-    float log_sum = 0.f;
+    const float log_sum = SPLIT ? 0.f : log_of(p, t);
     if (!SPLIT) {
-        if (tid == 0) write_sums(a, r, t, x_tok, has && want, log_sum);
-        else log_sum = t.top == -INFINITY || t.top == INFINITY ? 0.f : log2f(t.s) * kLn2;
+        if (tid == 0) write_sums(p, r, t, x_tok, has && want, log_sum);
     } else if (tid == 0) {
         p.sums[(int64_t)r * p.parts + part] = t;
     }
@@ -378,9 +384,8 @@ __global__ __launch_bounds__(NT) void logprobs_join_kernel(Params p, int first) 
     else move(s, e, (mine.top - t.top) * p.c);
     t.s = wave_sum(s);
     t.e = wave_sum(e);
-    float log_sum;
-    if (tid == 0) write_sums(a, r, t, x_tok, has, log_sum);
-    else log_sum = t.top == -INFINITY || t.top == INFINITY ? 0.f : log2f(t.s) * kLn2;
+    const float log_sum = log_of(p, t);
+    if (tid == 0) write_sums(p, r, t, x_tok, has, log_sum);
     if (a.top == 0) return;
     // a bound: the m-th largest of the parts' d-th entries, where m d is top or more
     const int d = (a.top + p.parts - 1) / p.parts, m = (a.top + d - 1) / d;
@@ -419,7 +424,9 @@ template <int T>
 LuxStatus launch_t(const LogprobArgs& a, hipStream_t st) {
     Params p = {};
     p.a = a;
-    p.c = a.scale * kLog2e;
+    const double c = (double)a.scale * 1.4426950408889634;
+    p.c = (float)c;
+    p.d = p.c > 0x1p-126f ? (float)(c / p.c - 1.) : 0.f;
     // two blocks per CU; parts of at least 4096 logits
     int parts = a.T > 0 ? 2 * a.cus / a.T : 1;
     if (parts > a.V / 4096) parts = a.V / 4096;
