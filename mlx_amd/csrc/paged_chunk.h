@@ -1027,12 +1027,12 @@ __global__ __launch_bounds__(512) void join_kernel(Params p) {
         for (int s0 = 0; s0 < cut.parts; s0 += 64) {
             const int n = cut.parts - s0 < 64 ? cut.parts - s0 : 64;
             constexpr int kB = 8;
-            float v[kB][NV];
+            float v[kB][NV];  // n is the wave's: as many loads as parts
             auto load = [&](int s) {
 #pragma unroll
                 for (int b = 0; b < kB; b++) {
-                    const int at = s + b < n ? s + b : n - 1;
-                    const float* src = p.part_o + ((int64_t)slot(w0, s0 + at) * A::ROWS + row) * DP + lane;
+                    if (s + b >= n) break;
+                    const float* src = p.part_o + ((int64_t)slot(w0, s0 + s + b) * A::ROWS + row) * DP + lane;
 #pragma unroll
                     for (int j = 0; j < NV; j++) v[b][j] = src[64 * j];
                 }
@@ -1054,9 +1054,10 @@ __global__ __launch_bounds__(512) void join_kernel(Params p) {
                 if (s > 0) load(s);
 #pragma unroll
                 for (int b = 0; b < kB; b++) {
-                    const float f = lane_f(wgt, s + b < n ? s + b : n - 1);
+                    if (s + b >= n) break;
+                    const float f = lane_f(wgt, s + b);
 #pragma unroll
-                    for (int j = 0; j < NV; j++) acc[j] = s + b < n ? fmaf(f, v[b][j], acc[j]) : acc[j];
+                    for (int j = 0; j < NV; j++) acc[j] = fmaf(f, v[b][j], acc[j]);
                 }
             }
         }
@@ -1097,7 +1098,7 @@ LuxStatus launch_as(Params& p, hipStream_t st) {
     p.part_ml = p.part_o + (size_t)2 * p.P * rows * DP;
     p.cuts = reinterpret_cast<Cut*>(p.part_ml + (size_t)2 * p.P * rows * 2);
     hipLaunchKernelGGL(main, dim3(p.P), dim3(A::NT), A::kLds, st, p);
-    hipLaunchKernelGGL(join, dim3(p.P), dim3(512), 0, st, p);
+    hipLaunchKernelGGL(join, dim3(4 * p.P), dim3(512), 0, st, p);
     return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
 }
 
