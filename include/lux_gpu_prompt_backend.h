@@ -24,7 +24,9 @@
  * free list is the plan's: free_pages from entry free_head[0] on (0 where it is
  * negative, free_count where above); each op writes the next head as counts[0].
  * Counts and free_head of one call are distinct buffers.  A request's table
- * entries behind ceil(its length / page_size) mean nothing.
+ * entries behind ceil(its length / page_size) mean nothing.  Forks, releases and
+ * compactions take up to 2^22 pages, 2^20 forks, and products of num_pages, or
+ * max_pages, and page_size, and of requests and max_pages below 2^31 - 1.
  */
 #ifndef LUX_GPU_PROMPT_BACKEND_H
 #define LUX_GPU_PROMPT_BACKEND_H
@@ -49,7 +51,8 @@ extern "C" {
  * positions t of [max(0, p + 1 - window), min(p + 1, n)), n = kv_lens[r] cut to
  * [0, max_pages * page_size] (window 0: from 0 on), but those whose page is none:
  *   s_t = scale * q . k_t, or softcap * tanh(scale * q . k_t / softcap) where
- *   softcap > 0 (2^-100 to 2^100; others but 0 are INVALID_ARGUMENT);
+ *   softcap > 0 (2^-100 to 2^100; others but 0 and a scale that is not finite are
+ *   INVALID_ARGUMENT);
  *   out = sum_t exp(s_t) v_t / sum_t exp(s_t);  lse = log(sum_t exp(s_t))
  * A row with no position gives out = 0 and lse = -infinity.  Places that a row
  * does not see are never part of its result, whatever they hold; an infinite

@@ -107,7 +107,7 @@ __device__ __forceinline__ Tile tile_of(const Params& p, int r, int tile) {
     const int cap = a.pool > 0 ? a.columns * a.page : 0;
     const int s0 = clamp(a.starts[r], 0, a.T), s1 = clamp(a.starts[r + 1], s0, a.T), i0 = tile * p.TB;
     t.first = s0 + i0;
-    t.m = clamp(s1 - s0 - i0, 0, p.TB);
+    t.m = tile < 0 ? 0 : clamp(s1 - s0 - i0, 0, p.TB);  // below 0: places of rows before the first request's
     t.pos = clamp(a.seq[r], 0, a.columns * a.page) + i0;
     t.n = clamp(a.lens[r], 0, cap);
     t.end = t.pos + t.m < t.n ? t.pos + t.m : t.n;

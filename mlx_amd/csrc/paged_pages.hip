@@ -237,7 +237,8 @@ __device__ __forceinline__ void write_kept(const ReleaseArgs& a, int r) {
 }
 
 // four pages of a thread: their counts, how many of them go back (a count below 0),
-// and their entries of the list from `to` on (below 0: lost)
+// and their entries of the list from `to` on (below 0: lost; none from `head` on,
+// whatever counts the caller had)
 struct Four {
     int p, v[4];
     __device__ __forceinline__ Four(const ReleaseArgs& a, int run) : p(run * kRun + 4 * (int)threadIdx.x) {
@@ -245,11 +246,11 @@ struct Four {
         for (int i = 0; i < 4; i++) v[i] = p + i < a.pool ? load_now(a.shares + p + i) : 0;
     }
     __device__ __forceinline__ int back() const { return (v[0] < 0) + (v[1] < 0) + (v[2] < 0) + (v[3] < 0); }
-    __device__ __forceinline__ void give(const ReleaseArgs& a, int to) const {
+    __device__ __forceinline__ void give(const ReleaseArgs& a, int to, int head) const {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (v[i] < 0) {
-                if (to >= 0) a.free_pages[to] = p + i;
+                if (to >= 0 && to < head) a.free_pages[to] = p + i;
                 to++;
                 a.shares[p + i] = 0;
             }
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(1024) void release_kernel(ReleaseArgs a) {
         const Four pages(a, run);
         int back;
         const int to = at + block_sum<16>(pages.back(), back, part);
-        pages.give(a, to);
+        pages.give(a, to, head);
         at += back;
     }
     if (tid == 0) release_counts(a, head, all[0], all[1]);
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(1024) void release_list_kernel(ReleaseArgs a, int d
         v[2] += i < (int)blockIdx.x ? n : 0;
     }
     block_sums<16, 4>(v, all, parts);
-    pages.give(a, head - all[1] + all[2] + v[0]);
+    pages.give(a, head - all[1] + all[2] + v[0], head);
     if (blockIdx.x == 0 && tid == 0) release_counts(a, head, all[1], all[3]);
 }
 

@@ -12,7 +12,7 @@ LuxBackendError op_paged_chunk_attention(LuxBackendContext* c, const lux_paged_c
     if (!ctx || !p || p->struct_size != sizeof(*p)) return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     if (p->requests < 0 || p->tokens < 0 || p->heads <= 0 ||
         !cache_ok(p->kv_heads, p->head_dim, p->page_size, p->num_pages) || p->heads % p->kv_heads || p->max_pages <= 0 ||
-        p->window < 0 || !cap_ok(p->softcap))
+        p->window < 0 || !cap_ok(p->softcap) || !(p->scale - p->scale == 0.f))
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     const int64_t row = (int64_t)p->heads * p->head_dim;
     if (!stride_ok(p->q_row_stride, row) || !stride_ok(p->out_row_stride, row) || !offset_ok(p->q_offset) ||
