@@ -76,6 +76,8 @@ struct LogprobArgs {
     int64_t row;
     char* ws;
     size_t ws_bytes;
+    uint32_t* count;  // `counts` counters, zero between launches
+    int counts;
     int cus;
 };
 LuxStatus launch_token_logprobs(const LogprobArgs& a, hipStream_t st);

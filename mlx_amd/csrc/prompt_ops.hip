@@ -218,6 +218,8 @@ LuxBackendError op_token_logprobs(LuxBackendContext* c, const lux_token_logprobs
     size_t n;
     a.ws = reinterpret_cast<char*>(words(ctx, n));
     a.ws_bytes = n * 4;
+    a.count = static_cast<uint32_t*>(ctx->counts);
+    a.counts = ctx->counts ? kCountWords : 0;
     a.cus = ctx->compute_units;
     if (hipSetDevice(ctx->device) != hipSuccess) return LUX_BACKEND_ERROR_DEVICE_LOST;
     return map_status(lxq::launch_token_logprobs(a, ctx->stream));

@@ -10,7 +10,7 @@
 // k lie in the few threads with a maximum from there on (24 logits on average for k
 // = 20): these are read again, out of the cache, and ranked by counting.
 //
-// Few rows are cut into parts, a block each, which a second launch joins.
+// Few rows are cut into parts, a block each; the last block of a row joins them.
 //
 // Rows in which that goes wrong (more logits from the bound on than are ranked, as
 // where most are -infinity, or NaN) are finished by a search, one largest logit
@@ -97,11 +97,34 @@ __device__ __forceinline__ uint64_t wave_most(uint64_t v) {
 struct Shared {
     uint64_t list[kRoom];
     uint64_t most[NW];
+    uint64_t lows[kMostParts];
+    uint64_t bound;
     uint32_t groups[kGroups];
     float part[NW][3];
-    int count, odd, threads;
+    int count, odd, threads, last;
     uint16_t who[NT];
 };
+
+// The block: at(i, rank) for each of the n entries of v (in LDS), rank: how many
+// come before it, the larger first, then the lower place.  Eight threads share an
+// entry's comparisons, which would be a chain of reads for one.
+template <class V, class F>
+__device__ __forceinline__ void ranks(const V* v, int n, F at) {
+    const int part = threadIdx.x & 7;
+    for (int i0 = 0; i0 < n; i0 += NT / 8) {
+        const int i = i0 + (int)(threadIdx.x >> 3);
+        const V mine = v[i < n ? i : 0];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = part; j < n; j += 8) {
+            const V o = v[j];
+            rank += o > mine || (o == mine && j < i);
+        }
+#pragma unroll
+        for (int k = 1; k < 8; k *= 2) rank += __shfl_xor(rank, k);
+        if (part == 0 && i < n) at(i, rank);
+    }
+}
 
 // lse - scale M
 __device__ __forceinline__ float log_of(const Params& p, const Sums& t) {
@@ -125,7 +148,79 @@ __device__ __forceinline__ float top_logprob(const LogprobArgs& a, const Sums& t
     return (x - t.top) * a.scale - log_sum;
 }
 
-// one block: part blockIdx of row; SPLIT: its results go to the workspace
+// what other blocks read: written through, read from beyond the block's own caches
+template <class V>
+__device__ __forceinline__ void put_out(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <class V>
+__device__ __forceinline__ V look(const V* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// a block, behind the last part: the row's scores from its parts' sums and entries
+__device__ __forceinline__ void join_parts(const Params& p, int r, float x_tok, bool has, Shared& sh) {
+    uint64_t* list = sh.list;
+    int& count = sh.count;
+    const LogprobArgs& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const uint64_t* tops = p.tops + (int64_t)r * p.parts * a.top;
+    if (tid == 0) count = 0;
+    const int entries = p.parts * a.top;
+    const uint64_t first_entry = tid < entries ? look(tops + tid) : 0, second_entry = tid + NT < entries ? look(tops + tid + NT) : 0;
+    // a bound: the m-th largest of the parts' d-th entries, where m d is top or more
+    const int d = (a.top + p.parts - 1) / p.parts, m = d ? (a.top + d - 1) / d : 0;
+    const uint64_t low_mine = a.top > 0 && tid < p.parts ? look(tops + tid * a.top + d - 1) : 0;
+    // each wave for itself
+    const Sums* its = p.sums + (int64_t)r * p.parts + lane;
+    const Sums mine = lane < p.parts ? Sums{look(&its->top), look(&its->s), look(&its->e)} : Sums{-INFINITY, 0.f, 0.f};
+    uint32_t k = lane < p.parts ? key_of(mine.top) : 0u;
+    uint32_t most = k;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+        const uint32_t o = (uint32_t)__shfl_xor((int)most, i);
+        most = most > o ? most : o;
+    }
+    Sums t = {value_of(most), 0.f, 0.f};
+    float s = mine.s, e = mine.e;
+    if (!(fabsf(mine.top) < INFINITY) || !(fabsf(t.top) < INFINITY)) s = e = 0.f;
+    else move(s, e, (mine.top - t.top) * p.c);
+    t.s = wave_sum(s);
+    t.e = wave_sum(e);
+    const float log_sum = log_of(p, t);
+    if (tid == 0) write_sums(p, r, t, x_tok, has, log_sum);
+    if (a.top == 0) return;
+    if (tid < p.parts) sh.lows[tid] = low_mine;
+    __syncthreads();
+    ranks(sh.lows, p.parts, [&](int i, int rank) {
+        if (rank == m - 1) sh.bound = sh.lows[i];
+    });
+    __syncthreads();
+    const uint64_t low = sh.bound;
+    for (int i = tid; i < entries; i += NT) {
+        const uint64_t x = i == tid ? first_entry : i == tid + NT ? second_entry : look(tops + i);
+        if (x >= low && x != 0) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kRoom) list[at] = x;
+        }
+    }
+    __syncthreads();
+    const int found = count;
+    auto write = [&](int rank, uint64_t x) {
+        if (rank >= a.top) return;
+        if (a.top_ids) a.top_ids[(int64_t)r * a.top + rank] = place_of(x);
+        if (a.top_lp) a.top_lp[(int64_t)r * a.top + rank] = top_logprob(a, t, value_of((uint32_t)(x >> 32)), log_sum);
+    };
+    if (found <= kRoom) {
+        ranks(list, found, [&](int i, int rank) { write(rank, list[i]); });
+        return;
+    }
+    for (int i = tid; i < entries; i += NT) {
+        const uint64_t x = look(tops + i);
+        int rank = 0;
+        for (int j = 0; j < entries; j++) rank += look(tops + j) > x;
+        if (x != 0) write(rank, x);
+    }
+}
+
+// one block: part blockIdx of row; SPLIT: its results go to the workspace, and the
+// last block of the row joins them
 template <int T, bool SPLIT>
 __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
     constexpr int E = T == DT_F32 ? 4 : 8;
@@ -136,10 +231,9 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
     const int from = part * p.len, to = SPLIT && from + p.len < a.V ? from + p.len : a.V, n = to > from ? to - from : 0;
     const char* base = static_cast<const char*>(a.logits) + ((int64_t)r * a.row + from) * (T == DT_F32 ? 4 : 2);
     const int vectors = n >= NT * E ? n / E : 0;  // fewer logits: one by one, so that all threads have some
-    const bool want = !SPLIT && a.tokens && a.logprobs;
-    const int token = want ? a.tokens[r] : -1;
+    const int token = a.tokens && a.logprobs ? a.tokens[r] : -1;
     const bool has = (uint32_t)token < (uint32_t)a.V;
-    const float x_tok = has ? logit<T>(base, token) : 0.f;
+    const float x_tok = has ? logit<T>(static_cast<const char*>(a.logits) + (int64_t)r * a.row * (T == DT_F32 ? 4 : 2), token) : 0.f;
     if (tid == 0) sh.count = sh.odd = sh.threads = 0;
 
     // the thread's vectors tid, tid + NT, ..., and logits behind the vectors likewise
@@ -179,18 +273,16 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
             take(x, E);
         }
     }
-    {
-        u4 d[kU - 1];
+    u4 rest[kU - 1];
 #pragma unroll
-        for (int k = 0; k < kU - 1; k++)
-            if (v + k * NT < vectors) d[k] = *reinterpret_cast<const u4h*>(base + (int64_t)(v + k * NT) * 16);
+    for (int k = 0; k < kU - 1; k++)
+        if (v + k * NT < vectors) rest[k] = *reinterpret_cast<const u4h*>(base + (int64_t)(v + k * NT) * 16);
 #pragma unroll
-        for (int k = 0; k < kU - 1; k++) {
-            if (v + k * NT >= vectors) break;
-            float x[E];
-            unpack<T>(d[k], x);
-            take(x, E);
-        }
+    for (int k = 0; k < kU - 1; k++) {
+        if (v + k * NT >= vectors) break;
+        float x[E];
+        unpack<T>(rest[k], x);
+        take(x, E);
     }
     const int behind = vectors * E;
     for (int i = behind + tid; i < n; i += NT) {
@@ -229,19 +321,13 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
         sh.part[w][1] = s;
         sh.part[w][2] = e;
     }
-    // the bound: the k-th largest of the groups' maxima, each wave for itself
-    uint32_t bound = 0;
-    if (a.top > 0) {
-        const uint32_t mine = sh.groups[lane];
-        int rank = 0;
-#pragma unroll
-        for (int i = 0; i < kGroups; i++) {
-            const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
-            rank += o > mine || (o == mine && i < lane);
-        }
-        bound = (uint32_t)__builtin_amdgcn_readlane((int)mine, __builtin_ctzll(__ballot(rank == a.top - 1)));
-    }
+    // the bound: the k-th largest of the groups' maxima
+    if (a.top > 0)
+        ranks(sh.groups, kGroups, [&](int i, int rank) {
+            if (rank == a.top - 1) sh.bound = sh.groups[i];
+        });
     __syncthreads();
+    const uint32_t bound = (uint32_t)sh.bound;
     Sums t = {all, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NW; i++) {
@@ -278,26 +364,35 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
 
     int found = 0;
     if (a.top > 0 && !nan) {
-        // the threads that have logits from the bound on, then those logits: a thread
-        // reads one vector of one of them
-        if (any && key_of(top) >= bound) {
-            const int at = atomicAdd(&sh.threads, 1);
-            sh.who[at] = (uint16_t)tid;
-        }
-        __syncthreads();
-        const int each = (vectors + NT - 1) / NT, items = sh.threads * each;
-        for (int x0 = tid; x0 < items; x0 += NT) {
-            const int which = (int)((uint32_t)x0 / (uint32_t)each), i = sh.who[which] + (x0 - which * each) * NT;
-            if (i >= vectors) continue;
+        auto list = [&](const u4& v, int i) {
             float x[E];
-            unpack<T>(*reinterpret_cast<const u4h*>(base + (int64_t)i * 16), x);
+            unpack<T>(v, x);
+            int some = 0;
+#pragma unroll
+            for (int j = 0; j < E; j++) some += key_of(x[j]) >= bound;
+            if (some == 0) return;
+            int at = atomicAdd(&sh.count, some);
 #pragma unroll
             for (int j = 0; j < E; j++) {
                 const uint32_t k = key_of(x[j]);
-                if (k >= bound) {
-                    const int at = atomicAdd(&sh.count, 1);
-                    if (at < kRoom) sh.list[at] = entry_of(k, from + i * E + j);
-                }
+                if (k >= bound && at < kRoom) sh.list[at] = entry_of(k, from + i * E + j);
+                at += k >= bound;
+            }
+        };
+        const bool mine = any && key_of(top) >= bound;
+        if (vectors <= (kU - 1) * NT) {  // they are still in registers
+#pragma unroll
+            for (int k = 0; k < kU - 1; k++)
+                if (mine && tid + k * NT < vectors) list(rest[k], tid + k * NT);
+        } else {
+            // the threads that have logits from the bound on, then those logits: a
+            // thread reads one vector of one of them
+            if (mine) sh.who[atomicAdd(&sh.threads, 1)] = (uint16_t)tid;
+            __syncthreads();
+            const int each = (vectors + NT - 1) / NT, items = sh.threads * each;
+            for (int x0 = tid; x0 < items; x0 += NT) {
+                const int which = (int)((uint32_t)x0 / (uint32_t)each), i = sh.who[which] + (x0 - which * each) * NT;
+                if (i < vectors) list(*reinterpret_cast<const u4h*>(base + (int64_t)i * 16), i);
             }
         }
         for (int i = behind + tid; i < n; i += NT) {
@@ -312,111 +407,57 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
     }
     const float log_sum = SPLIT ? 0.f : log_of(p, t);
     if (!SPLIT) {
-        if (tid == 0) write_sums(p, r, t, x_tok, has && want, log_sum);
+        if (tid == 0) write_sums(p, r, t, x_tok, has, log_sum);
     } else if (tid == 0) {
-        p.sums[(int64_t)r * p.parts + part] = t;
+        Sums* its = p.sums + (int64_t)r * p.parts + part;
+        put_out(&its->top, t.top);
+        put_out(&its->s, t.s);
+        put_out(&its->e, t.e);
     }
     auto put = [&](int rank, uint64_t entry) {
         if (SPLIT) {
-            p.tops[((int64_t)r * p.parts + part) * a.top + rank] = entry;
+            put_out(p.tops + ((int64_t)r * p.parts + part) * a.top + rank, entry);
         } else {
             if (a.top_ids) a.top_ids[(int64_t)r * a.top + rank] = place_of(entry);
             if (a.top_lp) a.top_lp[(int64_t)r * a.top + rank] = top_logprob(a, t, value_of((uint32_t)(entry >> 32)), log_sum);
         }
     };
-    if (a.top == 0) return;
-    if (!nan && found <= kRoom) {
-        for (int i = tid; i < found; i += NT) {
-            const uint64_t mine = sh.list[i];
-            int rank = 0;
-            for (int j = 0; j < found; j++) rank += sh.list[j] > mine;
-            if (rank < a.top) put(rank, mine);
-        }
+    if (a.top > 0 && !nan && found <= kRoom) {
+        ranks(sh.list, found, [&](int i, int rank) {
+            if (rank < a.top) put(rank, sh.list[i]);
+        });
         // a part with fewer logits than that
         if (SPLIT && tid >= found && tid < a.top) put(tid, 0);
-        return;
-    }
-    // one after the other: the largest entry below the last one
-    uint64_t last = ~0ull;
-    for (int k = 0; k < a.top; k++) {
-        uint64_t best = 0;
-        for (int i = tid; i < n; i += NT) {
-            const uint64_t x = entry_of(key_of(logit<T>(base, i)), from + i);
-            if (x < last && x > best) best = x;
-        }
-        best = wave_most(best);
-        if (lane == 0) sh.most[w] = best;
-        __syncthreads();
-        last = sh.most[0];
+    } else if (a.top > 0) {
+        // one after the other: the largest entry below the last one
+        uint64_t last = ~0ull;
+        for (int k = 0; k < a.top; k++) {
+            uint64_t best = 0;
+            for (int i = tid; i < n; i += NT) {
+                const uint64_t x = entry_of(key_of(logit<T>(base, i)), from + i);
+                if (x < last && x > best) best = x;
+            }
+            best = wave_most(best);
+            if (lane == 0) sh.most[w] = best;
+            __syncthreads();
+            last = sh.most[0];
 #pragma unroll
-        for (int i = 1; i < NW; i++) last = sh.most[i] > last ? sh.most[i] : last;
-        if (tid == 0) put(k, last);
+            for (int i = 1; i < NW; i++) last = sh.most[i] > last ? sh.most[i] : last;
+            if (tid == 0) put(k, last);
+            __syncthreads();
+        }
+    }
+    if constexpr (SPLIT) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the wave's part of the results is out
         __syncthreads();
-    }
-}
-
-// a block per row: its parts' sums and entries
-template <int T>
-__global__ __launch_bounds__(NT) void logprobs_join_kernel(Params p, int first) {
-    __shared__ uint64_t list[kRoom];
-    __shared__ int count;
-    const LogprobArgs& a = p.a;
-    const int tid = threadIdx.x, lane = tid & 63, r = first + (int)blockIdx.x;
-    const int token = a.tokens && a.logprobs ? a.tokens[r] : -1;
-    const bool has = (uint32_t)token < (uint32_t)a.V;
-    const float x_tok = has ? logit<T>(static_cast<const char*>(a.logits) + (int64_t)r * a.row * (T == DT_F32 ? 4 : 2), token) : 0.f;
-    const uint64_t* tops = p.tops + (int64_t)r * p.parts * a.top;
-    if (tid == 0) count = 0;
-    const int entries = p.parts * a.top;
-    const uint64_t first_entry = tid < entries ? tops[tid] : 0, second_entry = tid + NT < entries ? tops[tid + NT] : 0;
-    // each wave for itself
-    const Sums mine = lane < p.parts ? p.sums[(int64_t)r * p.parts + lane] : Sums{-INFINITY, 0.f, 0.f};
-    uint32_t k = lane < p.parts ? key_of(mine.top) : 0u;
-    uint32_t most = k;
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) {
-        const uint32_t o = (uint32_t)__shfl_xor((int)most, i);
-        most = most > o ? most : o;
-    }
-    Sums t = {value_of(most), 0.f, 0.f};
-    float s = mine.s, e = mine.e;
-    if (!(fabsf(mine.top) < INFINITY) || !(fabsf(t.top) < INFINITY)) s = e = 0.f;
-    else move(s, e, (mine.top - t.top) * p.c);
-    t.s = wave_sum(s);
-    t.e = wave_sum(e);
-    const float log_sum = log_of(p, t);
-    if (tid == 0) write_sums(p, r, t, x_tok, has, log_sum);
-    if (a.top == 0) return;
-    // a bound: the m-th largest of the parts' d-th entries, where m d is top or more
-    const int d = (a.top + p.parts - 1) / p.parts, m = (a.top + d - 1) / d;
-    const uint64_t low_mine = lane < p.parts ? tops[lane * a.top + d - 1] : 0;
-    int rank_low = 0;
-    for (int i = 0; i < p.parts; i++) {
-        const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(low_mine >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)low_mine, i);
-        rank_low += o > low_mine || (o == low_mine && i < lane);
-    }
-    const int holder = __builtin_ctzll(__ballot(lane < p.parts && rank_low == m - 1));
-    const uint64_t low = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(low_mine >> 32), holder) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)low_mine, holder);
-    __syncthreads();
-    for (int i = tid; i < entries; i += NT) {
-        const uint64_t x = i == tid ? first_entry : i == tid + NT ? second_entry : tops[i];
-        if (x >= low && x != 0) {
-            const int at = atomicAdd(&count, 1);
-            if (at < kRoom) list[at] = x;
+        if (tid == 0) {
+            // the last block of the row leaves the counter at 0
+            uint32_t* c = p.a.count + r;
+            sh.last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(p.parts - 1);
+            if (sh.last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-    }
-    __syncthreads();
-    const int found = count;
-    const uint64_t* from = found <= kRoom ? list : tops;
-    const int n = found <= kRoom ? found : entries;
-    for (int i = tid; i < n; i += NT) {
-        const uint64_t x = from[i];
-        int rank = 0;
-        for (int j = 0; j < n; j++) rank += from[j] > x;
-        if (rank < a.top && x != 0) {
-            if (a.top_ids) a.top_ids[(int64_t)r * a.top + rank] = place_of(x);
-            if (a.top_lp) a.top_lp[(int64_t)r * a.top + rank] = top_logprob(a, t, value_of((uint32_t)(x >> 32)), log_sum);
-        }
+        __syncthreads();
+        if (sh.last) join_parts(p, r, x_tok, has, sh);
     }
 }
 
@@ -432,7 +473,7 @@ LuxStatus launch_t(const LogprobArgs& a, hipStream_t st) {
     if (parts > a.V / 4096) parts = a.V / 4096;
     if (parts > kMostParts) parts = kMostParts;
     const size_t one = sizeof(Sums) + (size_t)a.top * 8;
-    if (parts > 1 && (!a.ws || (size_t)a.T * parts * one > a.ws_bytes)) parts = 1;
+    if (parts > 1 && (!a.ws || (size_t)a.T * parts * one > a.ws_bytes || a.T > a.counts)) parts = 1;
     if (parts <= 1) {
         p.parts = 1;
         p.len = a.V;
@@ -445,7 +486,6 @@ LuxStatus launch_t(const LogprobArgs& a, hipStream_t st) {
         p.tops = reinterpret_cast<uint64_t*>(a.ws);
         p.sums = reinterpret_cast<Sums*>(a.ws + (size_t)a.T * p.parts * a.top * 8);
         hipLaunchKernelGGL((logprobs_kernel<T, true>), dim3(a.T * p.parts), dim3(NT), 0, st, p, 0);
-        hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3(a.T), dim3(NT), 0, st, p, 0);
     }
     return hipGetLastError() == hipSuccess ? LuxStatus::Ok : LuxStatus::Internal;
 }
