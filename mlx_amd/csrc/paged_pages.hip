@@ -126,10 +126,16 @@ __global__ __launch_bounds__(1024) void fork_few_kernel(ForkArgs a) {
     made = made && has <= 0;
     dsts[f] = made ? d : -1;
     __syncthreads();
-    for (int g = 0; g < a.F; g += 4) {
-        const int4 x = *reinterpret_cast<const int4*>(dsts + g);
-        if ((g < f && x.x == d) || (g + 1 < f && x.y == d) || (g + 2 < f && x.z == d) || (g + 3 < f && x.w == d)) made = false;
+    // the forks before the wave's last one, without branches (which took 20 us for 224 forks)
+    const int end = __builtin_amdgcn_readfirstlane(f < a.F ? f + 64 : 0);
+    int twice = 0;
+#pragma unroll 4
+    for (int g = 0; g < end; g += 4) {
+        const u4 x = *reinterpret_cast<const u4*>(dsts + g);
+#pragma unroll
+        for (int i = 0; i < 4; i++) twice |= (g + i < f) & ((int)x[i] == d);
     }
+    made = made && !twice;
     const int n = made ? cut(held, cap) : -1, full = made ? div_by(n, a.div) : 0;
     const int last = n > full * a.page ? a.table[(int64_t)s * a.columns + full] : -1;
     if constexpr (ALL) {
