@@ -28,8 +28,8 @@
 // takes a run of ranges, so that its L2 holds the keys that its blocks share.
 //
 // What bounds it, and what it measured (32 heads on 8 of 128 channels, bf16):
-//   16384 tokens of one request: 2.50 ms, 880 TFLOP/s.  A stage of 64 tokens costs a
-//     wave 64 MFMAs of 32 cycles, 57 % of 3600 cycles; the rest is the softmax, and
+//   16384 tokens of one request: 2.50 ms, 880 TFLOP/s.  A stage of 64 tokens costs the
+//     two waves of a SIMD 64 MFMAs of 32 cycles, 57 % of 3600 cycles; the rest is the softmax, and
 //     at that rate the card's power holds the clock near 1.5 GHz (a large product of
 //     the library reaches 1110 to 1270 TFLOP/s).  The loop of whole, unmasked stages
 //     (kPlain, kRuns) brought 2.74 to 2.50: rows of the table looked up for 64 stages

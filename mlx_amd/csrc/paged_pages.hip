@@ -7,8 +7,8 @@
 // calls give equal results.  What bounds them is the number of launches and of trips
 // to memory in a row, so that each loads as much as it can before it waits: 64
 // requests of up to 256 pages given back in 10.5 us (three launches), 2048 of up to
-// 128 in 12.4, 24 forks with their copies and the losers' release in 17.6, a pool of
-// 1500 pages compacted in 4.9 and its pages copied in 6.5.  The copies are bound by
+// 128 in 12.4, 24 forks with their copies and the losers' release in 17.6, 37 requests of up to
+// 42 pages compacted in 4.9 and the pages copied in 6.5.  The copies are bound by
 // HBM: 0.87 GB read and written in 333 us, 5.2 TB/s.
 #include "serving_device.h"
 #include "prompt.h"
