@@ -25,8 +25,9 @@ struct HipContext {
     // launches on ws so far: each GEMM launch gets the next number as its
     // epoch (the split tiles meet by it; never 0)
     uint32_t epoch = 0;
-    // arrival counters of the attention's split pairs (three per range), zero
-    // between launches; without them the attention is not split
+    // arrival counters of the attention's split pairs (three per range) and of the
+    // parts of a row of logits (one per row), zero
+    // between launches; without them neither is split
     void* counts = nullptr;
     // partial results of the chunk attention's split tiles; like ws, used only
     // by work on `stream`
