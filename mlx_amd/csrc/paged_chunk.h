@@ -497,10 +497,11 @@ struct Chunk {
         for (int b = 0; b < NB; b++) x.s[b] = mfma<T>(f.k[k % AK][b], q[k], x.s[b]);
         if (k + AK < NK) read_k(f.k[k % AK], at, k + AK);
     }
-    __device__ __forceinline__ void scores(Scores& x, Ahead& f, uint32_t at) const {
+    __device__ __forceinline__ void scores(Scores& x, Ahead& f, uint32_t at, int dim) const {
         clear(x);
 #pragma unroll
         for (int k = 0; k < NK; k++) {
+            if (!EASY && k > 0 && 2 * k * E >= dim) break;  // nothing but padding from here on
             score(x, f, at, k);
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -760,7 +761,7 @@ struct Chunk {
                     Ahead f;
                     const uint32_t kat = key_at(here), vat = value_at(here);
                     begin(f, kat);
-                    scores(x, f, kat);
+                    scores(x, f, kat, a.D);
                     if (!EASY && a.softcap > 0.f) limit(p, x);
                     if (holes || tb < lo1 || tb + BT > hi0) mask(a, x, t, r, tb, holes);
                     follow(x, c);
@@ -788,7 +789,7 @@ struct Chunk {
                     next_rows(a, t, r, hk, first_tok, j + L);
                     fill_whole<false>(a, behind);
                     fill_whole<true>(a, behind);
-                    scores(x, f, kat);
+                    scores(x, f, kat, a.D);
                     if (!EASY && a.softcap > 0.f) limit(p, x);
                     follow(x, c);
                     begin_values(f, vat);
@@ -1121,7 +1122,7 @@ LuxStatus launch_as(Params& p, hipStream_t st) {
 
 template <int T, int DP, int RG, int KG, int BT, int NS>
 LuxStatus launch_page(Params& p, hipStream_t st) {
-    using A = Chunk<T, DP, RG, KG, BT, NS, kPlain>;
+    using A = Chunk<T, DP, RG, KG, BT, NS, kRuns>;
     if (p.a.page % A::LT != 0) return launch_as<T, DP, RG, KG, BT, NS, kLanes>(p, st);
     if constexpr (A::RS == DP * A::ES)
         if (p.a.D == DP && p.a.softcap == 0.f) return launch_as<T, DP, RG, KG, BT, NS, kPlain>(p, st);
@@ -1149,6 +1150,10 @@ LuxStatus launch_t(const ChunkArgs& a, hipStream_t st) {
     // of up to 512 among 64 requests 260 us, against 313 with wide tiles and 288 with
     // narrow ones; 16384 tokens of one request 3.1 ms against 2.5.
     const bool padded = (int64_t)a.T * a.G < 192 * (int64_t)a.R;
+    // 192 channels: eight waves and stages of 32 tokens (8192 tokens on 2048, bf16: 940
+    // TFLOP/s; four waves and stages of 64 tokens 651, as one wave per SIMD leaves the
+    // matrix cores idle in its softmax).  256 channels do not leave the registers for
+    // a second wave: 817.
     if constexpr (T == DT_F32) {
         if (a.D <= 64) return few || padded ? launch_page<T, 64, 2, 4, 32, 2>(p, st) : launch_page<T, 64, 8, 1, 32, 3>(p, st);
         if (a.D <= 96) return few || padded ? launch_page<T, 96, 4, 2, 32, 2>(p, st) : launch_page<T, 96, 8, 1, 32, 3>(p, st);
@@ -1164,7 +1169,7 @@ LuxStatus launch_t(const ChunkArgs& a, hipStream_t st) {
         if (few) return launch_page<T, 128, 2, 4, 32, 2>(p, st);
         return padded ? launch_page<T, 128, 4, 2, 64, 2>(p, st) : launch_page<T, 128, 8, 1, 64, 3>(p, st);
     } else if (a.D <= 192) {
-        return few || padded ? launch_page<T, 192, 2, 2, 32, 2>(p, st) : launch_page<T, 192, 4, 1, 64, 2>(p, st);
+        return few || padded ? launch_page<T, 192, 2, 2, 32, 2>(p, st) : launch_page<T, 192, 8, 1, 32, 2>(p, st);
     } else {
         return few || padded ? launch_page<T, 256, 2, 2, 32, 2>(p, st) : launch_page<T, 256, 4, 1, 64, 2>(p, st);
     }

@@ -11,7 +11,7 @@ namespace lxq {
 // to 256 rows of 128 channels or 128 of 256 and their maxima and sums; and a
 // record per range
 constexpr int kChunkRanges = 256;
-constexpr size_t kChunkPartBytes = (size_t)kChunkRanges * (2 * 256 * (128 + 2) * 4 + 32);
+constexpr size_t kChunkPartBytes = (size_t)kChunkRanges * (2 * 256 * (192 + 2) * 4 + 32);
 
 struct ChunkArgs {
     const void *q, *kc, *vc;
