@@ -45,6 +45,7 @@
 #pragma once
 #include <type_traits>
 
+#include "chunk_places.h"
 #include "prompt.h"
 #include "serving_device.h"
 
@@ -63,7 +64,6 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 constexpr float kLowest = -0x1.fffffep127f;  // the maximum of no score: no finite score is below
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 constexpr float kLeast = 0x1p-126f;
-constexpr int kLeastPiece = 2;
 
 // a tile that starts in a range and ends behind it: its parts, tokens and heads
 struct Cut {
@@ -103,15 +103,7 @@ __device__ __forceinline__ int afresh(int v) {
     asm volatile("" : "+v"(v));
     return v;
 }
-__device__ __forceinline__ int clamp(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-// rows and tokens of a tile
-struct Tile {
-    int first, m;    // first new token (row of q), tokens
-    int pos, n;      // position of the first one; tokens held
-    int base, end;   // cached tokens that the tile sees lie in [base, end)
-    int units;       // stages; a tile that sees nothing has one, which writes its zeros
-};
 // a tile, where it is, and a unit in it
 struct Found {
     Tile t;
@@ -120,17 +112,9 @@ struct Found {
 template <int ST>
 __device__ __forceinline__ Tile tile_of(const Params& p, int r, int tile) {
     const ChunkArgs& a = p.a;
-    Tile t;
     const int cap = a.pool > 0 ? a.columns * a.page : 0;
-    const int s0 = clamp(a.starts[r], 0, a.T), s1 = clamp(a.starts[r + 1], s0, a.T), i0 = tile * p.TB;
-    t.first = s0 + i0;
-    t.m = tile < 0 ? 0 : clamp(s1 - s0 - i0, 0, p.TB);  // below 0: places of rows before the first request's
-    t.pos = clamp(a.seq[r], 0, a.columns * a.page) + i0;
-    t.n = clamp(a.lens[r], 0, cap);
-    t.end = t.pos + t.m < t.n ? t.pos + t.m : t.n;
-    t.base = a.window > 0 && t.pos + 1 > a.window ? (t.pos + 1 - a.window) & ~15 : 0;
-    t.units = t.end > t.base ? (int)((uint32_t)(t.end - t.base + ST - 1) / ST) : 1;
-    return t;
+    const int s0 = clamp(a.starts[r], 0, a.T), s1 = clamp(a.starts[r + 1], s0, a.T);
+    return tile_at(s0, s1, clamp(a.seq[r], 0, a.columns * a.page), clamp(a.lens[r], 0, cap), tile, p.TB, a.window, ST);
 }
 
 // Request r's tiles take places from starts[r] / TB + r on: as many as it has
@@ -155,29 +139,6 @@ __device__ __forceinline__ int request_of_token(const ChunkArgs& a, int t) {
     }
     return lo;
 }
-
-// The units of all tiles in 2^log equal ranges, none of them empty.  A piece of a tile costs as
-// much beyond its units as a few of them: a cut less than `least` units from a
-// tile's end is moved there.  Ranges are at least four times as long, so that
-// at most one cut moves to each end.
-struct Ranges {
-    uint64_t units;
-    int log, least;
-    __device__ Ranges(uint64_t n, int l) : units(n), log(l) {
-        while (n >> log == 0) log--;
-        const uint64_t quarter = n >> (log + 2);
-        least = quarter < kLeastPiece ? (int)quarter : kLeastPiece;
-    }
-    __device__ uint64_t first(int w) const { return (units * (uint32_t)w) >> log; }
-    __device__ int of(uint64_t u) const {
-        int w = (int)((double)(u + 1) * (double)(1 << log) / (double)units);  // or one beside it
-        while (first(w) > u) w--;
-        while (first(w + 1) <= u) w++;
-        return w;
-    }
-    // where a cut `at` units into a tile of n goes
-    __device__ int cut(int at, int n) const { return at < least ? 0 : n - at < least ? n : at; }
-};
 
 // slot of the s-th part of a tile that starts in range w0: a range keeps the part
 // that its first units continue in slot 2 w, the one that its last units start in
@@ -312,11 +273,10 @@ struct Chunk {
 
     // The cache rows where the wave's parts of stages s0 + lane begin, tokens behind
     // the tile's last one taken as its run: 64 stages with one trip to the table
-    __device__ __forceinline__ void find(const ChunkArgs& a, const Tile& t, int r, int hk, int first_tok, int s0) {
+    __device__ __forceinline__ void find(const ChunkArgs& a, const Tile& t, int r, int hk, uint32_t first_tok, int s0) {
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int t0 = first_tok + (s0 + lane) * ST + w * NI * TI + i * LT;
-            const int tr = (uint32_t)t0 < (uint32_t)t.end ? t0 : (t.end - 1) & ~(LT - 1);
+            const int tr = or_last_run(t, first_tok + (uint32_t)(s0 + lane) * ST + (uint32_t)(w * NI * TI + i * LT), LT);
             const int col = div_by(tr, a.div);
             int pg = a.table[(int64_t)r * a.columns + col];
             pg = (uint32_t)pg < (uint32_t)a.pool ? pg : 0;
@@ -329,7 +289,7 @@ struct Chunk {
     // A stage's rows of keys (V: of values) into the slot at `slot` of their ring:
     // tokens from tb on, those past the tile's last one from its row
     template <bool V>
-    __device__ __forceinline__ void fill(const ChunkArgs& a, const Tile& t, int r, int hk, int tb, uint32_t slot) {
+    __device__ __forceinline__ void fill(const ChunkArgs& a, const Tile& t, int r, int hk, uint32_t tb, uint32_t slot) {
         const uint32_t dst = lds_at() + (V ? NS * kMat : 0) + slot;
         const uint32_t row_bytes = (uint32_t)(a.D * ES);
         const char* cache = static_cast<const char*>(V ? a.vc : a.kc);
@@ -342,14 +302,13 @@ struct Chunk {
                 const int i = j * TI / LT;
                 const char* from = cache + (uint64_t)(uint32_t)row_at[i] * row_bytes;
                 uint32_t at = c + (uint32_t)(ri + in) * row_bytes;
-                if (tb + ST > t.end) {
-                    const int t0 = tb + w * NI * TI + i * LT, tr = t0 < t.end ? t0 : (t.end - 1) & ~(LT - 1), last = t.end - 1 - tr;
+                if (!is_whole(t, tb, ST)) {
+                    const int last = t.end - 1 - or_last_run(t, tb + (uint32_t)(w * NI * TI + i * LT), LT);
                     at = c + (uint32_t)(ri + in < last ? ri + in : last) * row_bytes;
                 }
                 if (EASY || c < row_bytes) dma16(dst + j * 1024, from, at);
             } else {
-                int tok = tb + run * TI + ri;
-                tok = tok < t.end ? tok : t.end - 1;
+                const int tok = or_last(t, tb + (uint32_t)(run * TI + ri));
                 const int col = div_by(tok, a.div);
                 int pg = a.table[(int64_t)r * a.columns + col];
                 pg = (uint32_t)pg < (uint32_t)a.pool ? pg : 0;
@@ -373,7 +332,7 @@ struct Chunk {
         }
     }
     // the rows of stage s
-    __device__ __forceinline__ void next_rows(const ChunkArgs& a, const Tile& t, int r, int hk, int first_tok, int s) {
+    __device__ __forceinline__ void next_rows(const ChunkArgs& a, const Tile& t, int r, int hk, uint32_t first_tok, int s) {
         if constexpr (FORM != kLanes) {
             if ((s & 63) == 0 && s > 0) {
                 find(a, t, r, hk, first_tok, s);
@@ -397,11 +356,6 @@ struct Chunk {
         const int i = div_by(row, p.by_gt);
         return qt * p.GT + row - i * p.GT < p.a.G;
     }
-    __device__ __forceinline__ static void sees(const ChunkArgs& a, const Tile& t, int i, int& from, int& to) {
-        const int pos = t.pos + i;
-        from = a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0;
-        to = pos + 1 < t.n ? pos + 1 : t.n;
-    }
 
     __device__ __forceinline__ void load_q(const Params& p, const Tile& t, int hk, int qt) {
         const ChunkArgs& a = p.a;
@@ -418,16 +372,16 @@ struct Chunk {
             if (k % 16 == 15) __builtin_amdgcn_sched_barrier(0);
         }
         int from, to;
-        sees(a, t, i, from, to);
+        seen_by(t, i, a.window, from, to);
         lo = from;
         len = to > from ? to - from : 0;
     }
 
     // which of the 32 NB tokens from tb on have a page
-    __device__ __forceinline__ uint64_t pages_there(const ChunkArgs& a, const Tile& t, int r, int tb) const {
-        const int tok = tb + lane;
-        const bool in = lane < BT && tok < t.end;
-        const int pg = in ? a.table[(int64_t)r * a.columns + div_by(tok, a.div)] : -1;
+    __device__ __forceinline__ uint64_t pages_there(const ChunkArgs& a, const Tile& t, int r, uint32_t tb) const {
+        const uint32_t tok = tb + (uint32_t)lane;
+        const bool in = lane < BT && tok < (uint32_t)t.end;
+        const int pg = in ? a.table[(int64_t)r * a.columns + div_by((int)tok, a.div)] : -1;
         return __ballot((uint32_t)pg < (uint32_t)a.pool);
     }
 
@@ -509,14 +463,14 @@ struct Chunk {
 
     // the cap, and -infinity for tokens that the row does not see: those of a group's
     // part of a stage, from position tb on
-    __device__ __forceinline__ void mask(const ChunkArgs& a, Scores& x, const Tile& t, int r, int tb, bool holes) const {
+    __device__ __forceinline__ void mask(const ChunkArgs& a, Scores& x, const Tile& t, int r, uint32_t tb, bool holes) const {
         const int h = lane >> 5;
-        const int from = lo - tb - 4 * h;  // against the token's number without the lane's 4 h
+        const uint32_t from = (uint32_t)lo - tb - (uint32_t)(4 * h);  // against the token's number without the lane's 4 h
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                x.s[b][i] = (uint32_t)(32 * b + (i & 3) + 8 * (i >> 2) - from) < (uint32_t)len ? x.s[b][i] : -INFINITY;
+                x.s[b][i] = (uint32_t)(32 * b + (i & 3) + 8 * (i >> 2)) - from < (uint32_t)len ? x.s[b][i] : -INFINITY;
                 if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
         if (holes) {
@@ -703,13 +657,13 @@ struct Chunk {
     __device__ __forceinline__ void piece(const Tile& t, int r, int hk, int qt, int u0, int u1, int to, uint32_t* bad) {
         const Params& p = argument();
         const ChunkArgs& a = p.a;
-        const int first_tok = t.base + u0 * ST, last_tok = t.base + u1 * ST < t.end ? t.base + u1 * ST : t.end;
+        const uint32_t first_tok = stage_at(t, u0, ST), last_tok = stages_end(t, u1, ST);
         const bool any = last_tok > first_tok;
         // the table's entries, for the places of the stages and for pages that are none,
         // and the queries in one trip
         bool none = false;
         if (any) {
-            const int c0 = div_by(first_tok, a.div), c1 = div_by(last_tok - 1, a.div);
+            const int c0 = div_by((int)first_tok, a.div), c1 = div_by((int)last_tok - 1, a.div);
             for (int c = c0 + (int)threadIdx.x; c <= c1; c += NT)
                 none |= (uint32_t)a.table[(int64_t)r * a.columns + c] >= (uint32_t)a.pool;
             if constexpr (FORM != kLanes) find(a, t, r, hk, first_tok, 0);
@@ -723,8 +677,8 @@ struct Chunk {
         const int nu = any ? u1 - u0 : 0;
         auto fill_both = [&](int s, uint32_t slot) {
             next_rows(a, t, r, hk, first_tok, s);
-            fill<false>(a, t, r, hk, first_tok + s * ST, slot);
-            fill<true>(a, t, r, hk, first_tok + s * ST, slot);
+            fill<false>(a, t, r, hk, first_tok + (uint32_t)s * ST, slot);
+            fill<true>(a, t, r, hk, first_tok + (uint32_t)s * ST, slot);
         };
 #pragma unroll
         for (int s = 0; s < L; s++)
@@ -732,8 +686,8 @@ struct Chunk {
         const bool holes = __syncthreads_or(none);
         // the wave's rows: the first one's tokens and the last one's
         int head, lo0, hi0, lo1, hi1;
-        sees(a, t, token_of(p, t, rg * 32, qt, head), lo0, hi0);
-        sees(a, t, token_of(p, t, rg * 32 + 31, qt, head), lo1, hi1);
+        seen_by(t, token_of(p, t, rg * 32, qt, head), a.window, lo0, hi0);
+        seen_by(t, token_of(p, t, rg * 32 + 31, qt, head), a.window, lo1, hi1);
         const bool rows = rg * 32 < t.m * p.GT;
         m = kLowest;
         l = 0.f;
@@ -756,14 +710,14 @@ struct Chunk {
                 else wait_vm<0>();
                 barrier();
                 if (j + L < nu) fill_both(j + L, behind);
-                const int tb = first_tok + j * ST + kg * BT;
-                if (rows && tb < hi1 && tb + BT > lo0) {
+                const uint32_t tb = first_tok + (uint32_t)j * ST + (uint32_t)(kg * BT);
+                if (rows && is_seen(tb, BT, lo0, hi1)) {
                     Ahead f;
                     const uint32_t kat = key_at(here), vat = value_at(here);
                     begin(f, kat);
                     scores(x, f, kat, a.D);
                     if (!EASY && a.softcap > 0.f) limit(p, x);
-                    if (holes || tb < lo1 || tb + BT > hi0) mask(a, x, t, r, tb, holes);
+                    if (holes || !is_inside(tb, BT, lo1, hi0)) mask(a, x, t, r, tb, holes);
                     follow(x, c);
                     begin_values(f, vat);
                     weigh(x, c, wt);
@@ -774,9 +728,7 @@ struct Chunk {
             // steps in which the wave's rows see all of a stage and whole stages are filled
             int ja = 0, jb = 0;
             if (FORM != kLanes && rows && !holes) {
-                const int t0 = first_tok + kg * BT;
-                ja = lo1 > t0 ? (lo1 - t0 + ST - 1) / ST : 0;
-                jb = hi0 >= t0 + BT ? (hi0 - BT - t0) / ST + 1 : 0;
+                steps_inside(first_tok + (uint32_t)(kg * BT), BT, ST, lo1, hi0, ja, jb);
                 jb = jb < nu - 1 - L ? jb : nu - 1 - L;
             }
             for (int j = 0; j < nu; j++) {
@@ -878,7 +830,7 @@ struct Chunk {
                 int hd;
                 const int i = token_of(e, t, row, qt, hd);
                 const int64_t at = (int64_t)to * ROWS + row;
-                alone(e, t.first, t.pos, t.n, r, hk, hd, i, first_tok, last_tok, to >= 0 ? e.part_o + at * DP : nullptr, e.part_ml + at * 2);
+                alone(e, t.first, t.pos, t.n, r, hk, hd, i, (int)first_tok, (int)last_tok, to >= 0 ? e.part_o + at * DP : nullptr, e.part_ml + at * 2);
             }
         }
     }
