@@ -58,8 +58,9 @@ extern "C" {
  * does not see are never part of its result, whatever they hold; an infinite
  * value in one it sees is the channel's result, two opposite ones NaN (rows
  * with such values are computed again one by one, many times slower).  Scores, sums
- * and the running statistics are fp32; with 16-bit types exp(s - max), rounded to
- * the type, enters the product with v.
+ * and the running statistics are fp32; with 16-bit types exp(s - max) enters the
+ * product with v rounded to the type, or, of a request with at most 16 new tokens times
+ * heads / kv_heads (one that decodes), as two values of it, as in op_paged_attention.
  * head_dim: a multiple of 8, at most 256; heads a multiple of kv_heads;
  * num_pages * kv_heads * page_size and max_pages * page_size + tokens below 2^31,
  * and so is (tokens / n + requests) * (max_pages * page_size / 32 + 1), where n is
