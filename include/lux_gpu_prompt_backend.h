@@ -25,8 +25,9 @@
  * negative, free_count where above); each op writes the next head as counts[0].
  * Counts and free_head of one call are distinct buffers.  A request's table
  * entries behind ceil(its length / page_size) mean nothing.  Forks, releases and
- * compactions take up to 2^22 pages, 2^20 forks, and products of num_pages, or
- * max_pages, and page_size, and of requests and max_pages below 2^31 - 1.
+ * compactions take up to 2^22 pages, 2^20 forks, max_pages below 2^31 - 256, and
+ * products of num_pages, or max_pages, and page_size, and of requests and max_pages
+ * below 2^31 - 1.
  */
 #ifndef LUX_GPU_PROMPT_BACKEND_H
 #define LUX_GPU_PROMPT_BACKEND_H

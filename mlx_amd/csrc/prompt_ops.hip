@@ -59,13 +59,14 @@ int32_t* words(const HipContext* ctx, size_t& n) {
     return n ? reinterpret_cast<int32_t*>(static_cast<char*>(ctx->ws) + lxq::kWorkspaceWords) : nullptr;
 }
 
-// requests, table, pool and list that the records of pages in use have alike
+// requests, table, pool and list that the records of pages in use have alike.  A wave
+// looks at up to 256 columns at a time, in 31 bits
 template <class A>
 LuxBackendError pages_ok(const A* p) {
     if (p->requests < 0 || p->max_pages <= 0 || p->page_size <= 0 || p->num_pages < 0 || p->free_count < 0)
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     if (!rows_ok(1, p->page_size, p->num_pages) || !rows_ok(1, p->page_size, p->max_pages) ||
-        (int64_t)p->requests * p->max_pages >= (1ll << 31) - 1 || p->num_pages > (1 << 22))
+        (int64_t)p->requests * p->max_pages >= (1ll << 31) - 1 || p->num_pages > (1 << 22) || p->max_pages > INT32_MAX - 256)
         return LUX_BACKEND_ERROR_NOT_SUPPORTED;
     return LUX_BACKEND_OK;
 }
