@@ -71,8 +71,6 @@ __device__ __forceinline__ void block_sums(int (&v)[N], int (&all)[N], int (*par
 
 // --- fork -----------------------------------------------------------------------------
 
-constexpr int kNoEntry = -0x7fffffff - 1;
-
 // A wave: the table's entries of a fork that shares `full` pages of row s, four
 // columns a lane at a time
 __device__ __forceinline__ void fork_columns(const ForkArgs& a, int s, int d, int full) {
@@ -95,7 +93,8 @@ __device__ __forceinline__ void fork_columns(const ForkArgs& a, int s, int d, in
 // page for them, of which the forks before took those up to `at`.  `last`: the
 // source's entry
 struct Taken {
-    int entry;   // after the full pages' ones, or kNoEntry
+    int entry;   // after the full pages' ones, any number
+    bool rest;   // there is one
     int n;       // tokens that it holds
     bool there;  // a page was needed and there
 };
@@ -109,7 +108,7 @@ __device__ __forceinline__ Taken take_page(const ForkArgs& a, int f, int n, int 
         a.copy_src[f] = there ? last : -1;
         a.copy_dst[f] = page;
     }
-    return Taken{rest ? (take ? page : last) : kNoEntry, take && !there ? full * a.page : n, there};
+    return Taken{take ? page : last, rest, take && !there ? full * a.page : n, there};
 }
 __device__ __forceinline__ void fork_counts(const ForkArgs& a, int head, int taken, int shared, int out, int needed) {
     a.counts[0] = head + taken;
@@ -157,9 +156,9 @@ __global__ __launch_bounds__(1024) void fork_few_kernel(ForkArgs a) {
     if (made) a.lens[d] = t.n;
     if (f == 0) fork_counts(a, head, all[0], all[1], all[2], needed);
     if constexpr (ALL) {
-        if (t.entry != kNoEntry) a.table[(int64_t)d * a.columns + full] = t.entry;
+        if (t.rest) a.table[(int64_t)d * a.columns + full] = t.entry;
     } else if (f < a.F) {
-        a.ws[f] = full;
+        a.ws[f] = t.rest ? ~full : full;
         a.ws[a.F + f] = t.entry;
     }
 }
@@ -193,7 +192,7 @@ __global__ __launch_bounds__(1024) void fork_kernel(ForkArgs a) {
         const Taken t = take_page(a, f, made ? n : -1, full, last, head + needed, round, part);
         needed += round;
         if (f < a.F) {
-            a.ws[f] = full;
+            a.ws[f] = t.rest ? ~full : full;
             a.ws[a.F + f] = t.entry;
         }
         if (made) store_now(a.lens + d, t.n);
@@ -205,12 +204,12 @@ __global__ __launch_bounds__(1024) void fork_kernel(ForkArgs a) {
     if (tid == 0) fork_counts(a, head, all[0], all[1], all[2], needed);
 }
 
-// a wave per fork
+// a wave per fork: ws holds its full pages, below 0 (~full) where an entry follows them
 __global__ __launch_bounds__(256) void fork_table_kernel(ForkArgs a) {
     for (int64_t f = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); f < a.F; f += (int64_t)gridDim.x * 4) {
-        const int full = a.ws[f], entry = a.ws[a.F + f];
+        const int is = a.ws[f], entry = a.ws[a.F + f], full = is < 0 ? ~is : is;
         if (full > 0) fork_columns(a, a.src[f], a.dst[f], full);
-        if (entry != kNoEntry && (threadIdx.x & 63) == 0) a.table[(int64_t)a.dst[f] * a.columns + full] = entry;
+        if (is < 0 && (threadIdx.x & 63) == 0) a.table[(int64_t)a.dst[f] * a.columns + full] = entry;
     }
 }
 
