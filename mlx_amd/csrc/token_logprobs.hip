@@ -438,7 +438,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
             uint64_t best = 0;
             for (int i = tid; i < n; i += NT) {
                 const uint64_t x = entry_of(key_of(logit<T>(base, i)), from + i);
-                if (x < last && x > best) best = x;
+                if ((x < last || k == 0) && x > best) best = x;  // NaN in place 0 is all ones
             }
             best = wave_most(best);
             if (lane == 0) sh.most[w] = best;
