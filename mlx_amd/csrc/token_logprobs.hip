@@ -143,7 +143,7 @@ __device__ __forceinline__ void write_sums(const Params& p, int r, const Sums& t
     const float lse = fmaf(a.scale, t.top, log_sum);
     if (a.lse) a.lse[r] = lse;
     if (a.entropy) a.entropy[r] = none ? 0.f : high || nan ? __uint_as_float(0x7fc00000u) : fmaf(-kLn2, t.e / t.s, log_sum);
-    if (a.logprobs) a.logprobs[r] = none || !has_tok ? (nan ? t.top : -INFINITY) : high || nan ? fmaf(a.scale, x_tok, -lse) : (x_tok - t.top) * a.scale - log_sum;
+    if (a.logprobs) a.logprobs[r] = !has_tok || none ? -INFINITY : high || nan ? fmaf(a.scale, x_tok, -lse) : (x_tok - t.top) * a.scale - log_sum;
 }
 __device__ __forceinline__ float top_logprob(const LogprobArgs& a, const Sums& t, float x, float log_sum) {
     if (t.top == -INFINITY) return -INFINITY;

@@ -26,3 +26,22 @@ def test_nan_in_the_first_place(ctx, dtype, T, V):
     assert (got["top_ids"] == torch.tensor([0, 3, V - 1], dtype=torch.int32)).all()
     got = run_logprobs(ctx, dtype, torch.full_like(x, math.nan), torch.zeros(T, dtype=torch.int32), 64)
     assert (got["top_ids"] == torch.arange(64, dtype=torch.int32)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T", [2, 600])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_tokens_outside_of_rows_that_are_not_finite(ctx, dtype, T, what):
+    """-infinity for a token outside the vocabulary, whatever the row holds; NaN for one inside it where NaN is."""
+    x = rows(12, dtype, T, 9000)
+    x[:, 77] = what
+    tokens = torch.tensor([-1, 9000, 5, 77])[torch.arange(T) % 4].to(torch.int32)
+    got = run_logprobs(ctx, dtype, x, tokens, 3)["logprobs"]
+    inside = (tokens >= 0) & (tokens < 9000)
+    assert torch.isneginf(got[~inside]).all()
+    if math.isnan(what):
+        assert torch.isnan(got[inside]).all()
+    elif what > 0:
+        assert torch.isneginf(got[tokens == 5]).all() and torch.isnan(got[tokens == 77]).all()
+    else:
+        assert torch.isfinite(got[tokens == 5]).all() and torch.isneginf(got[tokens == 77]).all()
