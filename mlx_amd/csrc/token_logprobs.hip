@@ -33,6 +33,7 @@ constexpr int kRoom = 1024;     // logits that are ranked
 constexpr int kMostParts = 64;
 // r c up to which (x - r) c is taken as x c - r c: the rounding of r c is at most 4
 constexpr float kFar = 0x1p27f;
+constexpr float kNear = 4096.f;  // 2^-kNear is 0, and that of a few less: products by c are off by up to 8 there
 constexpr float kLn2 = 0.69314718055994531f;
 
 // order of logits: NaN above all, -0 as 0; 0 stands for no logit
@@ -337,10 +338,11 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
         t.s += sh.part[i][1];
         t.e += sh.part[i][2];
     }
-    // NaN, infinite and far logits, and rows of nothing else than far ones below 0:
-    // the sums once more
+    // NaN, infinite and far logits, and rows whose largest is far below 0, or so near
+    // to there that logits a thread left out as far ones (fresh) count beside it: the
+    // sums once more
     bool nan = false;
-    if (sh.odd || (all > -INFINITY && all * p.c <= -kFar)) {
+    if (sh.odd || (all > -INFINITY && all * p.c <= kNear - kFar)) {
         s = e = 0.f;
         for (int i = tid; i < n; i += NT) {
             const float x = logit<T>(base, i), y = fmaxf((x - all) * p.c, -1000.f), q = __builtin_amdgcn_exp2f(y);

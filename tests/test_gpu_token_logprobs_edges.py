@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from prompt_util import run_logprobs
+from prompt_util import logprobs_reference, run_logprobs
 from serving_util import BF16, F16, F32
 from test_gpu_token_logprobs import rows
 
@@ -45,3 +45,26 @@ def test_tokens_outside_of_rows_that_are_not_finite(ctx, dtype, T, what):
         assert torch.isneginf(got[tokens == 5]).all() and torch.isnan(got[tokens == 77]).all()
     else:
         assert torch.isfinite(got[tokens == 5]).all() and torch.isneginf(got[tokens == 77]).all()
+
+
+@pytest.mark.parametrize("T,V", [(1, 700), (1, 131072), (530, 9000)])
+@pytest.mark.parametrize("scale,far", [(1.0, 93032640), (0.7, 132903776), (0.7, 132903768)])
+def test_logits_around_the_far_ones(ctx, T, V, scale, far):
+    """Rows whose logits lie to both sides of -2^27 / (scale log2 e), where the sums change their reference: 8 is a step of f32.
+    Differences to the largest logit are exact, so only the terms of prompt_util.py that do not grow with the logits remain."""
+    for above in (8, 16, 32, 4000):
+        x = torch.full((T, V), -float(far))
+        x[:, V // 3] += above
+        x[:, V // 2:V // 2 + 3] += 8
+        tokens = torch.tensor([V // 3, 5, V // 2])[torch.arange(T) % 3].to(torch.int32)
+        got = run_logprobs(ctx, F32, x, tokens, 5, scale=scale)
+        want, _ = logprobs_reference(x, tokens, 5, scale)
+        # lse and the logits have few bits left at this size in 64 bits, too: from the differences instead
+        y = (x.double() - x.double().amax(-1, keepdim=True)) * float(torch.tensor(scale))
+        every = y - torch.logsumexp(y, -1, keepdim=True)
+        base = 2.0 ** -24 * (12 + V / 512 + 70 + math.log2(V) * 4)
+        for k, w in [("logprobs", every.gather(1, tokens.long()[:, None])[:, 0]), ("top_logprobs", every.gather(1, want["top_ids"].long()))]:
+            assert ((got[k].double() - w).abs() <= base + 2.0 ** -23 * w.abs()).all(), (k, above, got[k].flatten()[:5], w.flatten()[:5])
+        entropy = -(torch.exp(every) * every).sum(-1)
+        assert ((got["entropy"].double() - entropy).abs() <= base * (math.log2(V) + 2) + 2.0 ** -23 * entropy).all(), above
+        assert torch.equal(got["top_ids"], want["top_ids"])
