@@ -33,6 +33,7 @@ constexpr int kRoom = 1024;     // logits that are ranked
 constexpr int kMostParts = 64;
 // r c up to which (x - r) c is taken as x c - r c: the rounding of r c is at most 4
 constexpr float kFar = 0x1p27f;
+constexpr float kBehind = 8.f;  // by which a thread's maximum passes its r c
 constexpr float kNear = 4096.f;  // 2^-kNear is 0, and that of a few less: products by c are off by up to 8 there
 constexpr float kLn2 = 0.69314718055994531f;
 
@@ -248,21 +249,26 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
 #pragma unroll
         for (int j = 1; j < m; j++) mx = fmaxf(mx, x[j]);
         top = fmaxf(top, mx);
-        // a new r only where exp2 could pass 2^60
-        if (__any(fresh || fmaf(mx, p.c, -ref) > 60.f)) {
+        // A new r only where the maximum passes it by kBehind: what E / S leaves of the
+        // entropy when both are moved to the maximum is off by the roundings of that
+        // distance (with 60 bf16 rows were off by 2.4e-7 of it, with 8 by 6e-8, as with 2)
+        if (__any(fresh || fmaf(mx, p.c, -ref) > kBehind)) {
             const float to = mx * p.c;
-            if ((fresh || to - ref > 60.f) && fabsf(to) < kFar) {
+            if ((fresh || to - ref > kBehind) && fabsf(to) < kFar) {
                 if (!fresh) move(s, e, ref - to);
                 ref = to;
                 fresh = false;
             }
         }
+        float vs = 0.f, ve = 0.f;  // the vector's sums by themselves: fewer roundings at the size of all
 #pragma unroll
         for (int j = 0; j < m; j++) {
             const float y = fmaf(x[j], p.c, -ref), q = __builtin_amdgcn_exp2f(y);
-            s += q;
-            e = fmaf(q, fmaxf(y, -1000.f), e);  // not 0 times -infinity
+            vs += q;
+            ve = fmaf(q, fmaxf(y, -1000.f), ve);  // not 0 times -infinity
         }
+        s += vs;
+        e += ve;
     };
     constexpr int kU = 4;
     int v = tid;

@@ -68,3 +68,37 @@ def test_logits_around_the_far_ones(ctx, T, V, scale, far):
         entropy = -(torch.exp(every) * every).sum(-1)
         assert ((got["entropy"].double() - entropy).abs() <= base * (math.log2(V) + 2) + 2.0 ** -23 * entropy).all(), above
         assert torch.equal(got["top_ids"], want["top_ids"])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T", [1, 530])
+def test_entropy_of_rows_with_one_far_above(ctx, dtype, T):
+    """One logit far above all others, which its thread saw first.  The sum of exps about the largest is 1 and some 10^-5; it is
+    rounded at the size of 1, to 2^-24, in up to 8 additions of a vector, 5 of a thread, 6 of a wave, 8 of the block, 6 of the
+    parts and twice in its logarithm: 35 times.  The second sum is some 10^-4."""
+    for turn in range(1 if T > 1 else 20):
+        x = torch.zeros(T, 9000)
+        x[:, 4100] = 20.0 + (torch.arange(T) + turn) * (25.0 / (T if T > 1 else 20))
+        x = x.to({F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16}[dtype])
+        tokens = torch.zeros(T, dtype=torch.int32)
+        got = run_logprobs(ctx, dtype, x, tokens, 1)
+        want = logprobs_reference(x, tokens, 1, 1.0)[0]["entropy"]
+        off = (got["entropy"].double() - want).abs()
+        assert (off <= 35 * 2.0 ** -24 + 2.0 ** -20 * want).all(), f"{turn}: off by {float(off.max()):.3g}"
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T", [1, 530])
+def test_entropy_of_a_thread_with_one_far_above(ctx, dtype, T):
+    """The same where all other threads have nothing: one addition of all is rounded, at the size of 1, and the logarithm twice."""
+    type_, E = {F32: (torch.float32, 4), F16: (torch.float16, 8), BF16: (torch.bfloat16, 8)}[dtype]
+    for turn in range(1 if T > 1 else 20):
+        x = torch.full((T, 9000), -math.inf)
+        x[:, 3 * E:4 * E] = 0.0                 # thread 3's first vector
+        x[:, 512 * E + 3 * E + 1] = 25.0 + (torch.arange(T) + turn) * (16.0 / (T if T > 1 else 20))  # in its second
+        x = x.to(type_)
+        tokens = torch.zeros(T, dtype=torch.int32)
+        got = run_logprobs(ctx, dtype, x, tokens, 1)
+        want = logprobs_reference(x, tokens, 1, 1.0)[0]["entropy"]
+        off = (got["entropy"].double() - want).abs()
+        assert (off <= 3 * 2.0 ** -24 + 2.0 ** -20 * want).all(), f"{turn}: off by {float(off.max()):.3g}"
