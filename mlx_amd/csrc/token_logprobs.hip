@@ -403,7 +403,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(Params p, int first) {
             const int each = (vectors + NT - 1) / NT, items = sh.threads * each;
             for (int x0 = tid; x0 < items; x0 += NT) {
                 const int which = (int)((uint32_t)x0 / (uint32_t)each), i = sh.who[which] + (x0 - which * each) * NT;
-                if (i < vectors) list(*reinterpret_cast<const u4h*>(base + (int64_t)i * 16), i);
+                if (i < vectors) list(u4(*reinterpret_cast<const u4h*>(base + (int64_t)i * 16)), i);
             }
         }
         for (int i = behind + tid; i < n; i += NT) {
