@@ -83,7 +83,9 @@ struct Ranges {
         least = quarter < kLeastPiece ? (int)quarter : kLeastPiece;
     }
     LXQ_BOTH uint64_t first(int w) const { return (units * (uint32_t)w) >> log; }
+    // the range of unit u; of one behind all (starts that decrease lay tiles there) the last
     LXQ_BOTH int of(uint64_t u) const {
+        if (u >= units) return (1 << log) - 1;
         int w = (int)((double)(u + 1) * (double)(1 << log) / (double)units);  // or one beside it
         while (first(w) > u) w--;
         while (first(w + 1) <= u) w++;

@@ -106,3 +106,12 @@ def test_cuts(program):
     for (n, log, u), (cut, w, lo, hi) in ask(program, "cuts", every):
         assert cut == min(log, n.bit_length() - 1)
         assert 0 <= w < 2 ** cut and lo == n * w >> cut and hi == n * (w + 1) >> cut and lo <= u < hi, (n, log, u)
+
+
+def test_units_behind_all(program):
+    """Starts that decrease, which no call may have, lay tiles behind the last unit: their parts are taken for the last
+    range's, so that none is looked for behind the workspace."""
+    rng = random.Random(3)
+    every = [(n, log, n + more) for n in (1, 3, 256, 1000, 2 ** 31 - 1) for log in (0, 3, 8) for more in (0, 1, 100, 2 ** 31, rng.randrange(2 ** 40))]
+    for (n, log, u), (cut, w, lo, hi) in ask(program, "cuts", every):
+        assert w == 2 ** cut - 1 and hi == n, (n, log, u)
