@@ -63,7 +63,6 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLowest = -0x1.fffffep127f;  // the maximum of no score: no finite score is below
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
-constexpr float kLeast = 0x1p-126f;
 
 // a tile that starts in a range and ends behind it: its parts, tokens and heads
 struct Cut {
@@ -84,6 +83,10 @@ struct Params {
     float* part_ml;   // [2 P, rows, 2]
     Cut* cuts;        // [P]
 };
+
+// the weight of x, which never falls to 0 before an infinite x; before a finite one it
+// does: as small as it is, 2^-126 of a large x may be more than the result
+__device__ __forceinline__ float weight_of(float w, float x) { return fabsf(x) == INFINITY ? fmaxf(w, 0x1p-126f) : w; }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 // (address space 4: scalar loads)
@@ -617,7 +620,7 @@ struct Chunk {
     // One row over the cached tokens of [from, to), by one wave and token by token:
     // for rows that a value which is not finite reached.  In the tile's products it
     // reaches rows that do not see it too (0 times infinity); here each row meets
-    // its own tokens alone.  A weight never falls to 0 before an infinite value.
+    // its own tokens alone.
     __device__ __forceinline__ static void alone(const Params& p, int first, int pos, int n, int r, int hk, int head, int i, int from, int to,
                                               float* part_o, float* part_ml) {
         const ChunkArgs& a = p.a;
@@ -650,11 +653,11 @@ struct Chunk {
             if (a.softcap > 0.f) s = p.cap * tanh_of(s * p.c);
             const float was = m;
             m = fmaxf(m, s);
-            const float f = fmaxf(__builtin_amdgcn_exp2f((was - m) * c), kLeast);
+            const float f = __builtin_amdgcn_exp2f((was - m) * c);
             const float w = __builtin_amdgcn_exp2f(fmaf(s, c, -fmaxf(m * c, -0x1p126f)));
             l = fmaf(l, f, w);
 #pragma unroll
-            for (int j = 0; j < NV; j++) acc[j] = fmaf(fabsf(v[j]) == INFINITY ? fmaxf(w, kLeast) : w, v[j], acc[j] * f);
+            for (int j = 0; j < NV; j++) acc[j] = fmaf(weight_of(w, v[j]), v[j], acc[j] * weight_of(f, acc[j]));
         }
         const float up = 1.f / kDown, top = fmaxf(m * c, -0x1p126f);
         const int tok = first + i, hd = hk * a.G + head;
@@ -1053,11 +1056,10 @@ __global__ __launch_bounds__(512) void join_kernel(Params p) {
             for (int k = 1; k < 64; k *= 2) mx = fmaxf(mx, __shfl_xor(mx, k));
             const float to = fmaxf(top, mx), f0 = __builtin_amdgcn_exp2f(top - to);
             top = to;
-            // a part's weight never falls to 0: its sum may be infinite
-            const float wgt = lane < n ? fmaxf(__builtin_amdgcn_exp2f(tm - to), kLeast) : 0.f;
+            const float wgt = lane < n ? __builtin_amdgcn_exp2f(tm - to) : 0.f;
             sum = sum * f0 + wave_sum(lane < n ? wgt * __uint_as_float(ml[1]) : 0.f);
 #pragma unroll
-            for (int j = 0; j < NV; j++) acc[j] *= fmaxf(f0, kLeast);
+            for (int j = 0; j < NV; j++) acc[j] *= weight_of(f0, acc[j]);
             for (int s = 0; s < n; s += kB) {
                 if (s > 0) load(s);
 #pragma unroll
@@ -1065,7 +1067,7 @@ __global__ __launch_bounds__(512) void join_kernel(Params p) {
                     if (s + b >= n) break;
                     const float f = lane_f(wgt, s + b);
 #pragma unroll
-                    for (int j = 0; j < NV; j++) acc[j] = fmaf(f, v[b][j], acc[j]);
+                    for (int j = 0; j < NV; j++) acc[j] = fmaf(weight_of(f, v[b][j]), v[b][j], acc[j]);
                 }
             }
         }

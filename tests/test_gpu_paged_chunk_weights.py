@@ -65,3 +65,29 @@ def test_every_value_counts_once(ctx, dtype, new, held, H, Hk, D, page, window):
     assert torch.equal(torch.isneginf(lse), torch.isneginf(want_lse.float()))
     some = torch.isfinite(want_lse)
     assert ((lse.double() - want_lse)[some].abs() <= 4 * 2.0 ** -24 * (1 + want_lse[some].abs())).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,Hk", [(1, 1), (64, 4)])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_large_values_of_no_weight(ctx, dtype, H, Hk, infinite):
+    """Values of 3e37 whose weights are e^-900, in other parts of the row than those that count, and in rows that are computed
+    one by one: the result is that of the tokens that count, 1, with their sums' and its own roundings."""
+    q, kc, vc, table, starts, seq, lens = problem(21, dtype, [2], [3000], H, Hk, 64, 16)
+    q, kc = torch.zeros_like(q), torch.zeros_like(kc)
+    q.view(2, H, 64)[:, :, 0] = 1.0
+    line = torch.full((3008,), -1000.0)
+    line[:4], line[2992:] = -900.0, 0.0
+    value = torch.ones(3008)
+    value[:4] = 3e37
+    kc[table[0].long(), :, :, 0] = line.view(-1, 1, 16).to(kc.dtype)
+    vc[table[0].long()] = value.view(-1, 1, 16, 1).to(vc.dtype)
+    if infinite:
+        vc[int(table[0, 60]), :, 3, 5] = float("inf")
+    out, lse = run_chunk(ctx, dtype, q, kc, vc, table, starts, seq, lens, H, scale=1.0)
+    out = out.double().view(2, H, 64)
+    if infinite:
+        assert (out[:, :, 5] == float("inf")).all()
+        out[:, :, 5] = 1.0
+    assert ((out - 1).abs() <= ROUND[dtype] + (64 + 16) * 2.0 ** -24).all(), float((out - 1).abs().max())
+    assert ((lse.double() - torch.log(torch.tensor([[9.0], [10.0]], dtype=torch.float64))).abs() <= 16 * 2.0 ** -24).all()
