@@ -10,7 +10,9 @@
  * the probabilities (reference include/lux/gpu/backend_plugin.h:82-382).
  * Records, buffers, the cache's layout, strides and errors are those of the
  * serving table: nothing is remembered between calls, all ops are asynchronous
- * on the context's stream and make no allocation; NULL handle, impossible size
+ * on the context's stream and make no allocation, but for the 102 MB of workspace
+ * that the first chunk attention of a context allocates (captured or not) and the
+ * context keeps (OUT_OF_MEMORY where there are none); NULL handle, impossible size
  * or stride, wrong struct_size, a buffer too small, an output over an input or
  * another output (but where an op allows it) -> INVALID_ARGUMENT; a dtype,
  * head_dim, pool or count outside the stated ones -> NOT_SUPPORTED; HIP launch

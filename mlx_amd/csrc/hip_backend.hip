@@ -70,10 +70,6 @@ LuxBackendContext* hip_create_context(int device_index) {
     ctx->ws = zeroed(lxq::kSplitWorkspaceBytes);
     ctx->ws_bytes = ctx->ws ? lxq::kSplitWorkspaceBytes : 0;
     ctx->counts = zeroed(kCountWords * 4);
-    if (hipMalloc(&ctx->parts, lxq::kChunkPartBytes) != hipSuccess) {
-        (void)hipGetLastError();
-        ctx->parts = nullptr;
-    }
     return reinterpret_cast<LuxBackendContext*>(ctx);
 }
 

@@ -29,8 +29,8 @@ struct HipContext {
     // parts of a row of logits (one per row), zero
     // between launches; without them neither is split
     void* counts = nullptr;
-    // partial results of the chunk attention's split tiles; like ws, used only
-    // by work on `stream`
+    // partial results of the chunk attention's split tiles, allocated by the first
+    // one; like ws, used only by work on `stream`
     void* parts = nullptr;
 };
 constexpr int kCountWords = 2048;

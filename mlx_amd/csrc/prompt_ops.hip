@@ -7,6 +7,22 @@ using namespace lxh;
 
 namespace {
 
+// The memory for partial results of the context's chunk attentions: programs without
+// prompts go without it.  The first call may be one that is captured: an allocation is
+// no part of a graph, and relaxed capture lets it pass.
+char* chunk_parts(HipContext* ctx) {
+    if (!ctx->parts) {
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) return nullptr;
+        if (hipMalloc(&ctx->parts, lxq::kChunkPartBytes) != hipSuccess) {
+            (void)hipGetLastError();
+            ctx->parts = nullptr;
+        }
+        (void)hipThreadExchangeStreamCaptureMode(&mode);
+    }
+    return static_cast<char*>(ctx->parts);
+}
+
 LuxBackendError op_paged_chunk_attention(LuxBackendContext* c, const lux_paged_chunk_args* p) {
     HipContext* ctx = C(c);
     if (!ctx || !p || p->struct_size != sizeof(*p)) return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
@@ -47,9 +63,10 @@ LuxBackendError op_paged_chunk_attention(LuxBackendContext* c, const lux_paged_c
     a.page = p->page_size; a.pool = p->num_pages; a.columns = p->max_pages; a.window = p->window;
     a.dtype = p->dtype; a.scale = p->scale; a.softcap = p->softcap;
     a.div = lxq::DivBy(p->page_size);
-    a.ws = static_cast<char*>(ctx->parts);
     a.cus = ctx->compute_units;
     if (hipSetDevice(ctx->device) != hipSuccess) return LUX_BACKEND_ERROR_DEVICE_LOST;
+    a.ws = chunk_parts(ctx);
+    if (!a.ws) return LUX_BACKEND_ERROR_OUT_OF_MEMORY;
     return map_status(lxq::launch_paged_chunk(a, ctx->stream));
 }
 
