@@ -548,10 +548,14 @@ unsigned blocks_of(int64_t items, int per, int most) {
 
 LuxStatus launch_paged_fork(const ForkArgs& a, hipStream_t st) {
     if (!a.ws || (size_t)a.F * 2 > a.ws_words) return LuxStatus::NotSupported;
-    // A wave of the one block takes its forks one after the other, 2 us each; a second
-    // launch costs 3 us and has a wave for each: 24 forks (with 24 KB pages copied and
-    // given back again) take 18.8 us against 21.5, 224 forks 177 against 172.
-    if (a.F <= 64 && (int64_t)a.F * a.columns <= 16384) {
+    // A wave of the one block takes its forks one after the other, in rounds of 256
+    // columns; a second launch costs 2 to 3 us and has a wave for each.  Rows that are full,
+    // one launch against two: 16 forks of 64 columns 5.6 us, 8.6; 16 of 256 8.0, 9.0; 24 of 257
+    // 11.1, 9.4; 32 of 256 14.5, 9.2; 64 of 256 28, 9.3; 64 of 32 7.5, 8.0; 128 of 32 12, 9.1.  A
+    // table is wider than most of its rows are long: half full on average, with the copies
+    // and the release behind, 24 of 257 take 20.9 us, 21.7; 32 of 257 22.0 both; 48 of 257
+    // 24.2, 22.3; 64 of 129 22.4, 22.8; 16 of 1025 31.8, 28.3.
+    if (a.F <= 64 && (int64_t)a.F * a.columns <= 8192) {
         hipLaunchKernelGGL(fork_few_kernel<true>, dim3(1), dim3(1024), 0, st, a);
         return status();
     }
