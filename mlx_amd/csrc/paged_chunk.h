@@ -189,19 +189,6 @@ __device__ __forceinline__ float half_max(float v) {
     return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 
-// tanh(y) from z = 2 y log2 e: 1 - 2 / (1 + exp2(z)), off by 2^-22 at most.  Where y
-// is small that is a large share of it, and times a large cap a large part of the
-// score: there the series up to y^11, whose next term is below 2^-28 of y at 0.3.
-__device__ __forceinline__ float tanh_of(float z) {
-    const float far = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z)), -2.f, 1.f);
-    const float y = z * (0.5f * kLn2), q = y * y;
-    float near = fmaf(q, -1382.f / 155925.f, 62.f / 2835.f);
-    near = fmaf(q, near, -17.f / 315.f);
-    near = fmaf(q, near, 2.f / 15.f);
-    near = fmaf(q, near, -1.f / 3.f);
-    return fabsf(y) < 0.3f ? fmaf(y * q, near, y) : far;
-}
-
 template <int T>
 __device__ __forceinline__ f16v mfma(const u4& x, const u4& y, f16v c) {
     if constexpr (T == DT_F16) {
