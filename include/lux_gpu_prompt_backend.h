@@ -46,8 +46,9 @@ extern "C" {
  * Attention of a chunk of new tokens per request over the request's cached
  * tokens, the chunk's own among them (append comes first).  Rows of q from
  * token_starts[r] to token_starts[r + 1] are request r's, in order (any
- * number, 0 and 1 included); the i-th is at position p = seq_lens[r] + i.  A
- * plan's token_starts, seq_lens (its input) and kv_lens are these arrays.
+ * number, 0 and 1 included); the i-th is at position p = seq_lens[r] + i, with
+ * seq_lens[r] cut to [0, max_pages * page_size].  A plan's token_starts, seq_lens
+ * (its input) and kv_lens are these arrays.
  * token_starts does not decrease; rows of q below token_starts[0] and from
  * token_starts[requests] on are no request's: out and lse stay there as they were.
  * Head j reads the keys and values of head j / (heads / kv_heads).  Over the
@@ -211,7 +212,10 @@ typedef struct lux_paged_copy_args {
  *   is larger than all and equal to itself)
  * A row of -infinity alone gives lse = -infinity, logprobs -infinity, entropy 0;
  * +infinity or NaN in a row makes its lse that and NaN what the formulas make NaN.
- * Sums and outputs are fp32.  A NULL output is left out (tokens may be NULL with
+ * Sums and outputs are fp32.  Rows with few finite logits or many alike, where
+ * more than 1024 may be among the largest, and rows with NaN are read `top` times more:
+ * 4096 rows of 131072 in bf16 with 10 finite logits each take 11 ms for 20
+ * alternatives and 33 for 64, with 1 % of them finite 0.22 and 0.43.  A NULL output is left out (tokens may be NULL with
  * logprobs; top_ids and top_logprobs each where top is 0 or it is not wanted).
  * vocab: at least top, at most 2^24; top: 0 to 64.
  */

@@ -28,18 +28,20 @@
 // takes a run of ranges, so that its L2 holds the keys that its blocks share.
 //
 // What bounds it, and what it measured (32 heads on 8 of 128 channels, bf16):
-//   16384 tokens of one request: 2.50 ms, 880 TFLOP/s.  A stage of 64 tokens costs the
-//     two waves of a SIMD 64 MFMAs of 32 cycles, 57 % of 3600 cycles; the rest is the softmax, and
-//     at that rate the card's power holds the clock near 1.5 GHz (a large product of
-//     the library reaches 1110 to 1270 TFLOP/s).  The loop of whole, unmasked stages
-//     (kPlain, kRuns) brought 2.74 to 2.50: rows of the table looked up for 64 stages
-//     at a time (222 scalar instructions per stage and wave became 36), LDS reads
-//     kept three or four products ahead by fences.  Two groups of waves in opposite
-//     phases, scores of the next stage before the weights of this one, 64 rows per
-//     wave and 32-token stages were tried and were no faster.
-//   4 chunks of up to 512 tokens among 64 requests of up to 8192: 257 us, 4.2 TB/s of
+//   16384 tokens of one request: 2.48 ms, 890 TFLOP/s (a large product of the library
+//     reaches 1110 to 1270).  The MFMAs are busy 57 % of the cycles in which a CU has
+//     work, the rest of which is the softmax, and 44 % of the kernel's, at 1.8 GHz: a
+//     fifth of the CUs' time is idle, as ranges are cut by stages alone and the first
+//     ranges of a head hold dozens of short tiles, each with a start and an end of
+//     two to three stages' time (they end 10 % behind the mean).  The loop of whole,
+//     unmasked stages (kPlain, kRuns) brought 2.74 to 2.50: rows of the table looked up
+//     for 64 stages at a time (222 scalar instructions per stage and wave became 36),
+//     LDS reads kept three or four products ahead by fences.  Two groups of waves in
+//     opposite phases, scores of the next stage before the weights of this one, 64 rows
+//     per wave and 32-token stages were tried and were no faster.
+//   4 chunks of up to 512 tokens among 64 requests of up to 8192: 259 us, 4.2 TB/s of
 //     the cache; reading it, with 4.7 TB/s for a large copy, is what remains.
-//   64 new tokens on 4096 (f16): 25 us, of which the transfers and products of a
+//   64 new tokens on 4096 (f16): 25.5 us, of which the transfers and products of a
 //     block's four stages are 5; the start (lengths, table, queries), the meeting of
 //     the four groups and the second launch are chains of trips to memory.
 #pragma once
@@ -1129,10 +1131,11 @@ LuxStatus launch_t(const ChunkArgs& a, hipStream_t st) {
     // of up to 512 among 64 requests 260 us, against 313 with wide tiles and 288 with
     // narrow ones; 16384 tokens of one request 3.1 ms against 2.5.
     const bool padded = (int64_t)a.T * a.G < 192 * (int64_t)a.R;
-    // 192 channels: eight waves and stages of 32 tokens (8192 tokens on 2048, bf16: 940
-    // TFLOP/s; four waves and stages of 64 tokens 651, as one wave per SIMD leaves the
+    // 192 channels: eight waves and stages of 32 tokens (8192 tokens on 2048, bf16: 945 to
+    // 980 TFLOP/s; four waves and stages of 64 tokens 636, as one wave per SIMD leaves the
     // matrix cores idle in its softmax).  256 channels do not leave the registers for
-    // a second wave: 817.
+    // a second wave: 805 to 860, MFMAs busy 40 % of a working CU's cycles.  Both widths'
+    // few and padded calls take tiles of 64 rows, two groups of waves.
     if constexpr (T == DT_F32) {
         if (a.D <= 64) return few || padded ? launch_page<T, 64, 2, 4, 32, 2>(p, st) : launch_page<T, 64, 8, 1, 32, 3>(p, st);
         if (a.D <= 96) return few || padded ? launch_page<T, 96, 4, 2, 32, 2>(p, st) : launch_page<T, 96, 8, 1, 32, 3>(p, st);

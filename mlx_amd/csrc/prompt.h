@@ -8,8 +8,8 @@
 namespace lxq {
 
 // partial results of the chunk attention: two per range, one range per CU, each up
-// to 256 rows of 128 channels or 128 of 256 and their maxima and sums; and a
-// record per range
+// to 256 rows of 192 channels (or of fewer, or 128 of 256) and their maxima and
+// sums; and a record per range
 constexpr int kChunkRanges = 256;
 constexpr size_t kChunkPartBytes = (size_t)kChunkRanges * (2 * 256 * (192 + 2) * 4 + 32);
 
@@ -42,7 +42,7 @@ struct ReleaseArgs {
     int32_t *shares, *free_pages, *kv, *counts;
     int R, columns, page, pool, free_count;
     DivBy div;
-    int32_t* ws;  // a word per 4096 pages
+    int32_t* ws;  // 512 words, and one per 4096 pages
     size_t ws_words;
 };
 LuxStatus launch_paged_release(const ReleaseArgs& a, hipStream_t st);
@@ -52,7 +52,7 @@ struct CompactArgs {
     int32_t *table_out, *shares_out, *free_pages, *copy_src, *copy_dst, *counts;
     int R, columns, page, pool, free_count, limit, max_moves;
     DivBy div, by_columns;
-    int32_t* ws;
+    int32_t* ws;  // a bit and a word per page
     size_t ws_words;
 };
 LuxStatus launch_paged_compact(const CompactArgs& a, hipStream_t st);

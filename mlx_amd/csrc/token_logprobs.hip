@@ -11,13 +11,15 @@
 // = 20): these are read again, out of the cache, and ranked by counting.
 //
 // Few rows are cut into parts, a block each; the last block of a row joins them.
-// 4096 rows of 131072 bf16 logits: 193 us, 5.6 TB/s of the one read (a large copy
-// moves 4.7); 8 rows of f32: 11.5 us, of which the read is 1.3, the launch 2.5, and the rest
+// 4096 rows of 131072 bf16 logits: 194 us, 5.5 TB/s of the one read (a large copy
+// moves 4.7); 8 rows of f32: 11.4 us, of which the read is 1.3, the launch 2.5, and the rest
 // reductions over the block and trips to the counter and to the other parts' results.
 //
 // Rows in which that goes wrong (more logits from the bound on than are ranked, as
 // where most are -infinity, or NaN) are finished by a search, one largest logit
-// after the other.
+// after the other, a reading of the row each: those 4096 rows with 10 finite logits take
+// 11.1 ms for the 20 largest (0.22 with 1 % finite), 33.5 for 64 (0.45); the 8 rows 51
+// us and 955.
 #include "prompt.h"
 #include "serving_device.h"
 
