@@ -1115,8 +1115,8 @@ LuxStatus launch_t(const ChunkArgs& a, hipStream_t st) {
     Params p = {};
     p.a = a;
     const float s = a.softcap > 0.f ? 2.f * kLog2e * a.scale / a.softcap : kLog2e * a.scale;
-    // c above 0, so that c times a masked score is -infinity
-    p.c = s < 0.f ? -s : s > 0.f ? s : 0x1p-149f;
+    // c above 0, so that c times a masked score is -infinity, and finite, so that c times a score of 0 is 0
+    p.c = fminf(s < 0.f ? -s : s > 0.f ? s : 0x1p-149f, -kLowest);
     p.flip = s < 0.f ? (T == DT_F32 ? 0x80000000u : 0x80008000u) : 0u;
     p.cap = a.softcap * kLog2e;
     // Tiles of 64 rows (f32 of 128 channels: 128), whose stages are shared out among

@@ -91,3 +91,17 @@ def test_large_values_of_no_weight(ctx, dtype, H, Hk, infinite):
         out[:, :, 5] = 1.0
     assert ((out - 1).abs() <= ROUND[dtype] + (64 + 16) * 2.0 ** -24).all(), float((out - 1).abs().max())
     assert ((lse.double() - torch.log(torch.tensor([[9.0], [10.0]], dtype=torch.float64))).abs() <= 16 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("H,Hk", [(4, 2), (64, 4)])
+@pytest.mark.parametrize("scale,softcap", [(3e38, 0.0), (-3e38, 0.0), (1e10, 2.0 ** -100), (-3e38, 2.0 ** -100), (3e38, 30.0)])
+def test_factors_that_pass_32_bits(ctx, dtype, H, Hk, scale, softcap):
+    """Scores of 0 stay 0 where the factor by log2 e, or by the cap, passes f32: equal weights, exact sums."""
+    q, kc, vc, table, starts, seq, lens = problem(22, dtype, [250, 1], [20, 300], H, Hk, 64, 16)
+    q, vc = torch.zeros_like(q), (vc * 2).round()
+    out, lse = run_chunk(ctx, dtype, q, kc, vc, table, starts, seq, lens, H, scale=scale, softcap=softcap)
+    want, want_lse, _, _ = chunk_reference(q, kc, vc, table, starts, seq, lens, H, scale=1.0, dtype=dtype)
+    off = (out.double().view(want.shape) - want).abs()
+    assert (off <= (ROUND[dtype] + 3 * 2.0 ** -24) * want.abs() + (2.0 ** -25 if dtype == F16 else 0)).all()
+    assert ((lse.double() - want_lse).abs() <= 4 * 2.0 ** -24 * (1 + want_lse.abs())).all()
