@@ -479,7 +479,7 @@ LuxStatus launch_t(const LogprobArgs& a, hipStream_t st) {
     Params p = {};
     p.a = a;
     const double c = (double)a.scale * 1.4426950408889634;
-    p.c = (float)c;
+    p.c = c < 0x1.fffffep127 ? (float)c : 0x1.fffffep127f;  // finite: 0 times it is 0
     p.d = p.c > 0x1p-126f ? (float)(c / p.c - 1.) : 0.f;
     // two blocks per CU; parts of at least 4096 logits
     int parts = a.T > 0 ? 2 * a.cus / a.T : 1;

@@ -102,3 +102,18 @@ def test_entropy_of_a_thread_with_one_far_above(ctx, dtype, T):
         want = logprobs_reference(x, tokens, 1, 1.0)[0]["entropy"]
         off = (got["entropy"].double() - want).abs()
         assert (off <= 3 * 2.0 ** -24 + 2.0 ** -20 * want).all(), f"{turn}: off by {float(off.max()):.3g}"
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T,V", [(1, 700), (1, 20000), (530, 9000)])
+def test_scales_that_pass_32_bits_by_log2_e(ctx, dtype, T, V):
+    """Logits of 0, and of -infinity, are what they are by any scale: V / 2 equal ones."""
+    x = rows(13, dtype, T, V) * 0
+    x[:, ::2] = -math.inf
+    tokens = (torch.arange(T) % 2).to(torch.int32)
+    got = run_logprobs(ctx, dtype, x, tokens, 3, scale=3e38)
+    want = math.log(V // 2)
+    bound = 2.0 ** -24 * (12 + V / 512 + 70 + math.log2(V) * 4)
+    assert ((got["lse"].double() - want).abs() <= bound).all() and ((got["entropy"].double() - want).abs() <= bound * (math.log2(V) + 2)).all()
+    assert torch.isneginf(got["logprobs"][::2]).all() and ((got["logprobs"][1::2].double() + want).abs() <= bound).all()
+    assert (got["top_ids"] == torch.tensor([1, 3, 5], dtype=torch.int32)).all() and ((got["top_logprobs"].double() + want).abs() <= bound).all()
