@@ -18,7 +18,7 @@
 // Rows in which that goes wrong (more logits from the bound on than are ranked, as
 // where most are -infinity, or NaN) are finished by a search, one largest logit
 // after the other, a reading of the row each: those 4096 rows with 10 finite logits take
-// 11.1 ms for the 20 largest (0.22 with 1 % finite), 33.5 for 64 (0.45); the 8 rows 51
+// 11.1 ms for the 20 largest (0.22 with 1 % finite), 33.5 for 64 (0.43); the 8 rows 51
 // us and 955.
 #include "prompt.h"
 #include "serving_device.h"
